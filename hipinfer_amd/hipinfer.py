@@ -80,6 +80,17 @@ int hi_flash_prefill(ptr q, int ldq, ptr kc, ptr vc, int max_seq, ptr out, int l
                      int D, ptr stream);
 int hi_flash_prefill_lse(ptr q, int ldq, ptr kc, ptr vc, int max_seq, ptr out, int ldo, int T, int p0, int Hq,
                          int Hkv, int D, ptr lse, ptr stream);
+int hi_rope_cache_paged(ptr qkv, int ldq, ptr q_out, int ldqo, int M, int Hq, int Hkv, int D, ptr cs, int cs_rows,
+                        int cs_f32, int rot, int interleaved, ptr seq, ptr pos, ptr kp, ptr vp, i64 page_stride,
+                        int pages, int page, ptr table, int ldt, int W, int B, ptr stream);
+size hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged);
+int hi_attn_paged(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
+                  ptr start, ptr pos, ptr out, int ldo, ptr lse, int M, int B, int Hq, int Hkv, int D, ptr work,
+                  size work_bytes, ptr stream);
+size hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D);
+int hi_attn_shared(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
+                   int shared, ptr pos, ptr out, int ldo, ptr lse, int B, int Hq, int Hkv, int D, ptr work,
+                   size work_bytes, ptr stream);
 ptr hi_load(str path, int max_batch, int max_seq, int max_prefill);
 ptr hi_load_tp(str path, int max_batch, int max_seq, int max_prefill, int world, ptr devs);
 void hi_free(ptr e);
@@ -402,6 +413,163 @@ def flash_prefill_lse(q, kc, vc, T, p0, Hq, Hkv, out=None, lse=None):
         lse = torch.empty(Hq, T, dtype=torch.float32, device=q.device)
     _need("flash_prefill_lse", lse, torch.float32, 2)
     return _flash(q, kc, vc, T, p0, Hq, Hkv, out, lse), lse
+
+
+# ------------------------------------------------------------------ paged key/value cache
+def _paged(what, kp, vp, table, *others):
+    """Checks a paged cache kp / vp [pages, Hkv, page, D] and its table [B, W], and that every tensor of the call is on
+    the current device; returns the cache's arguments of a library call, and (Hkv, page, D)."""
+    for t in (kp, vp):
+        _need(what, t, torch.float16, 4)
+    _need(what, table, torch.int32, 2)
+    gpu = torch.cuda.current_device()
+    for t in (kp, vp, table, *others):
+        if t is not None and t.get_device() != gpu:
+            raise ValueError(f"hipinfer_amd.{what}: every tensor must be on the current device (cuda:{gpu}), got {t.device}")
+    pages, Hkv, page, D = kp.shape
+    B, W = table.shape
+    if vp.shape != kp.shape:
+        raise ValueError(f"hipinfer_amd.{what}: kp {tuple(kp.shape)} and vp {tuple(vp.shape)} must have the same shape")
+    step = kp.stride(0)
+    if pages > 1 and vp.stride(0) != step:
+        raise ValueError(f"hipinfer_amd.{what}: kp and vp must have the same page stride")
+    for t in (kp, vp):
+        for n, have, want in zip(t.shape[1:], t.stride()[1:], (page * D, D, 1)):
+            if n > 1 and have != want:
+                raise ValueError(f"hipinfer_amd.{what}: a page [Hkv, page, D] must be packed")
+    if W > 1 and table.stride(1) != 1:
+        raise ValueError(f"hipinfer_amd.{what}: table rows must be contiguous")
+    ldt = table.stride(0) if B > 1 else W
+    return ((_addr(kp), _addr(vp), step if pages > 1 else Hkv * page * D, pages, page, _addr(table), ldt, W),
+            (Hkv, page, D))
+
+
+def _row_stride(t, width):
+    """The row stride of a 2-dimensional tensor; a single row's is its width."""
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def _vector(what, t, n, name, optional=False):
+    """A packed int32 vector of n entries."""
+    _need(what, t, torch.int32, 1, optional=optional)
+    if t is not None and (t.shape[0] != n or (n > 1 and t.stride(0) != 1)):
+        raise ValueError(f"hipinfer_amd.{what}: {name} must be a packed vector of {n}, got shape {tuple(t.shape)}")
+
+
+def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved=False, q_out=None):
+    """rope_cache for a paged cache: after a QKV GEMM, rotates the q and k heads of qkv [M, (Hq+2Hkv)*D] and writes the
+    rotated k and the v of row m to position pos[m] of sequence seq[m] (of sequence m without seq): row
+    pos % page of page table[seq, pos // page] of kp / vp [pages, Hkv, page, D] fp16 (D 64 or 128, page a power of two
+    from 8 on; the pages may be strided, as where K and V share an allocation). The rotated q goes to q_out [M, Hq*D]
+    (memory apart from qkv), or in place.
+
+    cs [positions, rot/2, 2] holds cos and sin, fp16 or fp32; the first rot = 2 cs.shape[1] elements of a head are rotated in
+    pairs (j, j + rot/2), or (2j, 2j + 1) with interleaved=True, the others stay. Scaled positions are the table's:
+    any cos and sin will do. Results are rounded once (rope_cache rounds after each operation).
+
+    A row that has no place is left out, its q too: a negative position (padding), one behind its table row or cs,
+    a seq outside the table, a page id outside [0, pages). Rows of one call must have places of their own."""
+    what = "rope_cache_paged"
+    _need(what, qkv, torch.float16, 2, rows=True)
+    cache, (heads, page, D) = _paged(what, kp, vp, table, qkv, cs, pos, seq, q_out)
+    M, width = qkv.shape
+    if heads != Hkv or Hq < 1 or width < (Hq + 2 * Hkv) * D:
+        raise ValueError(f"hipinfer_amd.{what}: rows of {width} and a cache of {heads} heads for Hq {Hq}, Hkv {Hkv}, D {D}")
+    _need(what, cs, ndim=3)
+    if cs.dtype not in (torch.float16, torch.float32) or cs.shape[2] != 2 or not cs.is_contiguous():
+        raise ValueError(f"hipinfer_amd.{what}: cs must be packed [positions, rot/2, 2], fp16 or fp32")
+    _vector(what, pos, M, "pos")
+    _vector(what, seq, M, "seq", optional=True)
+    if seq is None and M > table.shape[0]:
+        raise ValueError(f"hipinfer_amd.{what}: {M} rows without seq need a table of as many sequences")
+    if q_out is None:
+        q_out = qkv
+    else:
+        _need(what, q_out, torch.float16, 2, rows=True)
+        if q_out.shape[0] != M or q_out.shape[1] < Hq * D:
+            raise ValueError(f"hipinfer_amd.{what}: q_out must be [{M}, {Hq * D}], got {tuple(q_out.shape)}")
+    check_rc(lib.hi_rope_cache_paged(_addr(qkv), _row_stride(qkv, width), _addr(q_out), _row_stride(q_out, q_out.shape[1]),
+                                     M, Hq, Hkv, D, _addr(cs), cs.shape[0], int(cs.dtype == torch.float32),
+                                     2 * cs.shape[1], int(interleaved), _addr(seq), _addr(pos), *cache, table.shape[0],
+                                     _stream()), what)
+
+
+def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, start=None):
+    """Checks what attn_paged and attn_shared have in common; returns (cache, D, out)."""
+    _need(what, q, torch.float16, 2, rows=True)
+    cache, (heads, page, D) = _paged(what, kp, vp, table, q, pos, start, out, lse, work)
+    M = q.shape[0]
+    if heads != Hkv or Hq < 1 or q.shape[1] < Hq * D:
+        raise ValueError(f"hipinfer_amd.{what}: rows of {q.shape[1]} and a cache of {heads} heads for Hq {Hq}, Hkv {Hkv}, D {D}")
+    _vector(what, pos, table.shape[0], "pos")
+    if out is None:
+        out = _alloc_rows(q, M, Hq * D)
+    _need(what, out, torch.float16, 2, rows=True)
+    if out.shape[0] != M or out.shape[1] < Hq * D:
+        raise ValueError(f"hipinfer_amd.{what}: out must be [{M}, {Hq * D}], got {tuple(out.shape)}")
+    if lse is not None:
+        _need(what, lse, torch.float32, 2)
+        if lse.shape != (Hq, M) or not lse.is_contiguous():
+            raise ValueError(f"hipinfer_amd.{what}: lse must be packed [{Hq}, {M}]")
+    if work is not None:
+        _need(what, work, torch.uint8, 1, rows=work.numel() > 1)
+    return cache, D, out
+
+
+def attn_paged_work(rows, seqs, Hq, Hkv, D, ragged=False):
+    """The work buffer of attn_paged for up to `rows` rows (ragged: with start), zeroed; calls that use one buffer must
+    not overlap in time."""
+    return torch.zeros(lib.hi_attn_paged_work_bytes(rows, seqs, Hq, Hkv, D, int(ragged)), dtype=torch.uint8, device="cuda")
+
+
+def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, work=None):
+    """Causal attention over a paged cache (rope_cache_paged's kp, vp, table [B, W]).
+
+    Without start, a decode step: row b of q [B, Hq*D] is sequence b's one row, at position pos[b]. With start [B + 1]
+    int32, a ragged batch: rows start[b] .. start[b + 1] - 1 of q are sequence b's, at positions pos[b], pos[b] + 1, ...
+    (prompt chunks, drafted rows to verify, single rows of decoding sequences, in any mixture; start does not
+    decrease). A row at position p sees keys 0 .. p, at most those its table row holds; keys whose page id lies outside
+    [0, pages) are left out. A row that sees no key (pos -1: padding) gives zeros.
+
+    Returns out [M, Hq*D]; rows that belong to no sequence are left as they were. lse [Hq, M] fp32, if given, receives the
+    base-2 log-sum-exp of each row's scaled logits (-inf without keys). `work` (attn_paged_work) can be kept
+    across calls; everything the call reads of pos, start and table is read on the device, so it can be captured."""
+    what = "attn_paged"
+    cache, D, out = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, start)
+    M, B = q.shape[0], table.shape[0]
+    if start is not None:
+        _vector(what, start, B + 1, "start")
+    elif M != B:
+        raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences (one row each without start)")
+    if work is None:
+        work = attn_paged_work(M, B, Hq, Hkv, D, start is not None)
+    check_rc(lib.hi_attn_paged(_addr(q), _row_stride(q, q.shape[1]), *cache, _addr(start), _addr(pos), _addr(out),
+                               _row_stride(out, out.shape[1]), _addr(lse), M, B, Hq, Hkv, D, _addr(work), work.numel(),
+                               _stream()), what)
+    return out
+
+
+def attn_shared_work(seqs, Hq, Hkv, D):
+    """The work buffer of attn_shared, zeroed; calls that use one buffer must not overlap in time."""
+    return torch.zeros(lib.hi_attn_shared_work_bytes(seqs, Hq, Hkv, D), dtype=torch.uint8, device="cuda")
+
+
+def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work=None):
+    """attn_paged's decode step for sequences whose first `shared` positions (whole pages) are the same: they are
+    read from the pages of table[0], once for the whole batch, each sequence's later ones from its own row. Same
+    result as attn_paged where every row of table begins with those pages; a sequence may also be shorter than the
+    shared part."""
+    what = "attn_shared"
+    cache, D, out = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
+    B = q.shape[0]
+    if B != table.shape[0]:
+        raise ValueError(f"hipinfer_amd.{what}: {B} rows for a table of {table.shape[0]} sequences")
+    if work is None:
+        work = attn_shared_work(B, Hq, Hkv, D)
+    check_rc(lib.hi_attn_shared(_addr(q), _row_stride(q, q.shape[1]), *cache, shared, _addr(pos), _addr(out),
+                                _row_stride(out, out.shape[1]), _addr(lse), B, Hq, Hkv, D, _addr(work), work.numel(),
+                                _stream()), what)
+    return out
 
 
 def argmax(logits, out=None):

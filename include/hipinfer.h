@@ -160,6 +160,40 @@ int hi_flash_prefill(const void* q, int ldq, const void* kc, const void* vc, int
 int hi_flash_prefill_lse(const void* q, int ldq, const void* kc, const void* vc, int max_seq, void* out, int ldo,
                          int T, int p0, int Hq, int Hkv, int D, float* lse, void* stream);
 
+/* ---- paged key/value cache. No counterpart in the reference, whose cache is slots of max_seq positions.
+ * kp / vp [pages][Hkv][page][D] fp16, D 64 or 128, page a power of two >= 8, pages page_stride elements apart (both
+ * alike; a multiple of 8); position p of sequence b is row p % page of page table[b * ldt + p / page], p / page < W. A
+ * page id outside [0, pages) is no page. kp, vp 16-byte aligned.
+ *
+ * Rotates and stores M rows qkv [M, ldq] = [q (Hq*D) | k (Hkv*D) | v (Hkv*D)], row m at position pos[m] of sequence
+ * seq[m] (m when seq is NULL; then M <= B): q to q_out [M, ldqo] (qkv itself: in place), k to kp, v to vp. The first rot
+ * elements of a head are rotated in pairs (j, j + rot/2), or (2j, 2j + 1) when interleaved != 0, by cs [cs_rows][rot/2]
+ * (cos, sin), fp32 when cs_f32 != 0, else fp16; one rounding per result. Rows without a place (pos < 0, behind the
+ * table or cs, seq outside [0, B), no page) are left out entirely. */
+int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int M, int Hq, int Hkv, int D, const void* cs,
+                        int cs_rows, int cs_f32, int rot, int interleaved, const int* seq, const int* pos, void* kp,
+                        void* vp, long long page_stride, int pages, int page, const int* table, int ldt, int W, int B,
+                        void* stream);
+/* Bytes of hi_attn_paged's work buffer for M rows of B sequences on the current device (ragged: calls with start);
+ * 0 for bad sizes. Zeroed once by the caller, left fit for the next call by every call. */
+size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged);
+/* Causal attention over the paged cache: start NULL, row b of q [M, ldq] at position pos[b] of sequence b (M == B); else
+ * rows start[b] .. start[b + 1] - 1 at positions pos[b], pos[b] + 1, ... of sequence b (start [B + 1], not
+ * decreasing). A row at position p sees keys 0 .. p that its table row and the pages hold; a row without any gives 0 and
+ * lse -inf. Rows of no sequence are left as they were. Hq / Hkv in 1..16, query head h reads kv head h / (Hq / Hkv). lse
+ * [Hq][M] fp32 (base-2 log-sum-exp of the scaled logits) or NULL. work: work_bytes >= hi_attn_paged_work_bytes(...),
+ * 16-byte aligned; launches that share it must not run concurrently. */
+int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,
+                  const int* table, int ldt, int W, const int* start, const int* pos, void* out, int ldo, float* lse,
+                  int M, int B, int Hq, int Hkv, int D, void* work, size_t work_bytes, void* stream);
+/* The same for hi_attn_shared. */
+size_t hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D);
+/* hi_attn_paged without start for B sequences whose first `shared` positions (a multiple of page) are one prefix, read
+ * from table row 0's pages once for the batch; later positions are each sequence's own. */
+int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,
+                   const int* table, int ldt, int W, int shared, const int* pos, void* out, int ldo, float* lse, int B,
+                   int Hq, int Hkv, int D, void* work, size_t work_bytes, void* stream);
+
 /* ---- RMSNorm (unfused form of the GEMV prologue; the reference's tests build references with it)
  * y[M, H] = w * fp16(x * rsqrt(mean(x^2) + eps)), rows contiguous. Replaces api.cu:76-79
  * (hi_rmsnorm); hipinfer.py:13. */
