@@ -41,66 +41,9 @@
 //    the key halves wholly above its rows' diagonal; cache rows past the block's last key read as
 //    zeros (the DMA's buffer range ends there);
 //  * blocks run the longest query tiles (the most keys) first, across all heads.
-#include <type_traits>
-
-#include "hi_common.h"
+#include "flash.h"
 
 namespace {
-
-constexpr int kFpRG = 4;              // 32-row groups per block (2 waves each); 2 for small grids
-constexpr int kFpKPW = 64;            // keys per wave per tile (32-key MFMA blocks of the wave's half)
-constexpr int kFpBKV = 2 * kFpKPW;    // keys per tile
-constexpr int kFpStages = 2;          // LDS stages of K/V tiles
-constexpr float kFpMaxLag = 8.f;      // log2 of how far a row's reference max may trail its max
-
-// XOR term of key r's 16-byte chunks in the K tile: the 16 keys (D = 128) or 8 key pairs (D = 64)
-// that one 128-bit fragment read serves per cycle land on distinct banks.
-template <int D>
-__device__ __forceinline__ int k_swz(int r) {
-  if constexpr (D == 128) return r & 15;
-  else return (r >> 1) & 7;
-}
-// XOR term of key r's chunks in the V tile. A transpose read covers keys r..r+3 (r % 4 == 0) at
-// 4 consecutive chunks per 32 lanes and 2 per 16 lanes; the terms 0, 6, 12, 10 (D = 128) or 0, 6,
-// 4, 2 (D = 64) for r % 4 = 0..3 move those chunks to distinct banks at either width.
-template <int D>
-__device__ __forceinline__ int v_swz(int r) {
-  const int a = r & 3;
-  return ((2 * a) ^ (4 * a)) & (D / 8 - 1);
-}
-
-// LDS of one block: two stages of K tiles and two of V tiles while the keys stream, then in the same
-// bytes the O^T accumulators the second wave of each row group hands to the first; last, the second
-// waves' m and l. It is dynamic LDS: reads of a __shared__ array that a DMA instruction also writes
-// made the compiler wait for every DMA in flight (s_waitcnt vmcnt(0)) before the first of them, right
-// after the next tile's DMA had been issued, so that no tile streamed in while another was computed.
-template <int D, int RG>
-struct FpSmem {
-  static constexpr int kTile = kFpBKV * D / 8;                // 16-byte chunks of one K or V tile
-  static constexpr int kMl = 2 * kFpStages * kTile;           // chunk index of m and l
-  static constexpr size_t kBytes = kMl * 16 + 2 * RG * 64 * 4;
-  static_assert(RG * (D / 32) * 64 * 64 <= kMl * 16, "merge fits the stages");
-};
-
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-
-// The two builtins below sit in the device pass only: in this kernel's host pass they made the
-// compiler drop the kernel's launch stub without a diagnostic (an undefined symbol at load).
-// 16-byte buffer DMA of each lane's chunk at byte offset voff into LDS slot lane of `lds`.
-__device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, void* lds, int voff) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)lds, 16, voff, 0, 0, 0);
-#endif
-}
-// ds_read_tr16_b64 at LDS address p: within each 16-lane group, lane i receives element i % 4 of
-// the 4 halves lane 4 e + i / 4 addresses, as its element e.
-__device__ __forceinline__ f16x4 lds_read_tr16(const f16* __restrict__ p) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)p));
-#else
-  return f16x4{};
-#endif
-}
 
 template <int D, int RG>
 __global__ void __launch_bounds__(128 * RG)
@@ -170,18 +113,6 @@ __global__ void __launch_bounds__(128 * RG)
     asm volatile("" : "+v"(voff[i]));
   };
 
-  // transpose reads of V: lane j of each 16-lane group g reads 4 d of key 4 (g / 2) + j / 4 (+ the
-  // step's key base), d = 16 (g % 2) + 4 (j % 4) (+ the output tile's d base); the group's lane i
-  // then holds d = 16 (g % 2) + i of those 4 keys. Keys of one read are 4-aligned, so the swizzle
-  // term is the lane's own.
-  const int vr = 4 * fk + ((lane & 15) >> 2);                  // key within a 16-key step
-  const int vc0 = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);   // logical chunk within a 32-d tile
-  const f16* vb[DT];                                           // the lane's first read of each output tile
-#pragma unroll
-  for (int dt = 0; dt < DT; dt++)
-    vb[dt] = reinterpret_cast<const f16*>(vs_) + (kFpKPW * kh + vr) * D + 8 * ((4 * dt + vc0) ^ v_swz<D>(vr)) + 4 * (lane & 1);
-  const int kr = kFpKPW * kh + fr;                             // K row of this lane's first fragments
-  const int ksw = k_swz<D>(kr);                                // the same for every block (kr % 16)
   const int xaddr = (lane ^ 32) << 2;                          // lane l ^ 32, for ds_bpermute
   auto xor32 = [&](float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(xaddr, __builtin_bit_cast(int, v)));
@@ -196,259 +127,17 @@ __global__ void __launch_bounds__(128 * RG)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[dt][e] = 0.f;
 
-  // S^T = K Q^T over 32-key block kt of the wave's keys in K stage st; lane (row fr, half fk) gets
-  // keys 32 kt + 8 g + 4 fk + e
-  auto logits = [&](int st, int kt, f32x16& s) {
-    f32x16 a;
-#pragma unroll
-    for (int e = 0; e < 16; e++) a[e] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < NQ; ks++) {
-      const f16x8 kf = __builtin_bit_cast(f16x8, ks_[st * Sm::kTile + (kr + 32 * kt) * CPR + ((2 * ks + fk) ^ ksw)]);
-      a = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[ks], a, 0, 0, 0);
-    }
-    s = a;
+  auto hidden = [&](int t, int kt, int e) {
+    return t * kFpBKV + kFpKPW * kh + 32 * kt + 8 * (e >> 2) + 4 * fk + (e & 3) > qpos;
   };
-  // the V^T fragments of block kt (V stage st): of step ss, lane half fk holds keys 32 kt + 16 ss +
-  // 4 fk + 0..3 and 32 kt + 16 ss + 8 + 4 fk + 0..3 of the wave's keys, as P's registers do
-  auto load_v = [&](int st, int kt, f16x8 (&vf)[2][DT]) {
-#pragma unroll
-    for (int ss = 0; ss < 2; ss++)
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++) {
-        const f16* pa = vb[dt] + st * (Sm::kTile * 8) + (32 * kt + 16 * ss) * D;
-        const f16x4 fa = lds_read_tr16(pa), fb = lds_read_tr16(pa + 8 * D);  // key + 8: same swizzle term
-        vf[ss][dt] = f16x8{fa[0], fa[1], fa[2], fa[3], fb[0], fb[1], fb[2], fb[3]};
-      }
-  };
-  // O^T += V^T P^T of one 32-key block
-  auto pv = [&](const f16x8 (&vf)[2][DT], const f16x8 (&pf)[2]) {
-#pragma unroll
-    for (int ss = 0; ss < 2; ss++)
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[ss][dt], pf[ss], o[dt], 0, 0, 0);
-  };
-  // p = exp2(c s - m) of one block, its sum into l_i, fp16 p in P.V operand order
-  auto softmax = [&](const f32x16& s, float m_use, f16x8 (&pf)[2]) {
-    float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale_log2, -m_use));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], scale_log2, -m_use));
-      sum0 += p;
-      sum1 += p1;
-      pf[e >> 3][e & 7] = (f16)p;
-      pf[e >> 3][(e & 7) + 1] = (f16)p1;
-    }
-    l_i += sum0 + sum1;
-  };
-
-  // One key tile t (stage t & 1, given as a constant in the main loop): the softmax and P.V of its
-  // logits sc, with the logits of tile t + 1 into sn in between. A wave issues in order, so the
-  // MFMAs of one product are interleaved with the vector work of the other tile's softmax by
-  // scheduling groups; otherwise each product's MFMAs run back to back, then the softmax with the
-  // matrix cores idle (both waves of a SIMD leave the tile's barrier together). The P.V of the
-  // tile's second block (pl, its V fragments vl read before the next barrier) runs after that
-  // barrier: matrix work that needs no LDS while the first K fragments are on their way.
-  f16x8 pl[2], vl[2][DT];
-#pragma unroll
-  for (int ss = 0; ss < 2; ss++) {
-    pl[ss] = f16x8{};
-#pragma unroll
-    for (int dt = 0; dt < DT; dt++) vl[ss][dt] = f16x8{};
-  }
-  auto tile = [&](auto stc, auto maskc, auto nextc, int t, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
-    constexpr bool MASK = decltype(maskc)::value;  // the tile holds keys past some row's diagonal
-    constexpr bool NEXT = decltype(nextc)::value;  // there is a tile t + 1
-    const int st = stc;
-    wait_lgkm0();
-    wait_vmcnt<0>();     // this wave's shares of K tile t + 1 and V tile t are in LDS
-    barrier_no_fence();  // every share is, and every wave is done with K tile t and V tile t - 1
-    const int k0 = t * kFpBKV + kFpKPW * kh;  // this wave's first key
-    if constexpr (MASK) {
-#pragma unroll
-      for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int kp = k0 + 32 * kt + 8 * (e >> 2) + 4 * fk + (e & 3);
-          if (kp > qpos) sc[kt][e] = -__builtin_huge_valf();
-        }
-    }
-    // the row's reference max m_i moves only when the tile's scaled max exceeds it by more than 2^8,
-    // so p = exp2(c s - m_i) stays at most 256 (exact range for fp16 P and fp32 sums) and O is
-    // rescaled only then; lanes l and l ^ 32 then agree on the new one. The max of the raw logits is
-    // scaled once (c > 0 keeps the order) and c s - m_i is one fma
-    // The MFMAs of this tile up to its first P.V, in slots: the last block's P.V, then (NEXT) the
-    // logits of tile t + 1. The 2 IPW DMA instructions of K tile t + 2 and V tile t + 1 go out over the
-    // slots of the first logits block; with 4 waves, each issuing twice as many and without a second
-    // wave on its SIMD to fill its stalls, over all of them (64 rows after 2000 positions 26.1 ->
-    // 22.6 us, 512 after 2048 36.0 -> 32.7; 8 waves: no gain, 2 % slower at T = 2048 after 4096).
-    constexpr int ND = 2 * IPW, LA = 3;  // DMA instructions, LDS reads ahead of their MFMA
-    constexpr int S0 = RG == 2 ? 0 : 2 * DT, NS = RG == 2 ? 2 * DT + 2 * NQ : NQ;
-    auto dma_here = [](int m) constexpr {  // DMA instructions that go before slot m
-      int n = 0;
-      for (int j = 0; j < ND; j++) n += S0 + j * NS / ND == m;
-      return n;
-    };
-    constexpr int kDma = (ND + NS - 1) / NS;  // at most this many before one slot
-    auto dma = [&](int m) {
-#pragma unroll
-      for (int j = 0; j < ND; j++)
-        if (S0 + j * NS / ND == m) j < IPW ? issue_k(j, st) : issue_v(j - IPW, st ^ 1);
-    };
-    auto load_k = [&](int kt, int ks) {
-      return __builtin_bit_cast(f16x8, ks_[(st ^ 1) * Sm::kTile + (kr + 32 * kt) * CPR + ((2 * ks + fk) ^ ksw)]);
-    };
-    float mx = -__builtin_huge_valf();
-    f16x8 kf[NQ];
-    f32x16 a0;
-#pragma unroll
-    for (int e = 0; e < 16; e++) a0[e] = 0.f;
-#pragma unroll
-    for (int m = 0; m < 2 * DT; m++) {
-      if constexpr (NEXT) {
-        dma(m);
-        if (m >= 2 * DT - LA) kf[m - (2 * DT - LA)] = load_k(0, m - (2 * DT - LA));
-      }
-      o[m % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl[m / DT][m % DT], pl[m / DT], o[m % DT], 0, 0, 0);
-    }
-    if constexpr (NEXT) {
-#pragma unroll
-      for (int ks = 0; ks < NQ; ks++) {
-        dma(2 * DT + ks);
-        if (ks + LA < NQ) kf[ks + LA] = load_k(0, ks + LA);
-        a0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], qf[ks], a0, 0, 0, 0);
-      }
-      sn[0] = a0;
-    }
-#pragma unroll
-    for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-      for (int e = 0; e < 16; e++) mx = fmaxf(mx, sc[kt][e]);
-    constexpr int kMaskOps = MASK ? 8 : 0;  // more vector work per MFMA
-#pragma unroll
-    for (int m = 0; m < 2 * DT; m++) {
-      if (NEXT && dma_here(m)) __builtin_amdgcn_sched_group_barrier(0x020, kDma, 0);  // DMA
-      if (NEXT && m >= 2 * DT - LA) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // MFMA (the last block's P.V)
-      __builtin_amdgcn_sched_group_barrier(0x002, 2 + kMaskOps, 0);  // VALU (the max)
-    }
-    if constexpr (NEXT) {
-#pragma unroll
-      for (int ks = 0; ks < NQ; ks++) {
-        if (dma_here(2 * DT + ks)) __builtin_amdgcn_sched_group_barrier(0x020, kDma, 0);
-        if (ks + LA < NQ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);           // MFMA (logits)
-        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-      }
-    }
-    if (__any(mx * scale_log2 > m_i + kFpMaxLag)) {  // m_i = -inf: moves to the first finite max
-      mx = fmaxf(mx, xor32(mx)) * scale_log2;
-      const bool move = mx > m_i + kFpMaxLag;
-      const float alpha = move ? __builtin_amdgcn_exp2f(m_i - mx) : 1.f;
-      if (move) m_i = mx;
-      l_i *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) o[dt][e] *= alpha;
-    }
-    // m_i is -inf only for a row that has seen no key yet (one whose first key lies in the other
-    // half): every logit is then -inf and every p 0
-    const float m_use = m_i == -__builtin_huge_valf() ? 0.f : m_i;
-    f16x8 pf[2], vf[2][DT];
-    if constexpr (NEXT) {
-      f32x16 a1;
-#pragma unroll
-      for (int e = 0; e < 16; e++) a1[e] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < LA; ks++) kf[ks] = load_k(1, ks);
-#pragma unroll
-      for (int ks = 0; ks < NQ; ks++) {
-        dma(2 * DT + NQ + ks);
-        if (ks + LA < NQ) kf[ks + LA] = load_k(1, ks + LA);
-        a1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], qf[ks], a1, 0, 0, 0);
-      }
-      sn[1] = a1;
-    }
-    softmax(sc[0], m_use, pf);
-    load_v(st, 0, vf);
-    pv(vf, pf);
-    softmax(sc[1], m_use, pl);
-    load_v(st, 1, vl);
-    if constexpr (NEXT) {
-      __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
-#pragma unroll
-      for (int ks = 0; ks < NQ; ks++) {
-        if (dma_here(2 * DT + NQ + ks)) __builtin_amdgcn_sched_group_barrier(0x020, kDma, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        if (ks + LA >= NQ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // MFMA (logits)
-        __builtin_amdgcn_sched_group_barrier(0x002, 56 / NQ, 0);       // VALU (softmax of block 0)
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * DT; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // MFMA (P.V of block 0)
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 56 / (2 * DT), 0); // VALU (softmax of block 1)
-      }
-    }
-  };
-
-  // ---- prologue: K tiles 0 and 1 and V tile 0 in flight, the logits of tile 0
-#pragma unroll
-  for (int i = 0; i < IPW; i++) issue_k(i, 0);
-#pragma unroll
-  for (int i = 0; i < IPW; i++) {
-    issue_v(i, 0);
-    issue_k(i, 1);
-  }
-  wait_vmcnt<2 * IPW>();
-  barrier_no_fence();
-  f32x16 sa[2], sb[2];
-  logits(0, 0, sa[0]);
-  logits(0, 1, sa[1]);
-  constexpr std::integral_constant<int, 0> kEven{};
-  constexpr std::integral_constant<int, 1> kOdd{};
-  int t = 0;
-  const std::true_type yes{};
-  const std::false_type no{};
-  for (; t + 2 <= n_full && t + 2 < nt; t += 2) {
-    tile(kEven, no, yes, t, sa, sb);
-    tile(kOdd, no, yes, t + 1, sb, sa);
-  }
-  // The other tiles may hold masked keys. A wave leaves out a tile whose keys (its half) lie wholly past
-  // its rows' diagonal or the block's last key, as it does every later one, but for its share of the
-  // DMA and the barrier: their weights are 0, but 0 times an infinity or NaN in a later row's V is not.
+  auto enter_masked = [](int) {};
+  auto advance = [] {};
   auto live = [&](int t) {
     const int k0 = t * kFpBKV + kFpKPW * kh;
     return k0 <= p0 + qw + 31 && k0 < kv_end;
   };
-  for (; t + 1 < nt; t++) {  // an odd full tile, the first of two tiles on the diagonal
-    if (live(t)) {
-      tile(t & 1, yes, yes, t, sa, sb);
-      sa[0] = sb[0];
-      sa[1] = sb[1];
-    } else {
-      wait_lgkm0();
-      wait_vmcnt<0>();
-      barrier_no_fence();
-#pragma unroll
-      for (int i = 0; i < IPW; i++) {
-        issue_k(i, t & 1);
-        issue_v(i, (t & 1) ^ 1);
-      }
-    }
-  }
-  if (live(t)) {
-    tile(t & 1, yes, no, t, sa, sb);
-  } else {
-    wait_lgkm0();
-    wait_vmcnt<0>();
-    barrier_no_fence();
-  }
 
-  pv(vl, pl);
+#include "flash_tile.h"
 
   // ---- merge the two key halves of each row group: the second wave hands (m, l, O) over
   wait_vmcnt<0>();
