@@ -1,6 +1,7 @@
 // Serving from a paged key/value cache: rotation and cache write of projected rows (hi_rope_cache_paged), attention over
 // the pages (hi_attn_paged) and attention of a batch whose sequences share their first positions (hi_attn_shared).
 // The cache and its table: paged.h.
+#include "decode_split.h"
 #include "flash.h"
 #include "paged.h"
 #include "paged_plan.h"
@@ -74,62 +75,6 @@ struct AttnArgs {
   int M, B, Hq, Hkv, shared;  // positions below `shared` are on the pages of table row 0
   float scale_log2;
 };
-
-// One block per (row, query head): tiles of 256 keys, a key per thread for the logits, a dim per thread for P.V.
-template <int D>
-__global__ void __launch_bounds__(256) attn_paged_simple_kernel(AttnArgs a, PagedCache c) {
-  __shared__ float sp[256], red[4], sq[D], so[256];
-  __shared__ int sid[256];
-  const int m = blockIdx.x, h = blockIdx.y, hk = h / (a.Hq / a.Hkv), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int b = m, t = 0;
-  if (a.start) {
-    for (b = 0; b < a.B; b++)
-      if (a.start[b] <= m && m < a.start[b + 1]) break;
-    if (b == a.B) return;
-    t = m - a.start[b];
-  }
-  const int n = (int)min((int64_t)a.pos[b] + t + 1, (int64_t)c.capacity());
-  if (tid < D) sq[tid] = (float)a.q[(int64_t)m * a.ldq + h * D + tid];
-  float mx = -__builtin_huge_valf(), l = 0.f, o = 0.f;
-  const int page = 1 << c.shift, d = tid % D, part = tid / D;
-  for (int k0 = 0; k0 < n; k0 += 256) {
-    __syncthreads();
-    const int k = k0 + tid;
-    const int id = k < n ? c.entry(k < a.shared ? 0 : b, k >> c.shift) : -1;
-    float x = -__builtin_huge_valf();
-    if (c.has(id)) {
-      const f16* kr = c.kp + id * c.stride + ((int64_t)hk * page + (k & (page - 1))) * D;
-      float s = 0.f;
-      for (int i = 0; i < D; i++) s = __builtin_fmaf(sq[i], (float)kr[i], s);
-      x = s * a.scale_log2;
-    }
-    const float wm = wave_max(x);
-    if (lane == 0) red[wave] = wm;
-    __syncthreads();
-    const float mn = fmaxf(mx, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float ref = mn == -__builtin_huge_valf() ? 0.f : mn;
-    const float alpha = exp2f(mx - ref), p = exp2f(x - ref);
-    mx = mn;
-    sp[tid] = p;
-    sid[tid] = c.has(id) ? id : -1;
-    l = l * alpha + p;
-    o *= alpha;
-    __syncthreads();
-    for (int j = part; j < 256; j += 256 / D)
-      if (sid[j] >= 0) o = __builtin_fmaf(sp[j], (float)c.vp[sid[j] * c.stride + ((int64_t)hk * page + ((k0 + j) & (page - 1))) * D + d], o);
-  }
-  l = wave_sum(l);
-  __syncthreads();
-  if (lane == 0) red[wave] = l;
-  so[tid] = o;
-  __syncthreads();
-  l = (red[0] + red[1]) + (red[2] + red[3]);
-  if (tid < D) {
-    for (int j = 1; j < 256 / D; j++) o += so[tid + j * D];
-    a.out[(int64_t)m * a.ldo + h * D + tid] = (f16)(l == 0.f ? 0.f : o / l);
-  }
-  if (a.lse && tid == 0) a.lse[(int64_t)h * a.M + m] = mx + log2f(l);
-}
 
 // ---- row runs (and the common part of a shared prefix)
 //
@@ -498,6 +443,325 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int cap, Fla
   if (a.lse && dt == 0 && g == 0 && fk == 0) a.lse[(int64_t)h * a.M + u.row0 + token] = m + log2f(l);
 }
 
+// ---- one row per sequence
+//
+// The slot cache's decode attention (decode.hip: a wave takes 32 keys, K Q^T and V^T P^T on 16x16x32 MFMAs with the group's
+// heads as columns, K and V straight into operand registers, refilled as soon as they are used) with its splits
+// (decode_split.h), over pages: the 8 keys that a lane's K rows, or its V rows, come from lie on one page, so a lane has
+// one 64-bit address each for K and V per tile, from entries requested a tile ahead. What the slot kernel leaves to the
+// buffer bounds is done in registers, in a wave's last tile and in tiles with an entry that is no page only: logits of
+// keys that are not there become -inf, their V rows zeros.
+// OWN: the part of a sequence behind a shared prefix; blocks leave their splits' results to attn_shared_join_kernel.
+struct StepPlan {
+  int S, S1;      // splits of a pair: the launch's, and those that give every CU its blocks (splits_used)
+  int* counters;  // [B * Hkv], arrivals of a pair's splits
+  float *ml, *po; // partial results: [B][Hq][S][2] m and l, [B][Hq][S][D] O
+};
+
+// Keys from `base` on that sequence b's row sees.
+__device__ __forceinline__ int step_keys(const AttnArgs& a, int cap, int b, int base) {
+  return plan_end(a.pos[b], 1, cap) > base ? plan_end(a.pos[b], 1, cap) - base : 0;
+}
+
+template <int GC, int D, int NWV>
+struct StepSmem {
+  float wo[NWV][GC][D];
+  float wm[NWV][GC], wl[NWV][GC];
+  float sm[GC][kDecodeMaxSplits], sw[GC][kDecodeMaxSplits];
+  int is_last;
+};
+
+template <int GC, int D, int NWV, bool OWN>
+__global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, PagedCache c, StepPlan f) {
+  constexpr int KS = D / 32;               // k steps of a logits product
+  constexpr int DL = D / 16;               // V dims (and P.V products) per lane
+  constexpr int BK = NWV * kDaTile;        // keys per block pass
+  constexpr int NT = NWV * 64;
+  typedef typename std::conditional<DL == 8, u32x4, u32x2>::type VT;
+  __shared__ StepSmem<GC, D, NWV> sh;
+  // split-major blocks: a pair's used splits come first in dispatch order
+  const int nhb = a.B * a.Hkv, G = a.Hq / a.Hkv, page = 1 << c.shift;
+  const int split = blockIdx.x / nhb, hk = blockIdx.x % a.Hkv, b = (blockIdx.x % nhb) / a.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int len = step_keys(a, c.capacity(), b, OWN ? a.shared : 0);
+  const int S_eff = splits_used(len, f.S, f.S1);
+  if (split >= S_eff) return;
+  const int chunk = (((len + S_eff - 1) / S_eff) + 7) & ~7;  // the groups of 8 keys start on multiples of 8
+  const int base = OWN ? a.shared : 0;
+  const int start = base + split * chunk, end = base + min(len, (split + 1) * chunk);
+
+  const int r = lane & 15, fk = lane >> 4;
+  // S^T = K Q^T (16x16x32): A row r of block x is the tile's key 8 (r / 4) + 4 x + r % 4, so lane group fk of the C layout
+  // ends up with keys 8 fk .. 8 fk + 7 of head r: the B operand of the 32-key P.V product. V: lane (r, fk) loads dims
+  // DL r .. of keys 8 fk + i.
+  const int kg = 8 * (r >> 2), vg = 8 * fk;  // the lane's key groups in a tile
+  const f16* const kl = c.kp + ((int64_t)hk * page + (r & 3)) * D + 8 * fk;
+  const f16* const vl = c.vp + (int64_t)hk * page * D + DL * r;
+  auto entry = [&](int key) { return key < end ? c.entry(b, key >> c.shift) : -1; };
+  // element offset of the group that starts at `key`; that of page 0 for keys that are not there
+  auto place = [&](int id, int key) { return c.has(id) ? id * c.stride + (int64_t)(key & (page - 1)) * D : (int64_t)0; };
+  u32x4 kf[2][KS];
+  VT vf[8];
+  auto load_k = [&](int64_t at) {
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int s = 0; s < KS; s++) kf[x][s] = *reinterpret_cast<const u32x4*>(kl + at + 4 * x * D + 32 * s);
+  };
+  auto load_v = [&](int64_t at) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) vf[i] = *reinterpret_cast<const VT*>(vl + at + i * D);
+  };
+  const int t_first = start + wave * kDaTile;
+  const f16* qg = a.q + (int64_t)b * a.ldq + (hk * G + (r < G ? r : 0)) * D + 8 * fk;
+  float m = -__builtin_huge_valf(), l = 0.f;  // of head r; l over this lane's keys only
+  f32x4 o[DL];                                // O^T: dim DL (4 fk + i) + n of head r in o[n][i]
+#pragma unroll
+  for (int n = 0; n < DL; n++) o[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (t_first < end) {
+    int kid = entry(t_first + kg), vid = entry(t_first + vg);
+    bool there = c.has(vid);  // this lane's V group of the tile lies on a page
+    bool whole = __all(there) && t_first + kDaTile <= end;
+    int64_t va = place(vid, t_first + vg);
+    load_k(place(kid, t_first + kg));
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) qf[s] = *reinterpret_cast<const u32x4*>(qg + 32 * s);
+    load_v(va);
+    kid = entry(t_first + BK + kg);
+    vid = entry(t_first + BK + vg);
+    // One tile; the next tile's K is requested as soon as this one's is used, and so is its V.
+    auto tile = [&](int t0, auto maskc, auto lastc) {
+      constexpr bool MASK = decltype(maskc)::value, LAST = decltype(lastc)::value;
+      f32x4 sc[2];
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        sc[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+          sc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[x][s]),
+                                                         __builtin_bit_cast(f16x8, qf[s]), sc[x], 0, 0, 0);
+      }
+      const bool was = there;
+      if constexpr (!LAST) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(place(kid, t0 + BK + kg));
+        there = c.has(vid);
+        whole = __all(there) && t0 + BK + kDaTile <= end;
+        va = place(vid, t0 + BK + vg);
+        kid = entry(t0 + 2 * BK + kg);
+        vid = entry(t0 + 2 * BK + vg);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      float p[8];
+      float mx = -__builtin_huge_valf();
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        p[k] = sc[k >> 2][k & 3] * a.scale_log2;
+        if (MASK && !(was && t0 + vg + k < end)) p[k] = -__builtin_huge_valf();
+        mx = fmaxf(mx, p[k]);
+      }
+      const float m_old = m;
+      m = fmaxf(m, rows_reduce<true>(mx));
+      // -inf while no key was there, or every logit so far is: their weights are 0
+      const float mn = m == -__builtin_huge_valf() ? 0.f : m;
+      const float alpha = exp2f(m_old - mn);  // 0 on the first tile (m = -inf)
+      float ps = 0.f;
+      f16x8 pf;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        p[k] = exp2f(p[k] - mn);
+        ps += p[k];
+        pf[k] = (f16)p[k];
+      }
+      l = __builtin_fmaf(l, alpha, ps);
+#pragma unroll
+      for (int n = 0; n < DL; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[n][i] *= alpha;
+      if constexpr (MASK) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (!(was && t0 + vg + k < end)) vf[k] = VT{};
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < DL; n++) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          w[k] = __builtin_amdgcn_perm(vf[2 * k + 1][n >> 1], vf[2 * k][n >> 1], n & 1 ? 0x07060302u : 0x05040100u);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), pf, o[n], 0, 0, 0);
+      }
+      if constexpr (!LAST) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(va);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    int t0 = t_first;
+    for (; t0 + BK < end; t0 += BK) {
+      if (whole) tile(t0, no, no);
+      else tile(t0, yes, no);
+    }
+    tile(t0, yes, yes);
+  }
+  l = rows_reduce<false>(l);
+
+  // ---- merge the block's waves (a wave without keys has m = -inf and weight 0)
+  if (r < G) {
+    if (fk == 0) {
+      sh.wm[wave][r] = m;
+      sh.wl[wave][r] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int n = 0; n < DL; n += 4)
+        *reinterpret_cast<f32x4*>(&sh.wo[wave][r][DL * (4 * fk + i) + n]) =
+            f32x4{o[n][i], o[n + 1][i], o[n + 2][i], o[n + 3][i]};
+  }
+  __syncthreads();
+  const bool single = S_eff == 1;
+  const int64_t pair = (int64_t)b * a.Hq + hk * G;  // of head 0 of the group; its partials start at pair * S
+  for (int i = tid; i < G * D; i += NT) {
+    const int g = i / D, d = i % D;
+    float M = -__builtin_huge_valf();
+#pragma unroll
+    for (int w = 0; w < NWV; w++) M = fmaxf(M, sh.wm[w][g]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < NWV; w++) {
+      const float e = sh.wm[w][g] == -__builtin_huge_valf() ? 0.f : exp2f(sh.wm[w][g] - M);
+      L = __builtin_fmaf(sh.wl[w][g], e, L);
+      O = __builtin_fmaf(sh.wo[w][g][d], e, O);
+    }
+    const int64_t at = (pair + g) * f.S + split;
+    if (OWN) {
+      f.po[at * D + d] = O;
+      if (d == 0) {
+        f.ml[2 * at] = M;
+        f.ml[2 * at + 1] = L;
+      }
+    } else if (single) {
+      a.out[(int64_t)b * a.ldo + (hk * G + g) * D + d] = (f16)(L == 0.f ? 0.f : O / L);
+      if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
+    } else {
+      st_coherent(f.po + at * D + d, O);
+      if (d == 0) {
+        st_coherent(f.ml + 2 * at, M);
+        st_coherent(f.ml + 2 * at + 1, L);
+      }
+    }
+  }
+  if (OWN || single) return;
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partial stores are complete
+  __syncthreads();
+  if (tid == 0) {
+    int* ctr = f.counters + b * a.Hkv + hk;
+    const int done = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sh.is_last = done == S_eff - 1;
+    if (sh.is_last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next launch
+  }
+  __syncthreads();
+  if (!sh.is_last) return;
+  // ---- the last block merges the S_eff splits of every head of its group, in split order. The (m, l) pairs and the first
+  //      16 splits' partial outputs are requested in one round.
+  constexpr int EPT = (GC * D + NT - 1) / NT;  // output elements per thread
+  float v0[EPT][16];
+#pragma unroll
+  for (int e = 0; e < EPT; e++) {
+    const int i = tid + e * NT;
+    const int g = min(i / D, G - 1), d = i % D;
+    const float* pp = f.po + (pair + g) * f.S * D + d;
+#pragma unroll
+    for (int k = 0; k < 16; k++) v0[e][k] = ld_coherent(pp + (int64_t)min(k, S_eff - 1) * D);
+  }
+  for (int i = tid; i < G * S_eff; i += NT) {
+    const int g = i / S_eff, s = i - g * S_eff;
+    const float* pp = f.ml + ((pair + g) * f.S + s) * 2;
+    sh.sm[g][s] = ld_coherent(pp);
+    sh.sw[g][s] = ld_coherent(pp + 1);
+  }
+  __syncthreads();
+  for (int g = wave; g < G; g += NWV) {  // S_eff is at most a wave's lanes
+    const float ms = lane < S_eff ? sh.sm[g][lane] : -__builtin_huge_valf(), ls = lane < S_eff ? sh.sw[g][lane] : 0.f;
+    const float M = wave_max(ms);
+    const float e = ms == -__builtin_huge_valf() ? 0.f : exp2f(ms - M);
+    const float L = wave_sum(ls * e);
+    if (lane < S_eff) sh.sw[g][lane] = L == 0.f ? 0.f : e / L;
+    if (a.lse && lane == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EPT; e++) {
+    const int i = tid + e * NT;
+    if (i < G * D) {
+      const int g = i / D, d = i % D;
+      const float* pp = f.po + (pair + g) * f.S * D + d;
+      float O = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; k++) O = __builtin_fmaf(v0[e][k], k < S_eff ? sh.sw[g][k] : 0.f, O);
+      for (int s0 = 16; s0 < S_eff; s0 += 16) {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) v[k] = ld_coherent(pp + (int64_t)min(s0 + k, S_eff - 1) * D);
+#pragma unroll
+        for (int k = 0; k < 16; k++) O = __builtin_fmaf(v[k], s0 + k < S_eff ? sh.sw[g][s0 + k] : 0.f, O);
+      }
+      a.out[(int64_t)b * a.ldo + (hk * G + g) * D + d] = (f16)O;
+    }
+  }
+}
+
+// Joins a shared prefix's splits and each sequence's own: block = (row tile of the prefix, kv head, row group, 32 dims), wave =
+// 8 of the dims, in the lanes' order of the prefix's partial results.
+template <int D, int RG>
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int cap, FlashPlan f, StepPlan st) {
+  constexpr int BQ = 32 * RG, DT = D / 32;
+  const int lane = threadIdx.x & 63, g8 = threadIdx.x >> 6, fr = lane & 31, fk = lane >> 5;
+  int i = blockIdx.x;
+  const int dt = i % DT, rg = i / DT % RG;
+  i /= DT * RG;
+  const int hk = i % a.Hkv, tile = i / a.Hkv, G = a.Hq / a.Hkv;
+  const int pr = tile * BQ + rg * 32 + fr;
+  if (pr >= a.M * G) return;
+  const int b = pr / G, h = hk * G + pr - b * G;
+  const int own = splits_used(step_keys(a, cap, b, a.shared), st.S, st.S1);
+  const int64_t slot = (int64_t)tile * f.splits * a.Hkv + hk;
+  const float* ml = f.ml + slot * 2 * BQ + rg * 32 + fr;
+  const f32x4* po = reinterpret_cast<const f32x4*>(f.po) + ((slot * RG + rg) * DT * 4 + dt * 4 + g8) * 64 + lane;
+  const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * RG * DT * 4 * 64;
+  const int d0 = dt * 32 + 8 * g8 + 4 * fk;
+  const float* oml = st.ml + ((int64_t)b * a.Hq + h) * st.S * 2;
+  const float* opo = st.po + ((int64_t)b * a.Hq + h) * st.S * D + d0;
+  float m = -__builtin_huge_valf();
+#pragma unroll 8
+  for (int s = 0; s < f.splits; s++) m = fmaxf(m, ml[s * sm]);
+  for (int s = 0; s < own; s++) m = fmaxf(m, oml[2 * s]);
+  const float ref = m == -__builtin_huge_valf() ? 0.f : m;
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float w, float ls, f32x4 v) {
+    l = __builtin_fmaf(w, ls, l);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, v[e], o[e]);
+  };
+#pragma unroll 8
+  for (int s = 0; s < f.splits; s++) add(exp2f(ml[s * sm] - ref), ml[s * sm + BQ], po[s * so]);
+  for (int s = 0; s < own; s++)
+    add(exp2f(oml[2 * s] - ref), oml[2 * s + 1], *reinterpret_cast<const f32x4*>(opo + (int64_t)s * D));
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  f16x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = (f16)(o[e] * inv);
+  *reinterpret_cast<f16x4*>(a.out + (int64_t)b * a.ldo + h * D + d0) = v;
+  if (a.lse && dt == 0 && g8 == 0 && fk == 0) a.lse[(int64_t)h * a.M + b] = m + log2f(l);
+}
+
 // Row groups per block: 4 (128 packed rows), or 2 where a sequence has 64 packed rows or less on average.
 int flash_row_groups(int M, int B, int G) { return (int64_t)M * G <= 64 * (int64_t)B ? 2 : 4; }
 
@@ -510,33 +774,124 @@ int flash_slots(int M, int G, int Hkv, int RG, int cus) {
   return plan_budget(least, Hkv, cus) ? max(2 * cus / Hkv, 1) : 0;
 }
 
+// The work buffer begins with the arrival counters, in every call: one buffer may serve calls of all forms. Only pairs
+// with more than one split count, and those are fewer than two for each CU (decode_splits).
+constexpr int kCounters = 4096;
+constexpr size_t kWorkHead = kCounters * 4;
+
+void step_splits(int B, int Hkv, int G, int cus, StepPlan& f, bool& wide) {
+  f.S1 = decode_splits(B, Hkv, cus);
+  wide = G <= 8 && f.S1 >= kDaWideSplits;
+  if (wide) f.S = f.S1 = decode_splits_wide(B, Hkv, cus);
+  else f.S = decode_splits_max(B, Hkv, f.S1, cus);
+}
+// Floats of the partial results' m and l, a multiple of 4 (O is read in 16-byte pieces).
+size_t step_ml(const StepPlan& f, int B, int Hq) { return ((size_t)B * Hq * f.S * 2 + 3) & ~(size_t)3; }
+size_t step_bytes(const StepPlan& f, int B, int Hq, int D) { return (step_ml(f, B, Hq) + (size_t)B * Hq * f.S * D) * 4; }
+
+// Splits of a prefix of `shared` positions for T row tiles: a block for each CU.
+int prefix_splits(int T, int Hkv, int shared, int cus) {
+  return max(1, min(cus / max(1, T * Hkv), (shared + 255) / 256));
+}
+
+// Largest grid's blocks and what a kernel's LDS limit needs; 0, or a negative code.
+template <typename K>
+int flash_fits(K kern, int threads, size_t lds, const char* who) {
+  const int bpc = hi_blocks_per_cu(reinterpret_cast<const void*>(kern), threads, lds);  // lifts the LDS limit
+  if (bpc < 0) return -2;
+  if (bpc == 0) HI_FAIL("%s: the kernel does not fit on a CU", who);
+  return 0;
+}
+
 template <int D, int RG>
-int flash_launch(AttnArgs a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
+int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
   const int G = a.Hq / a.Hkv, cap = c.W << c.shift;
   FlashPlan f{nullptr, nullptr, 0, 0, 1};
   const int slots = cap > kPlanMinSplit ? flash_slots(a.M, G, a.Hkv, RG, cus) : 0;
   if (slots) {
     f.slots = slots;
     f.cus = cus;
-    f.ml = (float*)work;
+    f.ml = (float*)((char*)work + kWorkHead);
     f.po = f.ml + (size_t)slots * a.Hkv * 2 * 32 * RG;
   }
   // every sequence with rows has at most one part-filled tile
   const int64_t tiles = a.B == 1 ? plan_tiles(a.M, G, 32 * RG) : (int64_t)a.M * G / (32 * RG) + min(a.B, a.M);
   const int64_t blocks = max(tiles, (int64_t)slots) * a.Hkv, join = tiles * a.Hkv * RG * (D / 32);
   // (the tiles of any start, also one that gives the same rows to every sequence, are counted in int)
-  if (blocks > INT32_MAX || (slots && join > INT32_MAX) || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX) HI_FAIL("%s: %d rows are too many", who, a.M);
+  if (blocks > INT32_MAX || (slots && join > INT32_MAX) || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
+    HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
   const auto kern = attn_pages_kernel<D, RG, false>;
   const size_t lds = FpSmem<D, RG>::kBytes;
-  const int bpc = hi_blocks_per_cu(reinterpret_cast<const void*>(kern), 128 * RG, lds);  // lifts the LDS limit
-  if (bpc < 0) return -2;
-  if (bpc == 0) HI_FAIL("%s: the kernel does not fit on a CU", who);
+  if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
   if (slots) {
     hipLaunchKernelGGL((attn_join_kernel<D, RG>), dim3((unsigned)join), dim3(256), 0, s, a, cap, f);
     HI_TRY(hipGetLastError());
   }
+  return 0;
+}
+
+template <int D, bool OWN>
+int step_launch(const AttnArgs& a, const PagedCache& c, const StepPlan& f, bool wide, hipStream_t s, const char* who) {
+  const int64_t blocks = (int64_t)f.S * a.B * a.Hkv;
+  if (blocks > INT32_MAX) HI_FAIL("%s: %d sequences of %d kv heads are too many", who, a.B, a.Hkv);
+  const dim3 grid((unsigned)blocks);
+  const int G = a.Hq / a.Hkv;
+  if (G > 8) hipLaunchKernelGGL((attn_step_kernel<16, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f);
+  else if (G > 4) {
+    if (wide) hipLaunchKernelGGL((attn_step_kernel<8, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f);
+    else hipLaunchKernelGGL((attn_step_kernel<8, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f);
+  } else {
+    if (wide) hipLaunchKernelGGL((attn_step_kernel<4, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f);
+    else hipLaunchKernelGGL((attn_step_kernel<4, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f);
+  }
+  HI_TRY(hipGetLastError());
+  return 0;
+}
+
+template <int D>
+int step_run(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
+  StepPlan f;
+  bool wide;
+  step_splits(a.B, a.Hkv, a.Hq / a.Hkv, cus, f, wide);
+  f.counters = (int*)work;
+  f.ml = (float*)((char*)work + kWorkHead);
+  f.po = f.ml + step_ml(f, a.B, a.Hq);
+  return step_launch<D, false>(a, c, f, wide, s, who);
+}
+
+size_t shared_bytes(int B, int Hq, int Hkv, int D, int cus) {
+  StepPlan st;
+  bool wide;
+  step_splits(B, Hkv, Hq / Hkv, cus, st, wide);
+  const int RG = flash_row_groups(B, 1, Hq / Hkv), T = plan_tiles(B, Hq / Hkv, 32 * RG);
+  return step_bytes(st, B, Hq, D) + (size_t)T * max(1, cus / max(1, T * Hkv)) * Hkv * flash_slot_bytes(RG, D);
+}
+
+template <int D, int RG>
+int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
+  const int G = a.Hq / a.Hkv, cap = c.W << c.shift, T = plan_tiles(a.M, G, 32 * RG);
+  StepPlan st;
+  bool wide;
+  step_splits(a.B, a.Hkv, G, cus, st, wide);
+  st.counters = (int*)work;
+  st.ml = (float*)((char*)work + kWorkHead);
+  st.po = st.ml + step_ml(st, a.B, a.Hq);
+  FlashPlan f{nullptr, nullptr, 0, 0, prefix_splits(T, a.Hkv, a.shared, cus)};
+  f.slots = T * f.splits;
+  f.ml = st.po + (size_t)a.B * a.Hq * st.S * D;
+  f.po = f.ml + (size_t)f.slots * a.Hkv * 2 * 32 * RG;
+  const int64_t blocks = (int64_t)f.slots * a.Hkv, join = (int64_t)T * a.Hkv * RG * (D / 32);
+  if (blocks > INT32_MAX || join > INT32_MAX) HI_FAIL("%s: %d sequences are too many", who, a.B);
+  const auto kern = attn_pages_kernel<D, RG, true>;
+  const size_t lds = FpSmem<D, RG>::kBytes;
+  if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
+  HI_TRY(hipGetLastError());
+  if (const int rc = step_launch<D, true>(a, c, st, wide, s, who)) return rc;
+  hipLaunchKernelGGL((attn_shared_join_kernel<D, RG>), dim3((unsigned)join), dim3(256), 0, s, a, cap, f, st);
+  HI_TRY(hipGetLastError());
   return 0;
 }
 
@@ -553,16 +908,24 @@ int attn_check(const char* who, const void* q, int ldq, const int* pos, const vo
 }
 
 int attn_run(const AttnArgs& a, const PagedCache& c, int D, int cus, void* work, hipStream_t s, const char* who) {
+  const int G = a.Hq / a.Hkv;
   if (a.start) {
-    const bool small = flash_row_groups(a.M, a.B, a.Hq / a.Hkv) == 2;
+    const bool small = flash_row_groups(a.M, a.B, G) == 2;
     return D == 64 ? (small ? flash_launch<64, 2>(a, c, cus, work, s, who) : flash_launch<64, 4>(a, c, cus, work, s, who))
                    : (small ? flash_launch<128, 2>(a, c, cus, work, s, who) : flash_launch<128, 4>(a, c, cus, work, s, who));
   }
-  const dim3 grid(a.M, a.Hq);
-  if (D == 64) hipLaunchKernelGGL(attn_paged_simple_kernel<64>, grid, dim3(256), 0, s, a, c);
-  else hipLaunchKernelGGL(attn_paged_simple_kernel<128>, grid, dim3(256), 0, s, a, c);
-  HI_TRY(hipGetLastError());
-  return 0;
+  if (a.shared) {
+    const bool small = flash_row_groups(a.M, 1, G) == 2;
+    return D == 64 ? (small ? shared_launch<64, 2>(a, c, cus, work, s, who) : shared_launch<64, 4>(a, c, cus, work, s, who))
+                   : (small ? shared_launch<128, 2>(a, c, cus, work, s, who) : shared_launch<128, 4>(a, c, cus, work, s, who));
+  }
+  return D == 64 ? step_run<64>(a, c, cus, work, s, who) : step_run<128>(a, c, cus, work, s, who);
+}
+
+// Sizes of a work buffer's call that the attention can take.
+bool work_sizes(int M, int B, int Hq, int Hkv, int D) {
+  return M >= 0 && B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16 && (D == 64 || D == 128) &&
+         (int64_t)max(M, B) * Hq <= (1 << 27);
 }
 
 }  // namespace
@@ -590,11 +953,16 @@ HI_EXPORT int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int
 
 HI_EXPORT size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged) {
   const HiDevice* d = hi_device();
-  if (!d || M < 0 || B < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || Hq / Hkv > 16 || (D != 64 && D != 128) || (int64_t)M * Hq > (1 << 27))
-    return 0;
-  if (!ragged) return 16;
-  const int RG = flash_row_groups(M, B, Hq / Hkv);
-  return 16 + (size_t)flash_slots(M, Hq / Hkv, Hkv, RG, d->cus) * Hkv * flash_slot_bytes(RG, D);
+  if (!d || !work_sizes(M, B, Hq, Hkv, D)) return 0;
+  if (M == 0 || B == 0) return kWorkHead;
+  if (ragged) {
+    const int RG = flash_row_groups(M, B, Hq / Hkv);
+    return kWorkHead + (size_t)flash_slots(M, Hq / Hkv, Hkv, RG, d->cus) * Hkv * flash_slot_bytes(RG, D);
+  }
+  StepPlan f;
+  bool wide;
+  step_splits(B, Hkv, Hq / Hkv, d->cus, f, wide);
+  return kWorkHead + step_bytes(f, B, Hq, D);
 }
 
 HI_EXPORT int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages,
@@ -617,8 +985,9 @@ HI_EXPORT int hi_attn_paged(const void* q, int ldq, const void* kp, const void* 
 }
 
 HI_EXPORT size_t hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D) {
-  (void)B, (void)Hq, (void)Hkv, (void)D;
-  return 16;
+  const HiDevice* d = hi_device();
+  if (!d || !work_sizes(B, B, Hq, Hkv, D)) return 0;
+  return kWorkHead + (B == 0 ? 0 : shared_bytes(B, Hq, Hkv, D, d->cus));
 }
 
 HI_EXPORT int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages,
