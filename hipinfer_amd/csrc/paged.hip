@@ -64,6 +64,69 @@ __global__ void __launch_bounds__(256) rope_paged_any_kernel(RopePagedArgs a, Pa
   }
 }
 
+// 16-byte accesses: a step turns 8 pairs (the 8 elements at d and the 8 at d + rot / 2, or 8 interleaved ones: 4 pairs) or
+// copies 8 elements; block per row, a thread per step up to 512. `per` steps a q or k head, `turns` of them rotate. The row is
+// requested before its place is known (position, table entry and cs row are a chain of three loads).
+template <typename CS, bool INTER>
+__global__ void __launch_bounds__(512) rope_paged_kernel(RopePagedArgs a, PagedCache c, int per, int turns) {
+  constexpr int NP = INTER ? 4 : 8;  // pairs of a step
+  const int m = blockIdx.x, nrot = (a.Hq + a.Hkv) * per, n = nrot + a.Hkv * a.D / 8, half = a.rot / 2;
+  const f16* row = a.qkv + (int64_t)m * a.ldq;
+  int i = threadIdx.x, h, d;
+  bool turning;
+  f16x8 x, y;
+  auto load = [&] {
+    turning = false;
+    if (i < nrot) {
+      h = i / per;
+      const int j = i - h * per;
+      turning = j < turns;
+      d = turning ? 8 * j : a.rot + 8 * (j - turns);
+    } else {
+      const int j = i - nrot, w = a.D / 8;
+      h = j / w;
+      d = 8 * (j - h * w);
+      h += a.Hq + a.Hkv;
+    }
+    const f16* src = row + h * a.D + d;
+    x = *reinterpret_cast<const f16x8*>(src);
+    if (!INTER && turning) y = *reinterpret_cast<const f16x8*>(src + half);
+  };
+  if (i < n) load();
+  int p;
+  const int64_t at = rope_place(a, c, m, p);
+  if (at < 0) return;
+  const int page = 1 << c.shift;
+  while (i < n) {
+    f16* dst = h < a.Hq ? a.qo + (int64_t)m * a.ldqo + h * a.D
+               : h < a.Hq + a.Hkv ? const_cast<f16*>(c.kp) + at + (int64_t)(h - a.Hq) * page * a.D
+                                  : const_cast<f16*>(c.vp) + at + (int64_t)(h - a.Hq - a.Hkv) * page * a.D;
+    if (turning) {
+      const CS* tab = (const CS*)a.cs + (int64_t)p * a.rot + (INTER ? d : 2 * d);
+      CS t[2 * NP];
+#pragma unroll
+      for (int k = 0; k < (int)(2 * NP * sizeof(CS) / 16); k++)
+        reinterpret_cast<u32x4*>(t)[k] = reinterpret_cast<const u32x4*>(tab)[k];
+#pragma unroll
+      for (int k = 0; k < NP; k++) {
+        f16 u = INTER ? x[2 * k] : x[k], v = INTER ? x[2 * k + 1] : y[k];
+        turn(u, v, (float)t[2 * k], (float)t[2 * k + 1]);
+        if constexpr (INTER) {
+          x[2 * k] = u;
+          x[2 * k + 1] = v;
+        } else {
+          x[k] = u;
+          y[k] = v;
+        }
+      }
+      if constexpr (!INTER) *reinterpret_cast<f16x8*>(dst + d + half) = y;
+    }
+    *reinterpret_cast<f16x8*>(dst + d) = x;
+    i += blockDim.x;
+    if (i < n) load();
+  }
+}
+
 // ------------------------------------------------------------------ attention
 struct AttnArgs {
   const f16* q;
@@ -945,8 +1008,20 @@ HI_EXPORT int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int
     HI_FAIL("%s: a null or misaligned pointer, ldq < (Hq + 2 Hkv) D or q_out's row stride < Hq D", who);
   if (!hi_device()) return -2;
   const RopePagedArgs a{(f16*)qkv, ldq, (f16*)q_out, ldqo, Hq, Hkv, D, rot, cs_rows, B, cs, seq, pos};
-  if (cs_f32) hipLaunchKernelGGL(rope_paged_any_kernel<float>, dim3(M), dim3(256), 0, (hipStream_t)stream, a, c, interleaved != 0);
-  else hipLaunchKernelGGL(rope_paged_any_kernel<f16>, dim3(M), dim3(256), 0, (hipStream_t)stream, a, c, interleaved != 0);
+  const hipStream_t s = (hipStream_t)stream;
+  const bool v8 = rot % (interleaved ? 8 : 16) == 0 && ldq % 8 == 0 && ldqo % 8 == 0 &&
+                  (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)cs) & 15) == 0;
+  if (v8) {
+    const int turns = rot / (interleaved ? 8 : 16), per = turns + (D - rot) / 8;
+    const int steps = (Hq + Hkv) * per + Hkv * D / 8;
+    const dim3 block(min(512, (steps + 63) & ~63));
+    const auto kern = cs_f32 ? (interleaved ? rope_paged_kernel<float, true> : rope_paged_kernel<float, false>)
+                             : (interleaved ? rope_paged_kernel<f16, true> : rope_paged_kernel<f16, false>);
+    hipLaunchKernelGGL(kern, dim3(M), block, 0, s, a, c, per, turns);
+  } else {
+    const auto kern = cs_f32 ? rope_paged_any_kernel<float> : rope_paged_any_kernel<f16>;
+    hipLaunchKernelGGL(kern, dim3(M), dim3(256), 0, s, a, c, interleaved != 0);
+  }
   HI_TRY(hipGetLastError());
   return 0;
 }

@@ -36,6 +36,8 @@ lib = ctypes.CDLL(LIBRARY_PATH)
 # instead of all experts; routing weights rounded to fp16.
 MOE_NORM_TOPK = 1
 MOE_FP16_WEIGHTS = 2
+# The front of the paged attention's work buffers, to be zeroed once.
+ATTN_COUNTER_BYTES = 16384
 
 # ------------------------------------------------------------------ the C-ABI, as prototypes
 ABI = """
@@ -416,44 +418,60 @@ def flash_prefill_lse(q, kc, vc, T, p0, Hq, Hkv, out=None, lse=None):
 
 
 # ------------------------------------------------------------------ paged key/value cache
-def _paged(what, kp, vp, table, *others):
-    """Checks a paged cache kp / vp [pages, Hkv, page, D] and its table [B, W], and that every tensor of the call is on
-    the current device; returns the cache's arguments of a library call, and (Hkv, page, D)."""
-    for t in (kp, vp):
-        _need(what, t, torch.float16, 4)
-    _need(what, table, torch.int32, 2)
-    gpu = torch.cuda.current_device()
-    for t in (kp, vp, table, *others):
+# These wrappers are half of a small call's time, so their checks read each property once and compare tuples; what fails is
+# looked at again for the message.
+def _on_device(what, *tensors):
+    """Every tensor (None aside) on the current device: the library launches there."""
+    gpu = tensors[0].get_device()
+    for t in tensors:
         if t is not None and t.get_device() != gpu:
-            raise ValueError(f"hipinfer_amd.{what}: every tensor must be on the current device (cuda:{gpu}), got {t.device}")
-    pages, Hkv, page, D = kp.shape
-    B, W = table.shape
-    if vp.shape != kp.shape:
-        raise ValueError(f"hipinfer_amd.{what}: kp {tuple(kp.shape)} and vp {tuple(vp.shape)} must have the same shape")
-    step = kp.stride(0)
-    if pages > 1 and vp.stride(0) != step:
-        raise ValueError(f"hipinfer_amd.{what}: kp and vp must have the same page stride")
-    for t in (kp, vp):
-        for n, have, want in zip(t.shape[1:], t.stride()[1:], (page * D, D, 1)):
-            if n > 1 and have != want:
+            raise ValueError(f"hipinfer_amd.{what}: tensors on {tensors[0].device} and {t.device}")
+    if gpu < 0 or gpu != torch._C._cuda_getDevice():
+        raise ValueError(f"hipinfer_amd.{what}: tensors must live on the current GPU (got {tensors[0].device})")
+
+
+def _paged(what, kp, vp, table, Hkv):
+    """Checks a paged cache kp / vp [pages, Hkv, page, D] and its table [B, W]; returns the cache's arguments of a library
+    call, B and D."""
+    _need(what, kp, torch.float16, 4)
+    shape, steps, tshape = kp.shape, kp.stride(), table.shape
+    pages, heads, page, D = shape
+    if vp.dtype is not torch.float16 or vp.shape != shape:
+        raise ValueError(f"hipinfer_amd.{what}: kp {tuple(shape)} and vp {tuple(vp.shape)} must have the same shape, in fp16")
+    if table.dtype is not torch.int32 or len(tshape) != 2:
+        raise ValueError(f"hipinfer_amd.{what}: the table must be int32 [B, W], got {table.dtype} {tuple(tshape)}")
+    if heads != Hkv:
+        raise ValueError(f"hipinfer_amd.{what}: a cache of {heads} heads for Hkv {Hkv}")
+    packed, vsteps = (page * D, D, 1), vp.stride()
+    if steps != vsteps or steps[1:] != packed:  # strides of dimensions of size 1 say nothing
+        for st in (steps, vsteps):
+            if any(n > 1 and have != want for n, have, want in zip(shape[1:], st[1:], packed)):
                 raise ValueError(f"hipinfer_amd.{what}: a page [Hkv, page, D] must be packed")
-    if W > 1 and table.stride(1) != 1:
+        if pages > 1 and vsteps[0] != steps[0]:
+            raise ValueError(f"hipinfer_amd.{what}: kp and vp must have the same page stride")
+    B, W = tshape
+    ldt, one = table.stride()
+    if one != 1 and W > 1:
         raise ValueError(f"hipinfer_amd.{what}: table rows must be contiguous")
-    ldt = table.stride(0) if B > 1 else W
-    return ((_addr(kp), _addr(vp), step if pages > 1 else Hkv * page * D, pages, page, _addr(table), ldt, W),
-            (Hkv, page, D))
+    return (kp.data_ptr(), vp.data_ptr(), steps[0] if pages > 1 else Hkv * page * D, pages, page, table.data_ptr(),
+            ldt if B > 1 else W, W), B, D
 
 
-def _row_stride(t, width):
-    """The row stride of a 2-dimensional tensor; a single row's is its width."""
-    return t.stride(0) if t.shape[0] > 1 else width
+def _rows_of(what, name, t, M, width):
+    """An fp16 [M, >= width] tensor of contiguous rows; returns its row stride (a single row's is its width)."""
+    shape = t.shape
+    if t.dtype is not torch.float16 or len(shape) != 2 or shape[0] != M or shape[1] < width:
+        raise ValueError(f"hipinfer_amd.{what}: {name} must be fp16 [{M}, {width}], got {t.dtype} {tuple(shape)}")
+    step, one = t.stride()
+    if one != 1 and shape[1] > 1:
+        raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous")
+    return step if M > 1 else shape[1]
 
 
-def _vector(what, t, n, name, optional=False):
+def _vector(what, name, t, n):
     """A packed int32 vector of n entries."""
-    _need(what, t, torch.int32, 1, optional=optional)
-    if t is not None and (t.shape[0] != n or (n > 1 and t.stride(0) != 1)):
-        raise ValueError(f"hipinfer_amd.{what}: {name} must be a packed vector of {n}, got shape {tuple(t.shape)}")
+    if t.dtype is not torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"hipinfer_amd.{what}: {name} must be a packed int32 vector of {n}, got {t.dtype} {tuple(t.shape)}")
 
 
 def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved=False, q_out=None):
@@ -470,56 +488,57 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
     A row that has no place is left out, its q too: a negative position (padding), one behind its table row or cs,
     a seq outside the table, a page id outside [0, pages). Rows of one call must have places of their own."""
     what = "rope_cache_paged"
-    _need(what, qkv, torch.float16, 2, rows=True)
-    cache, (heads, page, D) = _paged(what, kp, vp, table, qkv, cs, pos, seq, q_out)
-    M, width = qkv.shape
-    if heads != Hkv or Hq < 1 or width < (Hq + 2 * Hkv) * D:
-        raise ValueError(f"hipinfer_amd.{what}: rows of {width} and a cache of {heads} heads for Hq {Hq}, Hkv {Hkv}, D {D}")
-    _need(what, cs, ndim=3)
-    if cs.dtype not in (torch.float16, torch.float32) or cs.shape[2] != 2 or not cs.is_contiguous():
+    _on_device(what, qkv, cs, kp, vp, table, pos, seq, q_out)
+    cache, B, D = _paged(what, kp, vp, table, Hkv)
+    M = qkv.shape[0]
+    ldq = _rows_of(what, "qkv", qkv, M, (Hq + 2 * Hkv) * D)
+    cshape, wide = cs.shape, cs.dtype is torch.float32
+    if not (wide or cs.dtype is torch.float16) or len(cshape) != 3 or cshape[2] != 2 or not cs.is_contiguous():
         raise ValueError(f"hipinfer_amd.{what}: cs must be packed [positions, rot/2, 2], fp16 or fp32")
-    _vector(what, pos, M, "pos")
-    _vector(what, seq, M, "seq", optional=True)
-    if seq is None and M > table.shape[0]:
+    _vector(what, "pos", pos, M)
+    if seq is not None:
+        _vector(what, "seq", seq, M)
+    elif M > B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows without seq need a table of as many sequences")
     if q_out is None:
-        q_out = qkv
+        q_out, ldo = qkv, ldq
     else:
-        _need(what, q_out, torch.float16, 2, rows=True)
-        if q_out.shape[0] != M or q_out.shape[1] < Hq * D:
-            raise ValueError(f"hipinfer_amd.{what}: q_out must be [{M}, {Hq * D}], got {tuple(q_out.shape)}")
-    check_rc(lib.hi_rope_cache_paged(_addr(qkv), _row_stride(qkv, width), _addr(q_out), _row_stride(q_out, q_out.shape[1]),
-                                     M, Hq, Hkv, D, _addr(cs), cs.shape[0], int(cs.dtype == torch.float32),
-                                     2 * cs.shape[1], int(interleaved), _addr(seq), _addr(pos), *cache, table.shape[0],
-                                     _stream()), what)
+        ldo = _rows_of(what, "q_out", q_out, M, Hq * D)
+    check_rc(lib.hi_rope_cache_paged(qkv.data_ptr(), ldq, q_out.data_ptr(), ldo, M, Hq, Hkv, D, cs.data_ptr(), cshape[0],
+                                     wide, 2 * cshape[1], interleaved, _addr(seq), pos.data_ptr(), *cache, B, _stream()),
+             what)
 
 
-def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, start=None):
-    """Checks what attn_paged and attn_shared have in common; returns (cache, D, out)."""
-    _need(what, q, torch.float16, 2, rows=True)
-    cache, (heads, page, D) = _paged(what, kp, vp, table, q, pos, start, out, lse, work)
+def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work):
+    """Checks what attn_paged and attn_shared have in common; returns the cache's arguments, M, B, D, q's row stride, out
+    and its row stride."""
+    cache, B, D = _paged(what, kp, vp, table, Hkv)
     M = q.shape[0]
-    if heads != Hkv or Hq < 1 or q.shape[1] < Hq * D:
-        raise ValueError(f"hipinfer_amd.{what}: rows of {q.shape[1]} and a cache of {heads} heads for Hq {Hq}, Hkv {Hkv}, D {D}")
-    _vector(what, pos, table.shape[0], "pos")
+    ldq = _rows_of(what, "q", q, M, Hq * D)
+    _vector(what, "pos", pos, B)
     if out is None:
         out = _alloc_rows(q, M, Hq * D)
-    _need(what, out, torch.float16, 2, rows=True)
-    if out.shape[0] != M or out.shape[1] < Hq * D:
-        raise ValueError(f"hipinfer_amd.{what}: out must be [{M}, {Hq * D}], got {tuple(out.shape)}")
-    if lse is not None:
-        _need(what, lse, torch.float32, 2)
-        if lse.shape != (Hq, M) or not lse.is_contiguous():
-            raise ValueError(f"hipinfer_amd.{what}: lse must be packed [{Hq}, {M}]")
-    if work is not None:
-        _need(what, work, torch.uint8, 1, rows=work.numel() > 1)
-    return cache, D, out
+    ldo = _rows_of(what, "out", out, M, Hq * D)
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (Hq, M) or not lse.is_contiguous()):
+        raise ValueError(f"hipinfer_amd.{what}: lse must be packed fp32 [{Hq}, {M}]")
+    if work is not None and (work.dtype is not torch.uint8 or not work.is_contiguous()):
+        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8")
+    return cache, M, B, D, ldq, out, ldo
+
+
+def _attn_work(what, size):
+    """A work buffer: the arrival counters at its front start at zero, the rest may hold anything."""
+    if size == 0:
+        raise ValueError(f"hipinfer_amd.{what}: unsupported sizes")
+    work = torch.empty(size, dtype=torch.uint8, device="cuda")
+    work[:ATTN_COUNTER_BYTES].zero_()
+    return work
 
 
 def attn_paged_work(rows, seqs, Hq, Hkv, D, ragged=False):
-    """The work buffer of attn_paged for up to `rows` rows (ragged: with start), zeroed; calls that use one buffer must
-    not overlap in time."""
-    return torch.zeros(lib.hi_attn_paged_work_bytes(rows, seqs, Hq, Hkv, D, int(ragged)), dtype=torch.uint8, device="cuda")
+    """A work buffer of attn_paged for `rows` rows of `seqs` sequences (ragged: with start). It serves any later call of
+    attn_paged or attn_shared that needs no more bytes; calls that use one buffer must not overlap in time."""
+    return _attn_work("attn_paged_work", lib.hi_attn_paged_work_bytes(rows, seqs, Hq, Hkv, D, int(ragged)))
 
 
 def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, work=None):
@@ -535,23 +554,22 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     base-2 log-sum-exp of each row's scaled logits (-inf without keys). `work` (attn_paged_work) can be kept
     across calls; everything the call reads of pos, start and table is read on the device, so it can be captured."""
     what = "attn_paged"
-    cache, D, out = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, start)
-    M, B = q.shape[0], table.shape[0]
+    _on_device(what, q, kp, vp, table, pos, start, out, lse, work)
+    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
     if start is not None:
-        _vector(what, start, B + 1, "start")
+        _vector(what, "start", start, B + 1)
     elif M != B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences (one row each without start)")
     if work is None:
         work = attn_paged_work(M, B, Hq, Hkv, D, start is not None)
-    check_rc(lib.hi_attn_paged(_addr(q), _row_stride(q, q.shape[1]), *cache, _addr(start), _addr(pos), _addr(out),
-                               _row_stride(out, out.shape[1]), _addr(lse), M, B, Hq, Hkv, D, _addr(work), work.numel(),
-                               _stream()), what)
+    check_rc(lib.hi_attn_paged(q.data_ptr(), ldq, *cache, _addr(start), pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), M,
+                               B, Hq, Hkv, D, work.data_ptr(), work.numel(), _stream()), what)
     return out
 
 
 def attn_shared_work(seqs, Hq, Hkv, D):
-    """The work buffer of attn_shared, zeroed; calls that use one buffer must not overlap in time."""
-    return torch.zeros(lib.hi_attn_shared_work_bytes(seqs, Hq, Hkv, D), dtype=torch.uint8, device="cuda")
+    """A work buffer of attn_shared for `seqs` sequences, as attn_paged_work's."""
+    return _attn_work("attn_shared_work", lib.hi_attn_shared_work_bytes(seqs, Hq, Hkv, D))
 
 
 def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work=None):
@@ -560,15 +578,14 @@ def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work
     result as attn_paged where every row of table begins with those pages; a sequence may also be shorter than the
     shared part."""
     what = "attn_shared"
-    cache, D, out = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
-    B = q.shape[0]
-    if B != table.shape[0]:
-        raise ValueError(f"hipinfer_amd.{what}: {B} rows for a table of {table.shape[0]} sequences")
+    _on_device(what, q, kp, vp, table, pos, out, lse, work)
+    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
+    if M != B:
+        raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences")
     if work is None:
         work = attn_shared_work(B, Hq, Hkv, D)
-    check_rc(lib.hi_attn_shared(_addr(q), _row_stride(q, q.shape[1]), *cache, shared, _addr(pos), _addr(out),
-                                _row_stride(out, out.shape[1]), _addr(lse), B, Hq, Hkv, D, _addr(work), work.numel(),
-                                _stream()), what)
+    check_rc(lib.hi_attn_shared(q.data_ptr(), ldq, *cache, shared, pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), B, Hq,
+                                Hkv, D, work.data_ptr(), work.numel(), _stream()), what)
     return out
 
 

@@ -175,7 +175,8 @@ int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int M, int Hq
                         void* vp, long long page_stride, int pages, int page, const int* table, int ldt, int W, int B,
                         void* stream);
 /* Bytes of hi_attn_paged's work buffer for M rows of B sequences on the current device (ragged: calls with start);
- * 0 for bad sizes. Zeroed once by the caller, left fit for the next call by every call. */
+ * 0 for bad sizes. Its first 16384 bytes are zeroed once by the caller and left zero by every call; one buffer serves
+ * calls of hi_attn_paged and hi_attn_shared in turn, of any sizes that it is large enough for. */
 size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged);
 /* Causal attention over the paged cache: start NULL, row b of q [M, ldq] at position pos[b] of sequence b (M == B); else
  * rows start[b] .. start[b + 1] - 1 at positions pos[b], pos[b] + 1, ... of sequence b (start [B + 1], not
