@@ -5,6 +5,7 @@
 //   nt, n_full                                   key tiles, and how many at the front hold no masked key for this wave
 //   issue_k(i, st), issue_v(i, st)               DMA instruction i of the next K (V) tile into stage st
 //   advance()                                    called once before the DMA of each K tile but the first
+//   before_barrier(), after_barrier()            called around the prologue's barrier, before n_full is read
 //   enter_masked(t), hidden(t, kt, e)            whether the lane's query does not see element e of key block kt of tile t
 //   xor32(v)                                     lane l ^ 32's v
 //   m_i, l_i, o                                  the row's reference max (-inf), the lane's share of its sum (0), O^T (0)
@@ -229,8 +230,10 @@
     issue_v(i, 0);
     issue_k(i, 1);
   }
+  before_barrier();
   wait_vmcnt<2 * IPW>();
   barrier_no_fence();
+  after_barrier();
   f32x16 sa[2], sb[2];
   logits(0, 0, sa[0]);
   logits(0, 1, sa[1]);

@@ -152,38 +152,63 @@ struct AttnArgs {
 //    the masked tile for all of its keys, and hides them there.
 // Where the row tiles are fewer than the GPU's CUs, their keys are split (paged_plan.h); a split stores its
 // unnormalised O, m and l in fp32, in the lanes' order, and attn_join_kernel joins them.
+struct TileNote;
 struct FlashPlan {
+  int* tiles;      // row tiles of the batch, and their notes
+  TileNote* notes;
   float *ml, *po;  // partial results: [slot][2][BQ] m and l, [slot][RG][D / 8][64][4] O
   int slots;       // slots there are, each of all kv heads
   int cus;         // > 0: split over that many
   int splits;      // of the shared prefix
+  int most;        // notes there are
 };
 
 // What a block works on; found by every wave by itself from start and pos.
 struct FlashUnit {
   int b, row0, n, pos;   // sequence, its first row, rows, first position
   int tile, splits, split, slot;  // slot of split 0 (meaningful with splits > 1)
+  int note;                       // the tile's number in the batch (where keys may be split)
 };
 
+// What a row tile's join needs, written by the block of its first split (kv head 0).
+struct TileNote {
+  int row0, rows, first, splits, slot, pad[3];  // first row of the run, packed rows of the tile, its first packed row
+};
+
+// Integer reductions over a whole wave in DPP moves (a __shfl_xor is an LDS round trip, and a plan has dozens).
+template <int CTRL>
+__device__ __forceinline__ int dpp_or(int old, int v) {  // lanes without a source get `old`
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, 0xF, 0xF, false);
+}
 __device__ __forceinline__ int wave_total(int v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+  v += dpp_or<0xB1>(0, v);   // quad_perm [1,0,3,2]
+  v += dpp_or<0x4E>(0, v);   // quad_perm [2,3,0,1]
+  v += dpp_or<0x141>(0, v);  // row_half_mirror
+  v += dpp_or<0x140>(0, v);  // row_mirror
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+         __builtin_amdgcn_readlane(v, 48);
 }
-__device__ __forceinline__ int64_t wave_total(int64_t v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+__device__ __forceinline__ int wave_most(int v) {
+  v = max(v, dpp_or<0xB1>(v, v));
+  v = max(v, dpp_or<0x4E>(v, v));
+  v = max(v, dpp_or<0x141>(v, v));
+  v = max(v, dpp_or<0x140>(v, v));
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, kWave);
-    if (lane >= o) v += u;
-  }
-  return v;
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum
+  v += dpp_or<0x111>(0, v);  // row_shr 1, 2, 4, 8
+  v += dpp_or<0x112>(0, v);
+  v += dpp_or<0x114>(0, v);
+  v += dpp_or<0x118>(0, v);
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
+  return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
 }
 
-// Unit `at` of the batch, or with TILES row tile `at` (split 0 of it); false if there are not so many. Wave-uniform.
-template <int BQ, bool TILES>
-__device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const FlashPlan& f, int at, int lane, FlashUnit& u) {
+// Unit `at` of the batch; false if there are not so many. Wave-uniform. T: row tiles of the batch.
+template <int BQ>
+__device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const FlashPlan& f, int at, int lane, FlashUnit& u,
+                                           int& T) {
   const int G = a.Hq / a.Hkv;
   struct Seq { int row0, n, pos, tiles, end; };
   auto seq = [&](int b) {
@@ -200,21 +225,21 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
   };
   int L = kPlanNoSplit;
   const Seq first = seq(lane);
+  T = 0;
   if (f.cus > 0) {
-    int T = 0, longest = 0;
-    int64_t work = 0;
+    int longest = 0;
+    uint32_t work = 0;  // in key tiles; under the budget's T < 2 cus it does not overflow
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       const Seq s = b0 ? seq(b0 + lane) : first;
       T += s.tiles;
-      work += (int64_t)s.tiles * s.end;
+      work += (uint32_t)s.tiles * plan_key_tiles(s.end);
       if (s.tiles) longest = max(longest, s.end);
     }
     T = wave_total(T);
     const int budget = plan_budget(T, a.Hkv, f.cus);
     if (budget > 0) {
-      work = wave_total(work);
-      for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, kWave));
-      for (L = plan_length(work, budget); L < longest; L = plan_longer(L)) {
+      longest = wave_most(longest);
+      for (L = plan_length((uint32_t)wave_total((int)work), budget); L < longest; L = plan_longer(L)) {
         int units = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
           const Seq s = b0 ? seq(b0 + lane) : first;
@@ -224,13 +249,14 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
       }
     }
   }
-  int before = 0, slot = 0;
+  int before = 0, tiles_before = 0, slot = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const Seq s = b0 ? seq(b0 + lane) : first;
     const int splits = plan_splits(s.end, L);
-    const int n = TILES ? s.tiles : s.tiles * splits, own = splits > 1 ? s.tiles * splits : 0;
-    const int upto = wave_scan(n, lane), slots = wave_scan(own, lane);
+    const int n = s.tiles * splits, own = splits > 1 ? n : 0;
+    const int upto = wave_scan(n, lane);
     const uint64_t hit = __ballot(before + upto > at);
+    const int slots = f.cus > 0 ? wave_scan(own, lane) : 0, tiles_upto = f.cus > 0 ? wave_scan(s.tiles, lane) : 0;
     if (hit) {
       const int l = __builtin_ctzll(hit);
       auto take = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
@@ -240,13 +266,15 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
       u.pos = take(s.pos);
       u.splits = take(splits);
       const int tiles = take(s.tiles), i = at - before - (take(upto) - take(n));
-      u.tile = tiles - 1 - (TILES ? i : i / u.splits);  // the most keys first
-      u.split = TILES ? 0 : i % u.splits;
+      u.tile = tiles - 1 - i / u.splits;  // the most keys first
+      u.split = i % u.splits;
       u.slot = slot + take(slots) - take(own) + u.tile * u.splits;
+      u.note = tiles_before + take(tiles_upto) - tiles + u.tile;
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     slot += __builtin_amdgcn_readlane(slots, 63);
+    tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
   }
   return false;
 }
@@ -276,21 +304,33 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   const int G = a.Hq / a.Hkv, page = 1 << c.shift, cap = c.capacity();
   const int hk = blockIdx.x % a.Hkv;            // blocks of a kv head on as few XCDs as there can be
   FlashUnit u;
-  int end;  // keys that some row of the tile sees
+  int end;     // keys that some row of the tile sees
+  int kb, ke;  // the split's
+  // of the next key tile to be located: this lane's group of 8 keys, and its page
+  int key = wave * KPW + 8 * (lane & (NG - 1)), id;
   if constexpr (PREFIX) {
-    u = FlashUnit{0, 0, a.M, 0, (int)(blockIdx.x / a.Hkv) / f.splits, f.splits, (int)(blockIdx.x / a.Hkv) % f.splits, 0};
+    u = FlashUnit{0, 0, a.M, 0, (int)(blockIdx.x / a.Hkv) / f.splits, f.splits, (int)(blockIdx.x / a.Hkv) % f.splits, 0, 0};
     u.slot = u.tile * f.splits;
+    plan_range(a.shared, u.splits, u.split, kb, ke);
+    key += kb;
+    id = key < ke ? c.entry(0, key >> c.shift) : -1;  // requested together with the positions
     int most = -1;  // the last position of any of the tile's rows
     for (int i = u.tile * BQ + lane; i < min((u.tile + 1) * BQ, u.n * G); i += 64) most = max(most, a.pos[i / G]);
-    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, kWave));
-    end = __builtin_amdgcn_readfirstlane(max(min(most, a.shared - 1), -1) + 1);
+    end = max(min(wave_most(most), a.shared - 1), -1) + 1;
   } else {
-    if (!flash_unit<BQ, false>(a, cap, f, blockIdx.x / a.Hkv, lane, u)) return;
+    int T;
+    const bool any = flash_unit<BQ>(a, cap, f, blockIdx.x / a.Hkv, lane, u, T);
+    // (more tiles than notes are not split, or come of a start that gives rows to several sequences)
+    if (f.cus > 0 && blockIdx.x == 0 && tid == 0) *f.tiles = T <= f.most ? T : 0;
+    if (!any) return;
     end = plan_tile_end(u.pos, u.n, u.tile, G, BQ, cap);
+    plan_range(end, u.splits, u.split, kb, ke);
+    key += kb;
+    id = key < ke ? c.entry(u.b, key >> c.shift) : -1;
+    if (f.cus > 0 && hk == 0 && u.split == 0 && tid == 0 && u.note < f.most)
+      f.notes[u.note] = TileNote{u.row0, min(BQ, u.n * G - u.tile * BQ), u.tile * BQ, u.splits, u.slot, {}};
   }
-  int kb, kv_end;
-  plan_range(PREFIX ? a.shared : end, u.splits, u.split, kb, kv_end);
-  kv_end = min(kv_end, end);
+  const int kv_end = min(ke, end);
   const int nt = kv_end > kb ? (kv_end - kb + kFpBKV - 1) / kFpBKV : 0;
 
   // this lane's row and the last key it sees
@@ -321,13 +361,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
       if (row) v = *reinterpret_cast<const u32x4*>(a.q + qrow * a.ldq + h * D + 16 * ks + 8 * fk);
       qf[ks] = __builtin_bit_cast(f16x8, v);
     }
-    // whether some key of the block lies on no page
     const int tb = PREFIX ? 0 : u.b;  // table row
-    bool hole = false;
-    for (int i = (kb >> c.shift) + tid; i <= (kv_end - 1) >> c.shift; i += 128 * RG) hole |= !c.has(c.entry(tb, i));
-    const bool any_hole = __any(hole);
-    if (lane == 0) flag[wave] = any_hole;
-
     // DMA instruction i of this wave fills slots (wave IPW + i) * 64 + lane of a tile: slot s holds
     // key s / CPR, physical chunk s % CPR, i.e. logical chunk (s % CPR) ^ swz(key)
     int koff[IPW], voff[IPW];
@@ -340,7 +374,6 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
     // the groups' byte offsets in kp / vp and readable bytes: of the next K tile, and of the next V tile (one before)
     uint32_t klo[NG], khi[NG], vlo[NG], vhi[NG];
     int kn[NG], vn[NG];
-    int key = kb + wave * KPW + 8 * (lane & (NG - 1)), id = -1;  // of the tile after: this lane's group and its page
     auto fetch = [&] { id = key < kv_end ? c.entry(tb, key >> c.shift) : -1; };
     auto take = [&] {
       const bool ok = c.has(id);
@@ -375,24 +408,33 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
     auto issue_v = [&](int i, int st) {
       lds_dma16(group(c.vp, vlo[i / IPG], vhi[i / IPG], vn[i / IPG]), vs_ + st * Sm::kTile + (wave * IPW + i) * 64, voff[i]);
     };
-    fetch();
     take();
     fetch();
-
-    __syncthreads();  // every wave's flag is written
-    bool holes = false;
+    // whether some key of the block lies on no page
+    int hid[2], hi = (kb >> c.shift) + tid;
+    const int h_last = (kv_end - 1) >> c.shift;
 #pragma unroll
-    for (int w = 0; w < NW; w++) holes |= flag[w] != 0;
-    holes = __builtin_amdgcn_readfirstlane(holes);
+    for (int k = 0; k < 2; k++, hi += 128 * RG) hid[k] = hi <= h_last ? c.entry(tb, hi) : 0;
     // tiles at the front that all of this wave's rows see whole (none for a wave without rows), and the last key any sees
-    int least = row ? min(qpos, kv_end - 1) : kv_end, most = qpos;
-    for (int x = 16; x > 0; x >>= 1) {
-      least = min(least, __shfl_xor(least, x, kWave));
-      most = max(most, __shfl_xor(most, x, kWave));
-    }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-    const int n_full = holes || most < 0 ? 0 : max(least + 1 - kb, 0) / kFpBKV;
+    int least = row ? min(qpos, kv_end - 1) : kv_end;
+    least = -wave_most(-least);
+    const int most = wave_most(qpos);
+    bool holes = false;
+    int n_full = most < 0 ? 0 : max(least + 1 - kb, 0) / kFpBKV;
+    auto before_barrier = [&] {  // of the prologue
+      bool hole = !c.has(hid[0]) || !c.has(hid[1]);
+      for (; hi <= h_last; hi += 128 * RG) hole |= !c.has(c.entry(tb, hi));
+      const bool some = __any(hole);
+      if (lane == 0) flag[wave] = some;
+      asm volatile("" ::: "memory");
+      wait_lgkm0();
+    };
+    auto after_barrier = [&] {
+#pragma unroll
+      for (int w = 0; w < NW; w++) holes |= flag[w] != 0;
+      holes = __builtin_amdgcn_readfirstlane(holes);
+      if (holes) n_full = 0;
+    };
     uint32_t seen = 0xff;  // which of the wave's 8 groups of a masked tile lie on pages
     auto enter_masked = [&](int t) {
       if (holes) {
@@ -415,6 +457,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   // ---- merge the two key halves of each row group: the second wave hands (m, l, O) over
   wait_vmcnt<0>();
   __syncthreads();  // every wave is done with the stages, and no DMA is in flight
+  const bool rg_empty = u.tile * BQ + rg * 32 >= u.n * G;  // a row group behind the run
   l_i += xor32(l_i);
   if (kh == 1) {
 #pragma unroll
@@ -423,7 +466,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
     ml[(RG + rg) * 64 + lane] = l_i;
   }
   __syncthreads();
-  if (kh == 1) return;
+  if (kh == 1 || rg_empty) return;
   const float m1 = ml[rg * 64 + lane], l1 = ml[(RG + rg) * 64 + lane];
   const float m = fmaxf(m_i, m1), ref = m == -__builtin_huge_valf() ? 0.f : m;  // -inf: no key seen
   const float a0 = __builtin_amdgcn_exp2f(m_i - ref), a1 = __builtin_amdgcn_exp2f(m1 - ref);
@@ -466,44 +509,69 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   }
 }
 
-// Joins a tile's splits: block = (row tile, kv head, row group, 32 dims), wave = 8 of the dims, in the lanes' order of the
-// partial results. m = max m_s, w_s = 2^(m_s - m), out = sum w_s O_s / sum w_s l_s.
-template <int D, int RG>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int cap, FlashPlan f) {
-  constexpr int BQ = 32 * RG, DT = D / 32;
-  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6, fr = lane & 31, fk = lane >> 5;
-  int i = blockIdx.x;
-  const int dt = i % DT, rg = i / DT % RG;
-  i /= DT * RG;
-  const int hk = i % a.Hkv, G = a.Hq / a.Hkv;
-  FlashUnit u;
-  if (!flash_unit<BQ, true>(a, cap, f, i / a.Hkv, lane, u) || u.splits == 1 || u.slot + u.splits > f.slots) return;
-  const int pr = u.tile * BQ + rg * 32 + fr;
-  if (pr >= u.n * G) return;
-  const int token = pr / G, h = hk * G + pr - token * G;
-  const float* ml = f.ml + ((int64_t)u.slot * a.Hkv + hk) * 2 * BQ + rg * 32 + fr;
-  const f32x4* po = reinterpret_cast<const f32x4*>(f.po) + ((((int64_t)u.slot * a.Hkv + hk) * RG + rg) * DT * 4 + dt * 4 + g) * 64 + lane;
-  const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * RG * DT * 4 * 64;
-  float m = -__builtin_huge_valf();
-#pragma unroll 8
-  for (int s = 0; s < u.splits; s++) m = fmaxf(m, ml[s * sm]);
-  const float ref = m == -__builtin_huge_valf() ? 0.f : m;
-  float l = 0.f;
+// The running join of parts (m, l, O): O and l are relative to `ref`, which is the largest m so far (0 while that is -inf).
+struct Joined {
+  float m = -__builtin_huge_valf(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = 0; s < u.splits; s++) {
-    const float w = exp2f(ml[s * sm] - ref);
-    const f32x4 v = po[s * so];
-    l = __builtin_fmaf(w, ml[s * sm + BQ], l);
+  // N parts, requested together by the caller; those behind `count` are left out
+  template <int N>
+  __device__ __forceinline__ void add(const float (&ms)[N], const float (&ls)[N], const f32x4 (&os)[N], int count) {
+    float most = m;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, v[e], o[e]);
+    for (int k = 0; k < N; k++) most = fmaxf(most, k < count ? ms[k] : m);
+    const float ref = most == -__builtin_huge_valf() ? 0.f : most, w0 = exp2f(m - ref);
+    m = most;
+    l *= w0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] *= w0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      if (k >= count) continue;
+      const float w = exp2f(ms[k] - ref);
+      l = __builtin_fmaf(w, ls[k], l);
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, os[k][e], o[e]);
+    }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+};
+
+// Joins a tile's splits: a wave per (row tile, kv head, row group, 8 dims), in the lanes' order of the partial results: m = max
+// m_s, w_s = 2^(m_s - m), out = sum w_s O_s / sum w_s l_s. 16 parts are requested at once.
+template <int D, int RG>
+__global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, FlashPlan f) {
+  constexpr int BQ = 32 * RG, ND = D / 8, NJ = 16;
+  const int lane = threadIdx.x, fr = lane & 31, fk = lane >> 5;
+  int i = blockIdx.x;
+  const int d8 = i % ND, rg = i / ND % RG;
+  i /= ND * RG;
+  const int hk = i % a.Hkv, tile = i / a.Hkv, G = a.Hq / a.Hkv;
+  const TileNote u = f.notes[tile];
+  if (tile >= *f.tiles || u.splits == 1 || u.slot + u.splits > f.slots) return;
+  if (rg * 32 + fr >= u.rows) return;
+  const int pr = u.first + rg * 32 + fr, token = pr / G, h = hk * G + pr - token * G;
+  const int64_t row = u.row0 + token;
+  const float* ml = f.ml + ((int64_t)u.slot * a.Hkv + hk) * 2 * BQ + rg * 32 + fr;
+  const f32x4* po = reinterpret_cast<const f32x4*>(f.po) + ((((int64_t)u.slot * a.Hkv + hk) * RG + rg) * ND + d8) * 64 + lane;
+  const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * RG * ND * 64;
+  Joined j;
+  for (int s0 = 0; s0 < u.splits; s0 += NJ) {
+    float ms[NJ], ls[NJ];
+    f32x4 os[NJ];
+#pragma unroll
+    for (int k = 0; k < NJ; k++) {
+      const int s = min(s0 + k, u.splits - 1);
+      ms[k] = ml[s * sm];
+      ls[k] = ml[s * sm + BQ];
+      os[k] = po[s * so];
+    }
+    j.add(ms, ls, os, u.splits - s0);
+  }
+  const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
   f16x4 v;
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = (f16)(o[e] * inv);
-  *reinterpret_cast<f16x4*>(a.out + (int64_t)(u.row0 + token) * a.ldo + h * D + dt * 32 + 8 * g + 4 * fk) = v;
-  if (a.lse && dt == 0 && g == 0 && fk == 0) a.lse[(int64_t)h * a.M + u.row0 + token] = m + log2f(l);
+  for (int e = 0; e < 4; e++) v[e] = (f16)(j.o[e] * inv);
+  *reinterpret_cast<f16x4*>(a.out + row * a.ldo + h * D + 8 * d8 + 4 * fk) = v;
+  if (a.lse && d8 == 0 && fk == 0) a.lse[(int64_t)h * a.M + row] = j.m + log2f(j.l);
 }
 
 // ---- one row per sequence
@@ -837,6 +905,17 @@ int flash_slots(int M, int G, int Hkv, int RG, int cus) {
   return plan_budget(least, Hkv, cus) ? max(2 * cus / Hkv, 1) : 0;
 }
 
+// Row tiles that the rows can make: every sequence with rows has at most one part-filled tile.
+int64_t flash_tiles(int M, int B, int G, int RG) {
+  return B == 1 ? plan_tiles(M, G, 32 * RG) : (int64_t)M * G / (32 * RG) + min(B, M);
+}
+size_t flash_bytes(int M, int B, int G, int Hkv, int RG, int D, int cus) {
+  const int slots = flash_slots(M, G, Hkv, RG, cus);
+  return slots ? 16 + min(flash_tiles(M, B, G, RG), (int64_t)2 * cus) * sizeof(TileNote) +
+                     (size_t)slots * Hkv * flash_slot_bytes(RG, D)
+               : 0;
+}
+
 // The work buffer begins with the arrival counters, in every call: one buffer may serve calls of all forms. Only pairs
 // with more than one split count, and those are fewer than two for each CU (decode_splits).
 constexpr int kCounters = 4096;
@@ -869,17 +948,19 @@ int flash_fits(K kern, int threads, size_t lds, const char* who) {
 template <int D, int RG>
 int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
   const int G = a.Hq / a.Hkv, cap = c.W << c.shift;
-  FlashPlan f{nullptr, nullptr, 0, 0, 1};
+  FlashPlan f{};
   const int slots = cap > kPlanMinSplit ? flash_slots(a.M, G, a.Hkv, RG, cus) : 0;
+  const int64_t tiles = flash_tiles(a.M, a.B, G, RG);
   if (slots) {
     f.slots = slots;
     f.cus = cus;
-    f.ml = (float*)((char*)work + kWorkHead);
+    f.most = (int)min(tiles, (int64_t)2 * cus);  // more tiles are not split
+    f.tiles = (int*)((char*)work + kWorkHead);
+    f.notes = (TileNote*)(f.tiles + 4);
+    f.ml = (float*)(f.notes + f.most);
     f.po = f.ml + (size_t)slots * a.Hkv * 2 * 32 * RG;
   }
-  // every sequence with rows has at most one part-filled tile
-  const int64_t tiles = a.B == 1 ? plan_tiles(a.M, G, 32 * RG) : (int64_t)a.M * G / (32 * RG) + min(a.B, a.M);
-  const int64_t blocks = max(tiles, (int64_t)slots) * a.Hkv, join = tiles * a.Hkv * RG * (D / 32);
+  const int64_t blocks = max(tiles, (int64_t)slots) * a.Hkv, join = (int64_t)f.most * a.Hkv * RG * (D / 8);
   // (the tiles of any start, also one that gives the same rows to every sequence, are counted in int)
   if (blocks > INT32_MAX || (slots && join > INT32_MAX) || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
     HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
@@ -889,7 +970,7 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
   if (slots) {
-    hipLaunchKernelGGL((attn_join_kernel<D, RG>), dim3((unsigned)join), dim3(256), 0, s, a, cap, f);
+    hipLaunchKernelGGL((attn_join_kernel<D, RG>), dim3((unsigned)join), dim3(64), 0, s, a, f);
     HI_TRY(hipGetLastError());
   }
   return 0;
@@ -941,7 +1022,8 @@ int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, h
   st.counters = (int*)work;
   st.ml = (float*)((char*)work + kWorkHead);
   st.po = st.ml + step_ml(st, a.B, a.Hq);
-  FlashPlan f{nullptr, nullptr, 0, 0, prefix_splits(T, a.Hkv, a.shared, cus)};
+  FlashPlan f{};
+  f.splits = prefix_splits(T, a.Hkv, a.shared, cus);
   f.slots = T * f.splits;
   f.ml = st.po + (size_t)a.B * a.Hq * st.S * D;
   f.po = f.ml + (size_t)f.slots * a.Hkv * 2 * 32 * RG;
@@ -1032,7 +1114,7 @@ HI_EXPORT size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, 
   if (M == 0 || B == 0) return kWorkHead;
   if (ragged) {
     const int RG = flash_row_groups(M, B, Hq / Hkv);
-    return kWorkHead + (size_t)flash_slots(M, Hq / Hkv, Hkv, RG, d->cus) * Hkv * flash_slot_bytes(RG, D);
+    return kWorkHead + flash_bytes(M, B, Hq / Hkv, Hkv, RG, D, d->cus);
   }
   StepPlan f;
   bool wide;

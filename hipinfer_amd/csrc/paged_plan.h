@@ -47,10 +47,11 @@ PLAN_HD int plan_budget(int T, int Hkv, int cus) {
   const int64_t n = (int64_t)T * Hkv;
   return n >= 2 * (int64_t)cus ? 0 : (n <= cus ? cus : 2 * cus) / Hkv;
 }
-// The first split length to try for `work` keys over all tiles (a tile counts its sequence's keys), and the next longer one
-// while the splits are more than the budget.
-PLAN_HD int plan_length(int64_t work, int budget) {
-  const int64_t l = (work + budget - 1) / budget;
+PLAN_HD uint32_t plan_key_tiles(int end) { return (uint32_t)(end + kPlanTile - 1) / kPlanTile; }
+// The first split length to try for `work` key tiles over all row tiles (a row tile counts its sequence's), and the next
+// longer one while the splits are more than the budget.
+PLAN_HD int plan_length(uint32_t work, int budget) {
+  const int64_t l = (int64_t)(work / (uint32_t)budget + (work % (uint32_t)budget != 0)) * kPlanTile;
   return plan_round(l < kPlanMinSplit ? kPlanMinSplit : l);
 }
 PLAN_HD int plan_longer(int L) { return plan_round((int64_t)L + L / 8 + 1); }

@@ -132,6 +132,8 @@ __global__ void __launch_bounds__(128 * RG)
   };
   auto enter_masked = [](int) {};
   auto advance = [] {};
+  auto before_barrier = [] {};
+  auto after_barrier = [] {};
   auto live = [&](int t) {
     const int k0 = t * kFpBKV + kFpKPW * kh;
     return k0 <= p0 + qw + 31 && k0 < kv_end;

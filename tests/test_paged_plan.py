@@ -18,11 +18,11 @@ SOURCE = r"""
 extern "C" int cut(const int* start, const int* pos, int B, int M, int G, int BQ, int Hkv, int cap, int cus, int slots,
                    int* out, int room) {
   int T = 0, longest = 0;
-  int64_t work = 0;
+  uint32_t work = 0;
   for (int b = 0; b < B; b++) {
     const int n = plan_rows(start[b], start[b + 1], M), t = plan_tiles(n, G, BQ), e = plan_end(pos[b], n, cap);
     T += t;
-    work += (int64_t)t * e;
+    work += (uint32_t)t * plan_key_tiles(e);
     if (t) longest = std::max(longest, e);
   }
   int L = kPlanNoSplit;
