@@ -156,7 +156,7 @@ struct TileNote;
 struct FlashPlan {
   int* tiles;      // row tiles of the batch, and their notes
   TileNote* notes;
-  float *ml, *po;  // partial results: [slot][2][BQ] m and l, [slot][RG][D / 8][64][4] O
+  float *ml, *po;  // partial results: [slot][2][BQ] m and l, O [slot][RG][D / 8][64][4], a prefix's [slot][BQ][D]
   int slots;       // slots there are, each of all kv heads
   int cus;         // > 0: split over that many
   int splits;      // of the shared prefix
@@ -478,7 +478,8 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
       f.ml[slot * 2 * BQ + rg * 32 + fr] = m;
       f.ml[slot * 2 * BQ + BQ + rg * 32 + fr] = l;
     }
-    f32x4* po = reinterpret_cast<f32x4*>(f.po) + ((slot * RG + rg) * DT * 4) * 64 + lane;
+    // a join takes them in the lanes' order; a prefix's rows are read whole
+    f32x4* po = reinterpret_cast<f32x4*>(f.po) + (PREFIX ? (slot * BQ + rg * 32 + fr) * (D / 4) + fk : (slot * RG + rg) * DT * 4 * 64 + lane);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) {
       const f32x16 o1 = mo[(rg * DT + dt) * 64 + lane];
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = o[dt][4 * g + e] * a0 + o1[4 * g + e] * a1;
-        po[(dt * 4 + g) * 64] = v;
+        po[(dt * 4 + g) * (PREFIX ? 2 : 64)] = v;
       }
     }
     return;
@@ -509,37 +510,35 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   }
 }
 
-// The running join of parts (m, l, O): O and l are relative to `ref`, which is the largest m so far (0 while that is -inf).
-struct Joined {
-  float m = -__builtin_huge_valf(), l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  // N parts, requested together by the caller; those behind `count` are left out
-  template <int N>
-  __device__ __forceinline__ void add(const float (&ms)[N], const float (&ls)[N], const f32x4 (&os)[N], int count) {
-    float most = m;
+// Joins N parts (m, l, O) to the running (M, L, O), which is relative to M (-inf: no key yet); parts from `count` on are
+// left out.
+template <int N>
+__device__ __forceinline__ void join_parts(float& M, float& L, f32x4& O, const float (&ms)[N], const float (&ls)[N],
+                                           const f32x4 (&os)[N], int count) {
+  float most = M;
 #pragma unroll
-    for (int k = 0; k < N; k++) most = fmaxf(most, k < count ? ms[k] : m);
-    const float ref = most == -__builtin_huge_valf() ? 0.f : most, w0 = exp2f(m - ref);
-    m = most;
-    l *= w0;
+  for (int k = 0; k < N; k++)
+    if (k < count) most = fmaxf(most, ms[k]);
+  const float ref = most == -__builtin_huge_valf() ? 0.f : most, w0 = exp2f(M - ref);
+  M = most;
+  L *= w0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[e] *= w0;
+  for (int e = 0; e < 4; e++) O[e] *= w0;
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-      if (k >= count) continue;
-      const float w = exp2f(ms[k] - ref);
-      l = __builtin_fmaf(w, ls[k], l);
+  for (int k = 0; k < N; k++) {
+    if (k >= count) continue;
+    const float w = exp2f(ms[k] - ref);
+    L = __builtin_fmaf(w, ls[k], L);
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, os[k][e], o[e]);
-    }
+    for (int e = 0; e < 4; e++) O[e] = __builtin_fmaf(w, os[k][e], O[e]);
   }
-};
+}
 
 // Joins a tile's splits: a wave per (row tile, kv head, row group, 8 dims), in the lanes' order of the partial results: m = max
-// m_s, w_s = 2^(m_s - m), out = sum w_s O_s / sum w_s l_s. 16 parts are requested at once.
+// m_s, w_s = 2^(m_s - m), out = sum w_s O_s / sum w_s l_s. 4 parts are requested at once.
 template <int D, int RG>
 __global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, FlashPlan f) {
-  constexpr int BQ = 32 * RG, ND = D / 8, NJ = 16;
+  constexpr int BQ = 32 * RG, ND = D / 8, NJ = 4;
   const int lane = threadIdx.x, fr = lane & 31, fk = lane >> 5;
   int i = blockIdx.x;
   const int d8 = i % ND, rg = i / ND % RG;
@@ -553,7 +552,8 @@ __global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, FlashPlan f) 
   const float* ml = f.ml + ((int64_t)u.slot * a.Hkv + hk) * 2 * BQ + rg * 32 + fr;
   const f32x4* po = reinterpret_cast<const f32x4*>(f.po) + ((((int64_t)u.slot * a.Hkv + hk) * RG + rg) * ND + d8) * 64 + lane;
   const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * RG * ND * 64;
-  Joined j;
+  float m = -__builtin_huge_valf(), l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < u.splits; s0 += NJ) {
     float ms[NJ], ls[NJ];
     f32x4 os[NJ];
@@ -564,14 +564,14 @@ __global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, FlashPlan f) 
       ls[k] = ml[s * sm + BQ];
       os[k] = po[s * so];
     }
-    j.add(ms, ls, os, u.splits - s0);
+    join_parts(m, l, o, ms, ls, os, u.splits - s0);
   }
-  const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   f16x4 v;
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = (f16)(j.o[e] * inv);
+  for (int e = 0; e < 4; e++) v[e] = (f16)(o[e] * inv);
   *reinterpret_cast<f16x4*>(a.out + row * a.ldo + h * D + 8 * d8 + 4 * fk) = v;
-  if (a.lse && d8 == 0 && fk == 0) a.lse[(int64_t)h * a.M + row] = j.m + log2f(j.l);
+  if (a.lse && d8 == 0 && fk == 0) a.lse[(int64_t)h * a.M + row] = m + log2f(l);
 }
 
 // ---- one row per sequence
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, FlashPlan f) 
 // one 64-bit address each for K and V per tile, from entries requested a tile ahead. What the slot kernel leaves to the
 // buffer bounds is done in registers, in a wave's last tile and in tiles with an entry that is no page only: logits of
 // keys that are not there become -inf, their V rows zeros.
-// OWN: the part of a sequence behind a shared prefix; blocks leave their splits' results to attn_shared_join_kernel.
+// OWN: the keys behind a shared prefix, whose own splits' results (FlashPlan) are joined in when a pair's are.
 struct StepPlan {
   int S, S1;      // splits of a pair: the launch's, and those that give every CU its blocks (splits_used)
   int* counters;  // [B * Hkv], arrivals of a pair's splits
@@ -594,22 +594,30 @@ __device__ __forceinline__ int step_keys(const AttnArgs& a, int cap, int b, int 
   return plan_end(a.pos[b], 1, cap) > base ? plan_end(a.pos[b], 1, cap) - base : 0;
 }
 
-template <int GC, int D, int NWV>
+template <int NT>
+struct OwnSmem {
+  float m[NT], l[NT];
+  f32x4 o[NT];
+};
+
+template <int GC, int D, int NWV, bool OWN>
 struct StepSmem {
   float wo[NWV][GC][D];
   float wm[NWV][GC], wl[NWV][GC];
   float sm[GC][kDecodeMaxSplits], sw[GC][kDecodeMaxSplits];
+  float tm[GC], tl[GC];
   int is_last;
+  OwnSmem<OWN ? NWV * 64 : 1> own;
 };
 
 template <int GC, int D, int NWV, bool OWN>
-__global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, PagedCache c, StepPlan f) {
+__global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, PagedCache c, StepPlan f, FlashPlan pf, int BQ) {
   constexpr int KS = D / 32;               // k steps of a logits product
   constexpr int DL = D / 16;               // V dims (and P.V products) per lane
   constexpr int BK = NWV * kDaTile;        // keys per block pass
   constexpr int NT = NWV * 64;
   typedef typename std::conditional<DL == 8, u32x4, u32x2>::type VT;
-  __shared__ StepSmem<GC, D, NWV> sh;
+  __shared__ StepSmem<GC, D, NWV, OWN> sh;
   // split-major blocks: a pair's used splits come first in dispatch order
   const int nhb = a.B * a.Hkv, G = a.Hq / a.Hkv, page = 1 << c.shift;
   const int split = blockIdx.x / nhb, hk = blockIdx.x % a.Hkv, b = (blockIdx.x % nhb) / a.Hkv;
@@ -628,7 +636,7 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
   const int kg = 8 * (r >> 2), vg = 8 * fk;  // the lane's key groups in a tile
   const f16* const kl = c.kp + ((int64_t)hk * page + (r & 3)) * D + 8 * fk;
   const f16* const vl = c.vp + (int64_t)hk * page * D + DL * r;
-  auto entry = [&](int key) { return key < end ? c.entry(b, key >> c.shift) : -1; };
+  auto entry = [&](int key) { return key < end ? c.entry(!OWN && key < a.shared ? 0 : b, key >> c.shift) : -1; };
   // element offset of the group that starts at `key`; that of page 0 for keys that are not there
   auto place = [&](int id, int key) { return c.has(id) ? id * c.stride + (int64_t)(key & (page - 1)) * D : (int64_t)0; };
   u32x4 kf[2][KS];
@@ -699,12 +707,12 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
       const float mn = m == -__builtin_huge_valf() ? 0.f : m;
       const float alpha = exp2f(m_old - mn);  // 0 on the first tile (m = -inf)
       float ps = 0.f;
-      f16x8 pf;
+      f16x8 ph;
 #pragma unroll
       for (int k = 0; k < 8; k++) {
         p[k] = exp2f(p[k] - mn);
         ps += p[k];
-        pf[k] = (f16)p[k];
+        ph[k] = (f16)p[k];
       }
       l = __builtin_fmaf(l, alpha, ps);
 #pragma unroll
@@ -723,7 +731,7 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
 #pragma unroll
         for (int k = 0; k < 4; k++)
           w[k] = __builtin_amdgcn_perm(vf[2 * k + 1][n >> 1], vf[2 * k][n >> 1], n & 1 ? 0x07060302u : 0x05040100u);
-        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), pf, o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), ph, o[n], 0, 0, 0);
       }
       if constexpr (!LAST) {
         __builtin_amdgcn_sched_barrier(0);
@@ -758,139 +766,189 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
   __syncthreads();
   const bool single = S_eff == 1;
   const int64_t pair = (int64_t)b * a.Hq + hk * G;  // of head 0 of the group; its partials start at pair * S
-  for (int i = tid; i < G * D; i += NT) {
-    const int g = i / D, d = i % D;
-    float M = -__builtin_huge_valf();
+  // element d of head g over the block's waves
+  auto block_sum = [&](int g, int d, float& M, float& L, float& O) {
+    M = -__builtin_huge_valf();
 #pragma unroll
     for (int w = 0; w < NWV; w++) M = fmaxf(M, sh.wm[w][g]);
-    float L = 0.f, O = 0.f;
+    L = O = 0.f;
 #pragma unroll
     for (int w = 0; w < NWV; w++) {
       const float e = sh.wm[w][g] == -__builtin_huge_valf() ? 0.f : exp2f(sh.wm[w][g] - M);
       L = __builtin_fmaf(sh.wl[w][g], e, L);
       O = __builtin_fmaf(sh.wo[w][g][d], e, O);
     }
-    const int64_t at = (pair + g) * f.S + split;
-    if (OWN) {
-      f.po[at * D + d] = O;
-      if (d == 0) {
-        f.ml[2 * at] = M;
-        f.ml[2 * at + 1] = L;
-      }
-    } else if (single) {
-      a.out[(int64_t)b * a.ldo + (hk * G + g) * D + d] = (f16)(L == 0.f ? 0.f : O / L);
-      if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
-    } else {
-      st_coherent(f.po + at * D + d, O);
-      if (d == 0) {
-        st_coherent(f.ml + 2 * at, M);
-        st_coherent(f.ml + 2 * at + 1, L);
+  };
+  auto store = [&](int g, int d, float M, float L, float O) {
+    a.out[(int64_t)b * a.ldo + (hk * G + g) * D + d] = (f16)(L == 0.f ? 0.f : O / L);
+    if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
+  };
+  if (!single || !OWN) {
+    for (int i = tid; i < G * D; i += NT) {
+      const int g = i / D, d = i % D;
+      float M, L, O;
+      block_sum(g, d, M, L, O);
+      if (single) {
+        store(g, d, M, L, O);
+      } else {
+        const int64_t at = (pair + g) * f.S + split;
+        st_coherent(f.po + at * D + d, O);
+        if (d == 0) {
+          st_coherent(f.ml + 2 * at, M);
+          st_coherent(f.ml + 2 * at + 1, L);
+        }
       }
     }
+    if (single) return;
   }
-  if (OWN || single) return;
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partial stores are complete
-  __syncthreads();
-  if (tid == 0) {
-    int* ctr = f.counters + b * a.Hkv + hk;
-    const int done = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sh.is_last = done == S_eff - 1;
-    if (sh.is_last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next launch
-  }
-  __syncthreads();
-  if (!sh.is_last) return;
-  // ---- the last block merges the S_eff splits of every head of its group, in split order. The (m, l) pairs and the first
-  //      16 splits' partial outputs are requested in one round.
   constexpr int EPT = (GC * D + NT - 1) / NT;  // output elements per thread
+  constexpr bool AHEAD = !OWN && GC <= 8;      // (16 heads would not fit the registers)
   float v0[EPT][16];
+  if (!single) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partial stores are complete
+    __syncthreads();
+    if (tid == 0) {
+      int* ctr = f.counters + b * a.Hkv + hk;
+      const int done = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      sh.is_last = done == S_eff - 1;
+      if (sh.is_last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next launch
+    }
+    __syncthreads();
+    if (!sh.is_last) return;
+    // ---- the last block merges the S_eff splits of every head of its group, in split order. The (m, l) pairs and the
+    //      first 16 splits' partial outputs are requested in one round.
+    if constexpr (AHEAD) {
 #pragma unroll
-  for (int e = 0; e < EPT; e++) {
-    const int i = tid + e * NT;
-    const int g = min(i / D, G - 1), d = i % D;
+      for (int e = 0; e < EPT; e++) {
+        const int i = tid + e * NT;
+        const int g = min(i / D, G - 1), d = i % D;
+        const float* pp = f.po + (pair + g) * f.S * D + d;
+#pragma unroll
+        for (int k = 0; k < 16; k++) v0[e][k] = ld_coherent(pp + (int64_t)min(k, S_eff - 1) * D);
+      }
+    }
+    for (int i = tid; i < G * S_eff; i += NT) {
+      const int g = i / S_eff, s = i - g * S_eff;
+      const float* pp = f.ml + ((pair + g) * f.S + s) * 2;
+      sh.sm[g][s] = ld_coherent(pp);
+      sh.sw[g][s] = ld_coherent(pp + 1);
+    }
+    __syncthreads();
+    for (int g = wave; g < G; g += NWV) {  // S_eff is at most a wave's lanes
+      const float ms = lane < S_eff ? sh.sm[g][lane] : -__builtin_huge_valf(), ls = lane < S_eff ? sh.sw[g][lane] : 0.f;
+      const float M = wave_max(ms);
+      const float e = ms == -__builtin_huge_valf() ? 0.f : exp2f(ms - M);
+      const float L = wave_sum(ls * e);
+      if (lane < S_eff) sh.sw[g][lane] = e;
+      if (lane == 0) {
+        sh.tm[g] = M;
+        sh.tl[g] = L;
+      }
+    }
+    __syncthreads();
+  }
+  // splits s0 .. s0 + 15 of element (g, d)
+  auto sum16 = [&](int g, const float (&v)[16], int s0, float& O) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) O = __builtin_fmaf(v[k], s0 + k < S_eff ? sh.sw[g][s0 + k] : 0.f, O);
+  };
+  auto load16 = [&](int g, int d, int s0, float (&v)[16]) {
     const float* pp = f.po + (pair + g) * f.S * D + d;
 #pragma unroll
-    for (int k = 0; k < 16; k++) v0[e][k] = ld_coherent(pp + (int64_t)min(k, S_eff - 1) * D);
-  }
-  for (int i = tid; i < G * S_eff; i += NT) {
-    const int g = i / S_eff, s = i - g * S_eff;
-    const float* pp = f.ml + ((pair + g) * f.S + s) * 2;
-    sh.sm[g][s] = ld_coherent(pp);
-    sh.sw[g][s] = ld_coherent(pp + 1);
-  }
-  __syncthreads();
-  for (int g = wave; g < G; g += NWV) {  // S_eff is at most a wave's lanes
-    const float ms = lane < S_eff ? sh.sm[g][lane] : -__builtin_huge_valf(), ls = lane < S_eff ? sh.sw[g][lane] : 0.f;
-    const float M = wave_max(ms);
-    const float e = ms == -__builtin_huge_valf() ? 0.f : exp2f(ms - M);
-    const float L = wave_sum(ls * e);
-    if (lane < S_eff) sh.sw[g][lane] = L == 0.f ? 0.f : e / L;
-    if (a.lse && lane == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
-  }
-  __syncthreads();
+    for (int k = 0; k < 16; k++) v[k] = ld_coherent(pp + (int64_t)min(s0 + k, S_eff - 1) * D);
+  };
+  if constexpr (!OWN) {
 #pragma unroll
-  for (int e = 0; e < EPT; e++) {
-    const int i = tid + e * NT;
-    if (i < G * D) {
-      const int g = i / D, d = i % D;
-      const float* pp = f.po + (pair + g) * f.S * D + d;
-      float O = 0.f;
-#pragma unroll
-      for (int k = 0; k < 16; k++) O = __builtin_fmaf(v0[e][k], k < S_eff ? sh.sw[g][k] : 0.f, O);
-      for (int s0 = 16; s0 < S_eff; s0 += 16) {
-        float v[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) v[k] = ld_coherent(pp + (int64_t)min(s0 + k, S_eff - 1) * D);
-#pragma unroll
-        for (int k = 0; k < 16; k++) O = __builtin_fmaf(v[k], s0 + k < S_eff ? sh.sw[g][s0 + k] : 0.f, O);
+    for (int e = 0; e < EPT; e++) {
+      const int i = tid + e * NT;
+      if (i < G * D) {
+        const int g = i / D, d = i % D;
+        float O = 0.f;
+        if constexpr (AHEAD) sum16(g, v0[e], 0, O);
+        for (int s0 = AHEAD ? 16 : 0; s0 < S_eff; s0 += 16) {
+          float v[16];
+          load16(g, d, s0, v);
+          sum16(g, v, s0, O);
+        }
+        store(g, d, sh.tm[g], sh.tl[g], O);
       }
-      a.out[(int64_t)b * a.ldo + (hk * G + g) * D + d] = (f16)O;
+    }
+  } else {
+    // With the prefix's parts: a thread takes 4 dims of a head, and where there are more threads than those, every P-th part,
+    // 8 requested at once; the P threads' results are joined through LDS.
+    constexpr int D4 = D / 4;
+    const int items = G * D4, P = items < NT ? NT / items : 1;
+    const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * BQ * D;
+#pragma unroll 1
+    for (int i0 = 0; i0 < items; i0 += NT) {
+      const int part = items < NT ? tid / items : 0, item = items < NT ? tid - part * items : i0 + tid;
+      const bool active = part < P && item < items;
+      const int g = item / D4, d = 4 * (item % D4);
+      float M = -__builtin_huge_valf(), L = 0.f;
+      f32x4 O = {0.f, 0.f, 0.f, 0.f};
+      if (active) {
+        const int pr = b * G + g, tile = pr / BQ, at = pr - tile * BQ;
+        const int64_t slot = (int64_t)tile * pf.splits * a.Hkv + hk;
+        const float* ml = pf.ml + slot * 2 * BQ + at;
+        const float* po = pf.po + (slot * BQ + at) * D + d;
+        if (part == 0) {  // the sequence's own keys
+          if (single) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              float v;
+              block_sum(g, d + e, M, L, v);
+              O[e] = v;
+            }
+          } else {
+            M = sh.tm[g];
+            L = sh.tl[g];
+#pragma unroll 1
+            for (int s = 0; s < S_eff; s++) {
+              const float w = sh.sw[g][s];
+              const float* pp = f.po + ((pair + g) * f.S + s) * D + d;
+#pragma unroll
+              for (int e = 0; e < 4; e++) O[e] = __builtin_fmaf(ld_coherent(pp + e), w, O[e]);
+            }
+          }
+        }
+#pragma unroll 1
+        for (int s0 = part; s0 < pf.splits; s0 += 8 * P) {
+          float ms[8], ls[8];
+          f32x4 os[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            const int s = min(s0 + k * P, pf.splits - 1);
+            ms[k] = ml[s * sm];
+            ls[k] = ml[s * sm + BQ];
+            os[k] = *reinterpret_cast<const f32x4*>(po + s * so);
+          }
+          join_parts(M, L, O, ms, ls, os, (pf.splits - s0 + P - 1) / P);
+        }
+      }
+      if (P > 1) {
+        __syncthreads();
+        if (active && part > 0) {
+          sh.own.m[tid] = M;
+          sh.own.l[tid] = L;
+          sh.own.o[tid] = O;
+        }
+        __syncthreads();
+        if (active && part == 0)
+          for (int p = 1; p < P; p++) {
+            const float ms[1] = {sh.own.m[p * items + item]}, ls[1] = {sh.own.l[p * items + item]};
+            const f32x4 os[1] = {sh.own.o[p * items + item]};
+            join_parts(M, L, O, ms, ls, os, 1);
+          }
+      }
+      if (active && part == 0) {
+        f16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (f16)(L == 0.f ? 0.f : O[e] / L);
+        *reinterpret_cast<f16x4*>(a.out + (int64_t)b * a.ldo + (hk * G + g) * D + d) = v;
+        if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
+      }
     }
   }
-}
-
-// Joins a shared prefix's splits and each sequence's own: block = (row tile of the prefix, kv head, row group, 32 dims), wave =
-// 8 of the dims, in the lanes' order of the prefix's partial results.
-template <int D, int RG>
-__global__ void __launch_bounds__(256) attn_shared_join_kernel(AttnArgs a, int cap, FlashPlan f, StepPlan st) {
-  constexpr int BQ = 32 * RG, DT = D / 32;
-  const int lane = threadIdx.x & 63, g8 = threadIdx.x >> 6, fr = lane & 31, fk = lane >> 5;
-  int i = blockIdx.x;
-  const int dt = i % DT, rg = i / DT % RG;
-  i /= DT * RG;
-  const int hk = i % a.Hkv, tile = i / a.Hkv, G = a.Hq / a.Hkv;
-  const int pr = tile * BQ + rg * 32 + fr;
-  if (pr >= a.M * G) return;
-  const int b = pr / G, h = hk * G + pr - b * G;
-  const int own = splits_used(step_keys(a, cap, b, a.shared), st.S, st.S1);
-  const int64_t slot = (int64_t)tile * f.splits * a.Hkv + hk;
-  const float* ml = f.ml + slot * 2 * BQ + rg * 32 + fr;
-  const f32x4* po = reinterpret_cast<const f32x4*>(f.po) + ((slot * RG + rg) * DT * 4 + dt * 4 + g8) * 64 + lane;
-  const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * RG * DT * 4 * 64;
-  const int d0 = dt * 32 + 8 * g8 + 4 * fk;
-  const float* oml = st.ml + ((int64_t)b * a.Hq + h) * st.S * 2;
-  const float* opo = st.po + ((int64_t)b * a.Hq + h) * st.S * D + d0;
-  float m = -__builtin_huge_valf();
-#pragma unroll 8
-  for (int s = 0; s < f.splits; s++) m = fmaxf(m, ml[s * sm]);
-  for (int s = 0; s < own; s++) m = fmaxf(m, oml[2 * s]);
-  const float ref = m == -__builtin_huge_valf() ? 0.f : m;
-  float l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](float w, float ls, f32x4 v) {
-    l = __builtin_fmaf(w, ls, l);
-#pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, v[e], o[e]);
-  };
-#pragma unroll 8
-  for (int s = 0; s < f.splits; s++) add(exp2f(ml[s * sm] - ref), ml[s * sm + BQ], po[s * so]);
-  for (int s = 0; s < own; s++)
-    add(exp2f(oml[2 * s] - ref), oml[2 * s + 1], *reinterpret_cast<const f32x4*>(opo + (int64_t)s * D));
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  f16x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = (f16)(o[e] * inv);
-  *reinterpret_cast<f16x4*>(a.out + (int64_t)b * a.ldo + h * D + d0) = v;
-  if (a.lse && dt == 0 && g8 == 0 && fk == 0) a.lse[(int64_t)h * a.M + b] = m + log2f(l);
 }
 
 // Row groups per block: 4 (128 packed rows), or 2 where a sequence has 64 packed rows or less on average.
@@ -933,7 +991,17 @@ size_t step_bytes(const StepPlan& f, int B, int Hq, int D) { return (step_ml(f, 
 
 // Splits of a prefix of `shared` positions for T row tiles: a block for each CU.
 int prefix_splits(int T, int Hkv, int shared, int cus) {
-  return max(1, min(cus / max(1, T * Hkv), (shared + 255) / 256));
+  return max(1, min(cus / max(1, T * Hkv), max((shared + 255) / 256, min(8, (shared + 127) / 128))));
+}
+
+// Whether a decode step that reads the prefix again for every sequence is faster. Its re-reads mostly hit the caches, at 12
+// TB/s; sharing costs 10 us (a launch more, the parts' way through memory) and the prefix once, at 6 TB/s or 500 TFLOP/s.
+// Measured with 2 to 64 sequences after prefixes of 512 to 32768, 20 or 300 keys of their own, in 32/8 and 12/2 heads of
+// 128 and 32/4 of 64: 1 % above the faster of the two on average (us, sharing / re-reading: 8 after 2048, 32/8 of 128, 17.1 /
+// 14.2; after 8192 24.4 / 28.4; 32 after 8192 30.5 / 81.1; 4 after 16384 25.4 / 27.5).
+bool prefix_reread(const AttnArgs& a, int D) {
+  const double mb = 4e-6 * a.shared * a.Hkv * D, mflop = 4e-6 * D * a.Hq * a.shared * a.B;
+  return a.B * mb / 12 < 10 + fmax(mb / 6, mflop / 500);
 }
 
 // Largest grid's blocks and what a kernel's LDS limit needs; 0, or a negative code.
@@ -977,18 +1045,19 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
 }
 
 template <int D, bool OWN>
-int step_launch(const AttnArgs& a, const PagedCache& c, const StepPlan& f, bool wide, hipStream_t s, const char* who) {
+int step_launch(const AttnArgs& a, const PagedCache& c, const StepPlan& f, const FlashPlan& pf, int BQ, bool wide,
+                hipStream_t s, const char* who) {
   const int64_t blocks = (int64_t)f.S * a.B * a.Hkv;
   if (blocks > INT32_MAX) HI_FAIL("%s: %d sequences of %d kv heads are too many", who, a.B, a.Hkv);
   const dim3 grid((unsigned)blocks);
   const int G = a.Hq / a.Hkv;
-  if (G > 8) hipLaunchKernelGGL((attn_step_kernel<16, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f);
+  if (G > 8) hipLaunchKernelGGL((attn_step_kernel<16, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
   else if (G > 4) {
-    if (wide) hipLaunchKernelGGL((attn_step_kernel<8, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f);
-    else hipLaunchKernelGGL((attn_step_kernel<8, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f);
+    if (wide) hipLaunchKernelGGL((attn_step_kernel<8, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f, pf, BQ);
+    else hipLaunchKernelGGL((attn_step_kernel<8, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
   } else {
-    if (wide) hipLaunchKernelGGL((attn_step_kernel<4, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f);
-    else hipLaunchKernelGGL((attn_step_kernel<4, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f);
+    if (wide) hipLaunchKernelGGL((attn_step_kernel<4, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f, pf, BQ);
+    else hipLaunchKernelGGL((attn_step_kernel<4, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
   }
   HI_TRY(hipGetLastError());
   return 0;
@@ -1002,7 +1071,7 @@ int step_run(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStr
   f.counters = (int*)work;
   f.ml = (float*)((char*)work + kWorkHead);
   f.po = f.ml + step_ml(f, a.B, a.Hq);
-  return step_launch<D, false>(a, c, f, wide, s, who);
+  return step_launch<D, false>(a, c, f, FlashPlan{}, 0, wide, s, who);
 }
 
 size_t shared_bytes(int B, int Hq, int Hkv, int D, int cus) {
@@ -1015,7 +1084,7 @@ size_t shared_bytes(int B, int Hq, int Hkv, int D, int cus) {
 
 template <int D, int RG>
 int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
-  const int G = a.Hq / a.Hkv, cap = c.W << c.shift, T = plan_tiles(a.M, G, 32 * RG);
+  const int G = a.Hq / a.Hkv, T = plan_tiles(a.M, G, 32 * RG);
   StepPlan st;
   bool wide;
   step_splits(a.B, a.Hkv, G, cus, st, wide);
@@ -1027,17 +1096,14 @@ int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, h
   f.slots = T * f.splits;
   f.ml = st.po + (size_t)a.B * a.Hq * st.S * D;
   f.po = f.ml + (size_t)f.slots * a.Hkv * 2 * 32 * RG;
-  const int64_t blocks = (int64_t)f.slots * a.Hkv, join = (int64_t)T * a.Hkv * RG * (D / 32);
-  if (blocks > INT32_MAX || join > INT32_MAX) HI_FAIL("%s: %d sequences are too many", who, a.B);
+  const int64_t blocks = (int64_t)f.slots * a.Hkv;
+  if (blocks > INT32_MAX) HI_FAIL("%s: %d sequences are too many", who, a.B);
   const auto kern = attn_pages_kernel<D, RG, true>;
   const size_t lds = FpSmem<D, RG>::kBytes;
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
-  if (const int rc = step_launch<D, true>(a, c, st, wide, s, who)) return rc;
-  hipLaunchKernelGGL((attn_shared_join_kernel<D, RG>), dim3((unsigned)join), dim3(256), 0, s, a, cap, f, st);
-  HI_TRY(hipGetLastError());
-  return 0;
+  return step_launch<D, true>(a, c, st, f, 32 * RG, wide, s, who);
 }
 
 int attn_check(const char* who, const void* q, int ldq, const int* pos, const void* out, int ldo, const float* lse, int M,
@@ -1059,7 +1125,7 @@ int attn_run(const AttnArgs& a, const PagedCache& c, int D, int cus, void* work,
     return D == 64 ? (small ? flash_launch<64, 2>(a, c, cus, work, s, who) : flash_launch<64, 4>(a, c, cus, work, s, who))
                    : (small ? flash_launch<128, 2>(a, c, cus, work, s, who) : flash_launch<128, 4>(a, c, cus, work, s, who));
   }
-  if (a.shared) {
+  if (a.shared && !prefix_reread(a, D)) {
     const bool small = flash_row_groups(a.M, 1, G) == 2;
     return D == 64 ? (small ? shared_launch<64, 2>(a, c, cus, work, s, who) : shared_launch<64, 4>(a, c, cus, work, s, who))
                    : (small ? shared_launch<128, 2>(a, c, cus, work, s, who) : shared_launch<128, 4>(a, c, cus, work, s, who));

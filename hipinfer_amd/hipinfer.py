@@ -418,49 +418,51 @@ def flash_prefill_lse(q, kc, vc, T, p0, Hq, Hkv, out=None, lse=None):
 
 
 # ------------------------------------------------------------------ paged key/value cache
-# These wrappers are half of a small call's time, so their checks read each property once and compare tuples; what fails is
-# looked at again for the message.
-def _on_device(what, *tensors):
-    """Every tensor (None aside) on the current device: the library launches there."""
+# These wrappers are half of a small call's time, so their checks read each property once (60 to 90 ns each) and the common
+# case is one comparison; what fails is looked at again for the message.
+_F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
+
+
+def _gpu(what, *tensors):
+    """The current device, on which every tensor (None aside) has to be: the library launches there."""
     gpu = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != gpu:
             raise ValueError(f"hipinfer_amd.{what}: tensors on {tensors[0].device} and {t.device}")
     if gpu < 0 or gpu != torch._C._cuda_getDevice():
         raise ValueError(f"hipinfer_amd.{what}: tensors must live on the current GPU (got {tensors[0].device})")
+    return gpu
 
 
 def _paged(what, kp, vp, table, Hkv):
     """Checks a paged cache kp / vp [pages, Hkv, page, D] and its table [B, W]; returns the cache's arguments of a library
     call, B and D."""
-    _need(what, kp, torch.float16, 4)
     shape, steps, tshape = kp.shape, kp.stride(), table.shape
-    pages, heads, page, D = shape
-    if vp.dtype is not torch.float16 or vp.shape != shape:
-        raise ValueError(f"hipinfer_amd.{what}: kp {tuple(shape)} and vp {tuple(vp.shape)} must have the same shape, in fp16")
-    if table.dtype is not torch.int32 or len(tshape) != 2:
+    if len(shape) != 4 or kp.dtype is not _F16 or vp.dtype is not _F16 or vp.shape != shape or shape[1] != Hkv:
+        raise ValueError(f"hipinfer_amd.{what}: kp and vp must be fp16 [pages, Hkv {Hkv}, page, D], got {kp.dtype} "
+                         f"{tuple(shape)} and {vp.dtype} {tuple(vp.shape)}")
+    if len(tshape) != 2 or table.dtype is not _I32:
         raise ValueError(f"hipinfer_amd.{what}: the table must be int32 [B, W], got {table.dtype} {tuple(tshape)}")
-    if heads != Hkv:
-        raise ValueError(f"hipinfer_amd.{what}: a cache of {heads} heads for Hkv {Hkv}")
-    packed, vsteps = (page * D, D, 1), vp.stride()
-    if steps != vsteps or steps[1:] != packed:  # strides of dimensions of size 1 say nothing
+    pages, _, page, D = shape
+    step, vsteps = steps[0], vp.stride()
+    if vsteps != steps or steps != (step, page * D, D, 1):  # strides of dimensions of size 1 say nothing
         for st in (steps, vsteps):
-            if any(n > 1 and have != want for n, have, want in zip(shape[1:], st[1:], packed)):
+            if any(n > 1 and have != want for n, have, want in zip(shape[1:], st[1:], (page * D, D, 1))):
                 raise ValueError(f"hipinfer_amd.{what}: a page [Hkv, page, D] must be packed")
-        if pages > 1 and vsteps[0] != steps[0]:
+        if pages > 1 and vsteps[0] != step:
             raise ValueError(f"hipinfer_amd.{what}: kp and vp must have the same page stride")
     B, W = tshape
     ldt, one = table.stride()
     if one != 1 and W > 1:
         raise ValueError(f"hipinfer_amd.{what}: table rows must be contiguous")
-    return (kp.data_ptr(), vp.data_ptr(), steps[0] if pages > 1 else Hkv * page * D, pages, page, table.data_ptr(),
+    return (kp.data_ptr(), vp.data_ptr(), step if pages > 1 else Hkv * page * D, pages, page, table.data_ptr(),
             ldt if B > 1 else W, W), B, D
 
 
 def _rows_of(what, name, t, M, width):
     """An fp16 [M, >= width] tensor of contiguous rows; returns its row stride (a single row's is its width)."""
     shape = t.shape
-    if t.dtype is not torch.float16 or len(shape) != 2 or shape[0] != M or shape[1] < width:
+    if t.dtype is not _F16 or len(shape) != 2 or shape[0] != M or shape[1] < width:
         raise ValueError(f"hipinfer_amd.{what}: {name} must be fp16 [{M}, {width}], got {t.dtype} {tuple(shape)}")
     step, one = t.stride()
     if one != 1 and shape[1] > 1:
@@ -470,7 +472,7 @@ def _rows_of(what, name, t, M, width):
 
 def _vector(what, name, t, n):
     """A packed int32 vector of n entries."""
-    if t.dtype is not torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+    if t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"hipinfer_amd.{what}: {name} must be a packed int32 vector of {n}, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -488,12 +490,12 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
     A row that has no place is left out, its q too: a negative position (padding), one behind its table row or cs,
     a seq outside the table, a page id outside [0, pages). Rows of one call must have places of their own."""
     what = "rope_cache_paged"
-    _on_device(what, qkv, cs, kp, vp, table, pos, seq, q_out)
+    gpu = _gpu(what, qkv, cs, kp, vp, table, pos, seq, q_out)
     cache, B, D = _paged(what, kp, vp, table, Hkv)
     M = qkv.shape[0]
     ldq = _rows_of(what, "qkv", qkv, M, (Hq + 2 * Hkv) * D)
-    cshape, wide = cs.shape, cs.dtype is torch.float32
-    if not (wide or cs.dtype is torch.float16) or len(cshape) != 3 or cshape[2] != 2 or not cs.is_contiguous():
+    cshape, wide = cs.shape, cs.dtype is _F32
+    if not (wide or cs.dtype is _F16) or len(cshape) != 3 or cshape[2] != 2 or not cs.is_contiguous():
         raise ValueError(f"hipinfer_amd.{what}: cs must be packed [positions, rot/2, 2], fp16 or fp32")
     _vector(what, "pos", pos, M)
     if seq is not None:
@@ -505,8 +507,8 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
     else:
         ldo = _rows_of(what, "q_out", q_out, M, Hq * D)
     check_rc(lib.hi_rope_cache_paged(qkv.data_ptr(), ldq, q_out.data_ptr(), ldo, M, Hq, Hkv, D, cs.data_ptr(), cshape[0],
-                                     wide, 2 * cshape[1], interleaved, _addr(seq), pos.data_ptr(), *cache, B, _stream()),
-             what)
+                                     wide, 2 * cshape[1], interleaved, _addr(seq), pos.data_ptr(), *cache, B,
+                                     torch._C._cuda_getCurrentRawStream(gpu)), what)
 
 
 def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work):
@@ -519,7 +521,7 @@ def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work):
     if out is None:
         out = _alloc_rows(q, M, Hq * D)
     ldo = _rows_of(what, "out", out, M, Hq * D)
-    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (Hq, M) or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype is not _F32 or lse.shape != (Hq, M) or not lse.is_contiguous()):
         raise ValueError(f"hipinfer_amd.{what}: lse must be packed fp32 [{Hq}, {M}]")
     if work is not None and (work.dtype is not torch.uint8 or not work.is_contiguous()):
         raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8")
@@ -554,7 +556,7 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     base-2 log-sum-exp of each row's scaled logits (-inf without keys). `work` (attn_paged_work) can be kept
     across calls; everything the call reads of pos, start and table is read on the device, so it can be captured."""
     what = "attn_paged"
-    _on_device(what, q, kp, vp, table, pos, start, out, lse, work)
+    gpu = _gpu(what, q, kp, vp, table, pos, start, out, lse, work)
     cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
     if start is not None:
         _vector(what, "start", start, B + 1)
@@ -563,7 +565,7 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     if work is None:
         work = attn_paged_work(M, B, Hq, Hkv, D, start is not None)
     check_rc(lib.hi_attn_paged(q.data_ptr(), ldq, *cache, _addr(start), pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), M,
-                               B, Hq, Hkv, D, work.data_ptr(), work.numel(), _stream()), what)
+                               B, Hq, Hkv, D, work.data_ptr(), work.numel(), torch._C._cuda_getCurrentRawStream(gpu)), what)
     return out
 
 
@@ -578,14 +580,14 @@ def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work
     result as attn_paged where every row of table begins with those pages; a sequence may also be shorter than the
     shared part."""
     what = "attn_shared"
-    _on_device(what, q, kp, vp, table, pos, out, lse, work)
+    gpu = _gpu(what, q, kp, vp, table, pos, out, lse, work)
     cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
     if M != B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences")
     if work is None:
         work = attn_shared_work(B, Hq, Hkv, D)
     check_rc(lib.hi_attn_shared(q.data_ptr(), ldq, *cache, shared, pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), B, Hq,
-                                Hkv, D, work.data_ptr(), work.numel(), _stream()), what)
+                                Hkv, D, work.data_ptr(), work.numel(), torch._C._cuda_getCurrentRawStream(gpu)), what)
     return out
 
 
