@@ -150,29 +150,22 @@ struct AttnArgs {
 //    those lanes, and read out of them as scalars; lane offsets inside the 8 keys never change;
 //  * page ids outside the cache: found in one pass over the block's entries before the loop; only a block that has some takes
 //    the masked tile for all of its keys, and hides them there.
-// Where the row tiles are fewer than the GPU's CUs, their keys are split (paged_plan.h); a split stores its
-// unnormalised O, m and l in fp32, in the lanes' order, and attn_join_kernel joins them.
-struct TileNote;
+// Where the row tiles are fewer than the GPU's CUs, their keys are split (paged_plan.h). A split stores its unnormalised O, m
+// and l in fp32, in the lanes' order; of each kFan splits of a tile the block that arrives last joins them, of each kFan such
+// groups the last again, until one block has the tile. Nobody waits. Against a launch of its own for the joins: 8 x 5 rows
+// after 700 to 4000 keys XXX us, 7 prompt chunks of 1 to 411 rows XXX.
 struct FlashPlan {
-  int* tiles;      // row tiles of the batch, and their notes
-  TileNote* notes;
   float *ml, *po;  // partial results: [slot][2][BQ] m and l, O [slot][RG][D / 8][64][4], a prefix's [slot][BQ][D]
   int slots;       // slots there are, each of all kv heads
   int cus;         // > 0: split over that many
   int splits;      // of the shared prefix
-  int most;        // notes there are
+  int* counters;   // [slots * Hkv], arrivals of a tile's splits
 };
 
 // What a block works on; found by every wave by itself from start and pos.
 struct FlashUnit {
   int b, row0, n, pos;   // sequence, its first row, rows, first position
   int tile, splits, split, slot;  // slot of split 0 (meaningful with splits > 1)
-  int note;                       // the tile's number in the batch (where keys may be split)
-};
-
-// What a row tile's join needs, written by the block of its first split (kv head 0).
-struct TileNote {
-  int row0, rows, first, splits, slot, pad[3];  // first row of the run, packed rows of the tile, its first packed row
 };
 
 // Integer reductions over a whole wave in DPP moves (a __shfl_xor is an LDS round trip, and a plan has dozens).
@@ -205,10 +198,9 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum
   return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
 }
 
-// Unit `at` of the batch; false if there are not so many. Wave-uniform. T: row tiles of the batch.
+// Unit `at` of the batch; false if there are not so many. Wave-uniform.
 template <int BQ>
-__device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const FlashPlan& f, int at, int lane, FlashUnit& u,
-                                           int& T) {
+__device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const FlashPlan& f, int at, int lane, FlashUnit& u) {
   const int G = a.Hq / a.Hkv;
   struct Seq { int row0, n, pos, tiles, end; };
   auto seq = [&](int b) {
@@ -225,9 +217,8 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
   };
   int L = kPlanNoSplit;
   const Seq first = seq(lane);
-  T = 0;
   if (f.cus > 0) {
-    int longest = 0;
+    int T = 0, longest = 0;
     uint32_t work = 0;  // in key tiles; under the budget's T < 2 cus it does not overflow
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       const Seq s = b0 ? seq(b0 + lane) : first;
@@ -249,14 +240,14 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
       }
     }
   }
-  int before = 0, tiles_before = 0, slot = 0;
+  int before = 0, slot = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const Seq s = b0 ? seq(b0 + lane) : first;
     const int splits = plan_splits(s.end, L);
     const int n = s.tiles * splits, own = splits > 1 ? n : 0;
     const int upto = wave_scan(n, lane);
     const uint64_t hit = __ballot(before + upto > at);
-    const int slots = f.cus > 0 ? wave_scan(own, lane) : 0, tiles_upto = f.cus > 0 ? wave_scan(s.tiles, lane) : 0;
+    const int slots = f.cus > 0 ? wave_scan(own, lane) : 0;
     if (hit) {
       const int l = __builtin_ctzll(hit);
       auto take = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
@@ -269,15 +260,28 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
       u.tile = tiles - 1 - i / u.splits;  // the most keys first
       u.split = i % u.splits;
       u.slot = slot + take(slots) - take(own) + u.tile * u.splits;
-      u.note = tiles_before + take(tiles_upto) - tiles + u.tile;
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     slot += __builtin_amdgcn_readlane(slots, 63);
-    tiles_before += __builtin_amdgcn_readlane(tiles_upto, 63);
   }
   return false;
 }
+
+constexpr int kFan = 8;  // splits that one block joins
+
+// Partial results in 16-byte pieces (index i), past the L2s, which are not coherent with each other: sc1 (bit 4).
+struct PartBuffer {
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ PartBuffer(float* p, size_t bytes)
+      : rs(__builtin_amdgcn_make_buffer_rsrc(p, (short)0, (int)bytes, 0x00020000)) {}
+  __device__ __forceinline__ void store(int64_t i, f32x4 v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, (int)(i * 16), 0, 16);
+  }
+  __device__ __forceinline__ f32x4 load(int64_t i) const {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(i * 16), 0, 16));
+  }
+};
 
 template <int D, int RG, bool PREFIX>
 __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedCache c, FlashPlan f) {
@@ -309,7 +313,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   // of the next key tile to be located: this lane's group of 8 keys, and its page
   int key = wave * KPW + 8 * (lane & (NG - 1)), id;
   if constexpr (PREFIX) {
-    u = FlashUnit{0, 0, a.M, 0, (int)(blockIdx.x / a.Hkv) / f.splits, f.splits, (int)(blockIdx.x / a.Hkv) % f.splits, 0, 0};
+    u = FlashUnit{0, 0, a.M, 0, (int)(blockIdx.x / a.Hkv) / f.splits, f.splits, (int)(blockIdx.x / a.Hkv) % f.splits, 0};
     u.slot = u.tile * f.splits;
     plan_range(a.shared, u.splits, u.split, kb, ke);
     key += kb;
@@ -318,17 +322,11 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
     for (int i = u.tile * BQ + lane; i < min((u.tile + 1) * BQ, u.n * G); i += 64) most = max(most, a.pos[i / G]);
     end = max(min(wave_most(most), a.shared - 1), -1) + 1;
   } else {
-    int T;
-    const bool any = flash_unit<BQ>(a, cap, f, blockIdx.x / a.Hkv, lane, u, T);
-    // (more tiles than notes are not split, or come of a start that gives rows to several sequences)
-    if (f.cus > 0 && blockIdx.x == 0 && tid == 0) *f.tiles = T <= f.most ? T : 0;
-    if (!any) return;
+    if (!flash_unit<BQ>(a, cap, f, blockIdx.x / a.Hkv, lane, u)) return;
     end = plan_tile_end(u.pos, u.n, u.tile, G, BQ, cap);
     plan_range(end, u.splits, u.split, kb, ke);
     key += kb;
     id = key < ke ? c.entry(u.b, key >> c.shift) : -1;
-    if (f.cus > 0 && hk == 0 && u.split == 0 && tid == 0 && u.note < f.most)
-      f.notes[u.note] = TileNote{u.row0, min(BQ, u.n * G - u.tile * BQ), u.tile * BQ, u.splits, u.slot, {}};
   }
   const int kv_end = min(ke, end);
   const int nt = kv_end > kb ? (kv_end - kb + kFpBKV - 1) / kFpBKV : 0;
@@ -466,20 +464,23 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
     ml[(RG + rg) * 64 + lane] = l_i;
   }
   __syncthreads();
-  if (kh == 1 || rg_empty) return;
-  const float m1 = ml[rg * 64 + lane], l1 = ml[(RG + rg) * 64 + lane];
-  const float m = fmaxf(m_i, m1), ref = m == -__builtin_huge_valf() ? 0.f : m;  // -inf: no key seen
-  const float a0 = __builtin_amdgcn_exp2f(m_i - ref), a1 = __builtin_amdgcn_exp2f(m1 - ref);
-  const float l = l_i * a0 + l1 * a1;
-  if (PREFIX || u.splits > 1) {  // rows behind the run hold what their zero queries gave; nothing reads them
-    if (u.slot + u.split >= f.slots) return;
-    const int64_t slot = (int64_t)(u.slot + u.split) * a.Hkv + hk;
-    if (fk == 0) {
-      f.ml[slot * 2 * BQ + rg * 32 + fr] = m;
-      f.ml[slot * 2 * BQ + BQ + rg * 32 + fr] = l;
+  const bool parts = PREFIX || u.splits > 1;
+  if (parts && u.slot + u.split >= f.slots) return;  // (not reached: the plan stays within the slots)
+  const int64_t slot = (int64_t)(u.slot + u.split) * a.Hkv + hk;
+  const PartBuffer po(f.po, (size_t)f.slots * a.Hkv * BQ * D * 4);
+  if (kh == 0 && !rg_empty) {
+    const float m1 = ml[rg * 64 + lane], l1 = ml[(RG + rg) * 64 + lane];
+    const float m = fmaxf(m_i, m1), ref = m == -__builtin_huge_valf() ? 0.f : m;  // -inf: no key seen
+    const float a0 = __builtin_amdgcn_exp2f(m_i - ref), a1 = __builtin_amdgcn_exp2f(m1 - ref);
+    const float l = l_i * a0 + l1 * a1, inv = l == 0.f ? 0.f : 1.f / l;
+    if (parts) {  // (lanes without a row store what their zero queries gave; nothing reads it)
+      if (fk == 0) {
+        st_coherent(f.ml + slot * 2 * BQ + rg * 32 + fr, m);
+        st_coherent(f.ml + slot * 2 * BQ + BQ + rg * 32 + fr, l);
+      }
+    } else if (a.lse && row && fk == 0) {
+      a.lse[(int64_t)h * a.M + qrow] = m + log2f(l);
     }
-    // a join takes them in the lanes' order; a prefix's rows are read whole
-    f32x4* po = reinterpret_cast<f32x4*>(f.po) + (PREFIX ? (slot * BQ + rg * 32 + fr) * (D / 4) + fk : (slot * RG + rg) * DT * 4 * 64 + lane);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) {
       const f32x16 o1 = mo[(rg * DT + dt) * 64 + lane];
@@ -488,25 +489,104 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
         f32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = o[dt][4 * g + e] * a0 + o1[4 * g + e] * a1;
-        po[(dt * 4 + g) * (PREFIX ? 2 : 64)] = v;
+        // a prefix's rows are read whole by the next launch, a split's by the blocks of this one, in the lanes' order
+        if (PREFIX) reinterpret_cast<f32x4*>(f.po)[(slot * BQ + rg * 32 + fr) * (D / 4) + fk + (dt * 4 + g) * 2] = v;
+        else if (parts) po.store(((slot * RG + rg) * DT * 4 + dt * 4 + g) * 64 + lane, v);
+        else if (row) {
+          f16x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[e] = (f16)(v[e] * inv);
+          *reinterpret_cast<f16x4*>(a.out + qrow * a.ldo + h * D + dt * 32 + 8 * g + 4 * fk) = w;
+        }
       }
     }
-    return;
   }
-  if (!row) return;
-  if (a.lse && fk == 0) a.lse[(int64_t)h * a.M + qrow] = m + log2f(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  f16* orow = a.out + qrow * a.ldo + h * D;
-#pragma unroll
-  for (int dt = 0; dt < DT; dt++) {
-    const f32x16 o1 = mo[(rg * DT + dt) * 64 + lane];
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      f16x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = (f16)((o[dt][4 * g + e] * a0 + o1[4 * g + e] * a1) * inv);
-      *reinterpret_cast<f16x4*>(orow + dt * 32 + 8 * g + 4 * fk) = v;
+  if (PREFIX || !parts) return;
+
+  // ---- joins: the block's waves share the row groups that have rows, and a group's waves its 8-dim chunks, CB of them requested
+  // at once. Members of a group of splits stand `step` slots apart; the joined part goes to its first member's place, its
+  // arrivals are counted at that slot's counter, one further on for every level.
+  constexpr int NC = DT * 4, CB = 4;
+  const int groups = min(RG, (u.n * G - u.tile * BQ + 31) / 32), jg = wave % groups, P = NW / groups, part = wave / groups;
+  const int jr = jg * 32 + fr, jpr = u.tile * BQ + jr;  // the lane's row here
+  const bool jrow = jpr < u.n * G;
+  const int jtoken = jrow ? jpr / G : 0, jh = hk * G + (jrow ? jpr - jtoken * G : 0);
+  f16* const jout = a.out + (int64_t)(u.row0 + jtoken) * a.ldo + jh * D + 4 * fk;
+  int n = u.splits, at = u.split, step = 1;
+  for (int level = 0;; level++, at /= kFan, n = (n + kFan - 1) / kFan, step *= kFan) {
+    const int first = at / kFan * kFan, size = min(kFan, n - first);
+    if (size == 1) continue;  // in its place already (and a counter further on may be another tile's)
+    const int64_t s0 = (int64_t)(u.slot + first * step) * a.Hkv + hk, ds = (int64_t)step * a.Hkv;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's stores are complete
+    __syncthreads();
+    if (tid == 0) {
+      int* ctr = f.counters + s0 + (int64_t)level * a.Hkv;
+      const bool last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
+      if (last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next launch
+      *flag = last;
     }
+    __syncthreads();
+    if (*flag == 0) return;
+    const bool done = n <= kFan;
+    if (part < P) {
+      float w[kFan], ls[kFan], m = -__builtin_huge_valf(), l = 0.f;
+#pragma unroll
+      for (int k = 0; k < kFan; k++) {
+        const float* p = f.ml + (s0 + min(k, size - 1) * ds) * 2 * BQ + jr;
+        w[k] = ld_coherent(p);
+        ls[k] = ld_coherent(p + BQ);
+      }
+      f32x4 v[CB][kFan];
+      auto request = [&](int c0) {
+#pragma unroll
+        for (int i = 0; i < CB; i++)
+#pragma unroll
+          for (int k = 0; k < kFan; k++)
+            if (k < size) v[i][k] = po.load((((s0 + k * ds) * RG + jg) * NC + min(c0 + i * P, NC - 1)) * 64 + lane);
+      };
+      request(part);
+#pragma unroll
+      for (int k = 0; k < kFan; k++) m = fmaxf(m, w[k]);
+      const float ref = m == -__builtin_huge_valf() ? 0.f : m;
+#pragma unroll
+      for (int k = 0; k < kFan; k++) {
+        w[k] = exp2f(w[k] - ref);
+        if (k < size) l = __builtin_fmaf(w[k], ls[k], l);
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      for (int c0 = part; c0 < NC; c0 += CB * P) {
+        if (c0 != part) request(c0);
+#pragma unroll
+        for (int i = 0; i < CB; i++) {
+          const int c8 = c0 + i * P;
+          f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < kFan; k++)
+            if (k < size)
+#pragma unroll
+              for (int e = 0; e < 4; e++) sum[e] = __builtin_fmaf(w[k], v[i][k][e], sum[e]);
+          if (c8 < NC) {
+            if (!done) {
+              po.store(((s0 * RG + jg) * NC + c8) * 64 + lane, sum);
+            } else if (jrow) {
+              f16x4 y;
+#pragma unroll
+              for (int e = 0; e < 4; e++) y[e] = (f16)(sum[e] * inv);
+              *reinterpret_cast<f16x4*>(jout + 8 * c8) = y;
+            }
+          }
+        }
+      }
+      if (part == 0 && fk == 0) {
+        if (!done) {
+          st_coherent(f.ml + s0 * 2 * BQ + jr, m);
+          st_coherent(f.ml + s0 * 2 * BQ + BQ + jr, l);
+        } else if (a.lse && jrow) {
+          a.lse[(int64_t)jh * a.M + u.row0 + jtoken] = m + log2f(l);
+        }
+      }
+    }
+    if (done) return;
   }
 }
 
@@ -532,46 +612,6 @@ __device__ __forceinline__ void join_parts(float& M, float& L, f32x4& O, const f
 #pragma unroll
     for (int e = 0; e < 4; e++) O[e] = __builtin_fmaf(w, os[k][e], O[e]);
   }
-}
-
-// Joins a tile's splits: a wave per (row tile, kv head, row group, 8 dims), in the lanes' order of the partial results: m = max
-// m_s, w_s = 2^(m_s - m), out = sum w_s O_s / sum w_s l_s. 4 parts are requested at once.
-template <int D, int RG>
-__global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a, FlashPlan f) {
-  constexpr int BQ = 32 * RG, ND = D / 8, NJ = 4;
-  const int lane = threadIdx.x, fr = lane & 31, fk = lane >> 5;
-  int i = blockIdx.x;
-  const int d8 = i % ND, rg = i / ND % RG;
-  i /= ND * RG;
-  const int hk = i % a.Hkv, tile = i / a.Hkv, G = a.Hq / a.Hkv;
-  const TileNote u = f.notes[tile];
-  if (tile >= *f.tiles || u.splits == 1 || u.slot + u.splits > f.slots) return;
-  if (rg * 32 + fr >= u.rows) return;
-  const int pr = u.first + rg * 32 + fr, token = pr / G, h = hk * G + pr - token * G;
-  const int64_t row = u.row0 + token;
-  const float* ml = f.ml + ((int64_t)u.slot * a.Hkv + hk) * 2 * BQ + rg * 32 + fr;
-  const f32x4* po = reinterpret_cast<const f32x4*>(f.po) + ((((int64_t)u.slot * a.Hkv + hk) * RG + rg) * ND + d8) * 64 + lane;
-  const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * RG * ND * 64;
-  float m = -__builtin_huge_valf(), l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < u.splits; s0 += NJ) {
-    float ms[NJ], ls[NJ];
-    f32x4 os[NJ];
-#pragma unroll
-    for (int k = 0; k < NJ; k++) {
-      const int s = min(s0 + k, u.splits - 1);
-      ms[k] = ml[s * sm];
-      ls[k] = ml[s * sm + BQ];
-      os[k] = po[s * so];
-    }
-    join_parts(m, l, o, ms, ls, os, u.splits - s0);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  f16x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = (f16)(o[e] * inv);
-  *reinterpret_cast<f16x4*>(a.out + row * a.ldo + h * D + 8 * d8 + 4 * fk) = v;
-  if (a.lse && d8 == 0 && fk == 0) a.lse[(int64_t)h * a.M + row] = m + log2f(l);
 }
 
 // ---- one row per sequence
@@ -967,15 +1007,12 @@ int flash_slots(int M, int G, int Hkv, int RG, int cus) {
 int64_t flash_tiles(int M, int B, int G, int RG) {
   return B == 1 ? plan_tiles(M, G, 32 * RG) : (int64_t)M * G / (32 * RG) + min(B, M);
 }
-size_t flash_bytes(int M, int B, int G, int Hkv, int RG, int D, int cus) {
-  const int slots = flash_slots(M, G, Hkv, RG, cus);
-  return slots ? 16 + min(flash_tiles(M, B, G, RG), (int64_t)2 * cus) * sizeof(TileNote) +
-                     (size_t)slots * Hkv * flash_slot_bytes(RG, D)
-               : 0;
+size_t flash_bytes(int M, int G, int Hkv, int RG, int D, int cus) {
+  return (size_t)flash_slots(M, G, Hkv, RG, cus) * Hkv * flash_slot_bytes(RG, D);
 }
 
-// The work buffer begins with the arrival counters, in every call: one buffer may serve calls of all forms. Only pairs
-// with more than one split count, and those are fewer than two for each CU (decode_splits).
+// The work buffer begins with the arrival counters, in every call: one buffer may serve calls of all forms. Pairs with more
+// than one split count there, which are fewer than two for each CU (decode_splits), or slots, two for each CU at most.
 constexpr int kCounters = 4096;
 constexpr size_t kWorkHead = kCounters * 4;
 
@@ -1018,29 +1055,22 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
   const int G = a.Hq / a.Hkv, cap = c.W << c.shift;
   FlashPlan f{};
   const int slots = cap > kPlanMinSplit ? flash_slots(a.M, G, a.Hkv, RG, cus) : 0;
-  const int64_t tiles = flash_tiles(a.M, a.B, G, RG);
   if (slots) {
     f.slots = slots;
     f.cus = cus;
-    f.most = (int)min(tiles, (int64_t)2 * cus);  // more tiles are not split
-    f.tiles = (int*)((char*)work + kWorkHead);
-    f.notes = (TileNote*)(f.tiles + 4);
-    f.ml = (float*)(f.notes + f.most);
+    f.counters = (int*)work;
+    f.ml = (float*)((char*)work + kWorkHead);
     f.po = f.ml + (size_t)slots * a.Hkv * 2 * 32 * RG;
   }
-  const int64_t blocks = max(tiles, (int64_t)slots) * a.Hkv, join = (int64_t)f.most * a.Hkv * RG * (D / 8);
+  const int64_t blocks = max(flash_tiles(a.M, a.B, G, RG), (int64_t)slots) * a.Hkv;
   // (the tiles of any start, also one that gives the same rows to every sequence, are counted in int)
-  if (blocks > INT32_MAX || (slots && join > INT32_MAX) || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
+  if (blocks > INT32_MAX || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
     HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
   const auto kern = attn_pages_kernel<D, RG, false>;
   const size_t lds = FpSmem<D, RG>::kBytes;
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
-  if (slots) {
-    hipLaunchKernelGGL((attn_join_kernel<D, RG>), dim3((unsigned)join), dim3(64), 0, s, a, f);
-    HI_TRY(hipGetLastError());
-  }
   return 0;
 }
 
@@ -1180,7 +1210,7 @@ HI_EXPORT size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, 
   if (M == 0 || B == 0) return kWorkHead;
   if (ragged) {
     const int RG = flash_row_groups(M, B, Hq / Hkv);
-    return kWorkHead + flash_bytes(M, B, Hq / Hkv, Hkv, RG, D, d->cus);
+    return kWorkHead + flash_bytes(M, Hq / Hkv, Hkv, RG, D, d->cus);
   }
   StepPlan f;
   bool wide;

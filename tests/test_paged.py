@@ -49,11 +49,12 @@ class Cache:
         self.k = np.full((self.pages, Hkv, page, D), np.nan, np.float16)
         self.v = np.full((self.pages, Hkv, page, D), np.inf, np.float16)
         for b, n in enumerate(lens):
-            first = 0 if b == 0 else min(shared, n)
-            for p in range(first, max(n, shared) if b == 0 else n):
+            first, last = (0, max(n, shared)) if b == 0 else (shared, n)
+            for p in range(first, last, page):
+                m = min(page, last - p)
                 pg = self.table[b, p // page]
-                self.k[pg, :, p % page] = r.standard_normal((Hkv, D)) * sd
-                self.v[pg, :, p % page] = r.standard_normal((Hkv, D))
+                self.k[pg, :, :m] = r.standard_normal((Hkv, m, D)) * sd
+                self.v[pg, :, :m] = r.standard_normal((Hkv, m, D))
         self.layout = layout
 
     def cuda(self):
@@ -279,6 +280,65 @@ def test_ragged_one_chunk(hi, T, p0, D, G, Hkv):
     compare("rows", host(got)[rows], attend(c, [(0, p0 + t) for t in rows], q[rows], Hq))
 
 
+@pytest.mark.parametrize("Hkv,G,n,p0", [(1, 1, 3, 40000), (1, 2, 64, 33000), (2, 4, 1, 60000), (1, 16, 40, 20000), (8, 4, 32, 9000)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_ragged_many_splits(hi, D, Hkv, G, n, p0):
+    """Few rows after a long context: up to a split per CU, joined in more than one level; a short sequence beside."""
+    Hq, rows, before = Hkv * G, [n, 2], [p0, 100]
+    c = Cache(75 + G, [p + m for p, m in zip(before, rows)], Hkv, D, 64)
+    q = rng(76).standard_normal((n + 2, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    start, pos = dev(np.array([0, n, n + 2], np.int32)), dev(np.array(before, np.int32))
+    work = hi.attn_paged_work(n + 2, 2, Hq, Hkv, D, ragged=True)
+    lse = torch.empty(Hq, n + 2, device="cuda")
+    got = [host(hi.attn_paged(dev(q), k, v, table, pos, Hq, Hkv, start=start, work=work, lse=lse)) for _ in range(3)]
+    at = [(b, p + t) for b, (m, p) in enumerate(zip(rows, before)) for t in range(m)]
+    some = sorted({0, n // 2, n - 1, n, n + 1})
+    want = attend(c, [at[m] for m in some], q[some], Hq)
+    compare("ragged", got[0][some], want)
+    compare_lse("ragged", host(lse)[:, some], want)
+    for g in got[1:]:
+        assert np.array_equal(bits(g), bits(got[0])), "a kept work buffer"
+    assert (work[:16384] == 0).all(), "the counters are left at zero"
+
+
+def test_one_work_buffer_for_all_forms(hi):
+    """A buffer made for one form serves the others in turn (where it is large enough), each as with its own."""
+    D, G, Hkv, B = 128, 4, 8, 12
+    Hq, lens = Hkv * G, [2500 + 31 * b for b in range(B)]
+    c = Cache(78, lens, Hkv, D, 16)
+    q = dev(rng(79).standard_normal((B, Hq * D)).astype(np.float16))
+    k, v, table = c.cuda()
+    pos = dev(np.array(lens, np.int32) - 1)
+    start = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    sizes = [hi.attn_paged_work(B, B, Hq, Hkv, D), hi.attn_paged_work(B, B, Hq, Hkv, D, ragged=True),
+             hi.attn_shared_work(B, Hq, Hkv, D)]
+    one = max(sizes, key=lambda w: w.numel())
+    one[16384:].fill_(0xff)
+
+    def forms(work):
+        yield hi.attn_paged(q, k, v, table, pos, Hq, Hkv, work=work)
+        yield hi.attn_paged(q, k, v, table, pos, Hq, Hkv, start=start, work=work)
+        yield hi.attn_shared(q, k, v, table, pos, 2048, Hq, Hkv, work=work)
+        yield hi.attn_paged(q[:1], k, v, table[:1], pos[:1], Hq, Hkv, work=work)
+    for own, shared in zip(forms(None), list(forms(one)) and forms(one)):
+        assert torch.equal(own, shared)
+
+
+def test_ragged_bad_start_large(hi):
+    """Runs that overlap and together are more than the rows there are: the call ends, nothing outside the rows is written."""
+    D, G, Hkv, M = 64, 2, 2, 700
+    c = Cache(92, [900, 900, 900], Hkv, D, 16)
+    q = rng(93).standard_normal((M, Hkv * G * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    wide = torch.full((M + 4, Hkv * G * D), 7.0, dtype=torch.float16, device="cuda")
+    for start in ([0, M, 0, M], [M, 0, M, 0], [-9, M + 9, 5, 2**31 - 1]):
+        hi.attn_paged(dev(q), k, v, table, dev(np.array([100, 200, 3], np.int32)), Hkv * G, Hkv,
+                      start=dev(np.array(start, np.int32)), out=wide[2:M + 2])
+        got = host(wide)
+        assert (got[:2] == 7).all() and (got[M + 2:] == 7).all()
+
+
 def test_ragged_many_sequences(hi):
     """More sequences than a wave's lanes, most of one row, some empty, one long."""
     D, G, Hkv, B = 64, 8, 4, 150
@@ -338,6 +398,52 @@ def test_shared(hi, D, G, Hkv, B, shared, page):
     if shared:  # the same as each sequence by itself
         alone = host(hi.attn_paged(dev(q), k, v, table, pos, Hq, Hkv))
         compare("paged", alone, want)
+
+
+@pytest.mark.parametrize("D,G,Hkv,B,shared,page", [
+    (64, 8, 4, 70, 4096, 64), (64, 8, 4, 8, 24576, 64), (128, 4, 8, 8, 8192, 128), (128, 4, 8, 70, 2048, 16),
+    (128, 6, 2, 33, 8192, 32), (64, 1, 3, 70, 8192, 128), (128, 16, 1, 40, 8192, 64), (64, 16, 1, 9, 65536, 256),
+    (64, 5, 2, 64, 8192, 8), (128, 1, 2, 100, 4096, 16)])
+def test_shared_once(hi, D, G, Hkv, B, shared, page):
+    """Batches and prefixes where reading the prefix once is faster than once per sequence: row tiles of both heights, one
+    and several, own parts in one block and in several, sequences shorter than the prefix, empty ones."""
+    own = [0, 1, 17, 300, 64, 5, 130, 1100]
+    lens = [shared + own[b % len(own)] for b in range(B)]
+    lens[2], lens[3], lens[4] = 0, shared // 2 - 3, 1
+    c = Cache(105 + B + D, lens, Hkv, D, page, layout=["packed", "joint", "strided"][B % 3], shared=shared)
+    c.table[5 % B, 0] = -1  # not looked at
+    want_table = c.table.copy()
+    want_table[:, :shared // page] = c.table[0, :shared // page]
+    Hq = Hkv * G
+    q = rng(106).standard_normal((B, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    lse = torch.empty(Hq, B, device="cuda")
+    work = hi.attn_shared_work(B, Hq, Hkv, D)
+    pos = dev(np.array(lens, np.int32) - 1)
+    got = [host(hi.attn_shared(dev(q), k, v, table, pos, shared, Hq, Hkv, lse=lse, work=work)) for _ in range(2)]
+    c.table = want_table
+    rows = sorted({0, 1, 2, 3, 4, 5, 6, 7, B // 2, B - 1})
+    want = attend(c, [(b, lens[b] - 1) for b in rows], q[rows], Hq)
+    compare("shared", got[0][rows], want)
+    compare_lse("shared", host(lse)[:, rows], want)
+    assert np.array_equal(bits(got[0]), bits(got[1])), "a kept work buffer"
+    alone = hi.attn_paged(dev(q), k, v, dev(want_table), pos, Hq, Hkv)
+    # each is within 2^-10 1.125 (sum w |v|) of the exact value, and |v| < 2^3
+    assert (alone.float() - torch.from_numpy(got[0]).cuda().float()).abs().max().item() <= 2 * 2**-10 * 1.125 * 8
+
+
+def test_shared_unwritten_tail(hi):
+    """All sequences shorter than the prefix: the positions behind the longest hold NaN and inf, and take no part."""
+    D, G, Hkv, B, page, shared = 128, 4, 8, 40, 16, 4096
+    lens = [1000 + 7 * b for b in range(B)]
+    c = Cache(108, [max(lens)], Hkv, D, page, shared=0)
+    c.table = np.concatenate([c.table, np.full((1, shared // page - c.table.shape[1]), c.pages - 1, np.int32)], 1)
+    c.table = np.repeat(c.table, B, 0)
+    Hq = Hkv * G
+    q = rng(109).standard_normal((B, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    got = hi.attn_shared(dev(q), k, v, table, dev(np.array(lens, np.int32) - 1), shared, Hq, Hkv)
+    compare("shared", host(got), attend(c, [(b, n - 1) for b, n in enumerate(lens)], q, Hq))
 
 
 def test_shared_long(hi):
