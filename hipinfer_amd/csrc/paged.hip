@@ -136,6 +136,8 @@ struct AttnArgs {
   float* lse;  // [Hq][M] or null
   const int *start, *pos;
   int M, B, Hq, Hkv, shared;  // positions below `shared` are on the pages of table row 0
+  int G;                      // Hq / Hkv, and what divides by it (plan_token)
+  uint32_t magic;
   float scale_log2;
 };
 
@@ -157,7 +159,7 @@ struct AttnArgs {
 struct FlashPlan {
   float *ml, *po;  // partial results: [slot][2][BQ] m and l, O [slot][RG][D / 8][64][4], a prefix's [slot][BQ][D]
   int slots;       // slots there are, each of all kv heads
-  int cus;         // > 0: split over that many
+  int cus, b1, b2; // > 0: split over that many; plan_budget's quotients
   int splits;      // of the shared prefix
   int* counters;   // [slots * Hkv], arrivals of a tile's splits
 };
@@ -201,8 +203,7 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive sum
 // Unit `at` of the batch; false if there are not so many. Wave-uniform.
 template <int BQ>
 __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const FlashPlan& f, int at, int lane, FlashUnit& u) {
-  const int G = a.Hq / a.Hkv;
-  struct Seq { int row0, n, pos, tiles, end; };
+  struct Seq { int row0, n, pos, tiles, te; };  // te: key tiles
   auto seq = [&](int b) {
     Seq s{0, 0, 0, 0, 0};
     if (b < a.B) {
@@ -210,8 +211,8 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
       s.pos = a.pos[b];
       s.row0 = plan_first(s0, a.M);
       s.n = plan_rows(s0, s1, a.M);
-      s.tiles = plan_tiles(s.n, G, BQ);
-      s.end = plan_end(s.pos, s.n, cap);
+      s.tiles = plan_tiles(s.n, a.G, BQ);
+      s.te = plan_key_tiles(plan_end(s.pos, s.n, cap));
     }
     return s;
   };
@@ -223,18 +224,18 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       const Seq s = b0 ? seq(b0 + lane) : first;
       T += s.tiles;
-      work += (uint32_t)s.tiles * plan_key_tiles(s.end);
-      if (s.tiles) longest = max(longest, s.end);
+      work += (uint32_t)s.tiles * (uint32_t)s.te;
+      if (s.tiles) longest = max(longest, s.te);
     }
     T = wave_total(T);
-    const int budget = plan_budget(T, a.Hkv, f.cus);
+    const int budget = plan_budget(T, a.Hkv, f.cus, f.b1, f.b2);
     if (budget > 0) {
       longest = wave_most(longest);
       for (L = plan_length((uint32_t)wave_total((int)work), budget); L < longest; L = plan_longer(L)) {
         int units = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
           const Seq s = b0 ? seq(b0 + lane) : first;
-          units += s.tiles * plan_splits(s.end, L);
+          units += s.tiles * plan_splits(s.te, L);
         }
         if (wave_total(units) <= min(budget, f.slots)) break;
       }
@@ -243,7 +244,7 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
   int before = 0, slot = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const Seq s = b0 ? seq(b0 + lane) : first;
-    const int splits = plan_splits(s.end, L);
+    const int splits = plan_splits(s.te, L);
     const int n = s.tiles * splits, own = splits > 1 ? n : 0;
     const int upto = wave_scan(n, lane);
     const uint64_t hit = __ballot(before + upto > at);
@@ -257,8 +258,9 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
       u.pos = take(s.pos);
       u.splits = take(splits);
       const int tiles = take(s.tiles), i = at - before - (take(upto) - take(n));
-      u.tile = tiles - 1 - i / u.splits;  // the most keys first
-      u.split = i % u.splits;
+      const int down = u.splits == 1 ? i : plan_div(i, u.splits);
+      u.tile = tiles - 1 - down;  // the most keys first
+      u.split = i - down * u.splits;
       u.slot = slot + take(slots) - take(own) + u.tile * u.splits;
       return true;
     }
@@ -305,25 +307,25 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wave % RG, kh = wave / RG;     // row group, key half
   const int fr = lane & 31, fk = lane >> 5;
-  const int G = a.Hq / a.Hkv, page = 1 << c.shift, cap = c.capacity();
-  const int hk = blockIdx.x % a.Hkv;            // blocks of a kv head on as few XCDs as there can be
+  const int G = a.G, page = 1 << c.shift, cap = c.capacity();
+  const int hk = blockIdx.x;                    // grid (Hkv, units): a kv head's blocks on as few XCDs as there can be
   FlashUnit u;
   int end;     // keys that some row of the tile sees
   int kb, ke;  // the split's
   // of the next key tile to be located: this lane's group of 8 keys, and its page
   int key = wave * KPW + 8 * (lane & (NG - 1)), id;
   if constexpr (PREFIX) {
-    u = FlashUnit{0, 0, a.M, 0, (int)(blockIdx.x / a.Hkv) / f.splits, f.splits, (int)(blockIdx.x / a.Hkv) % f.splits, 0};
+    u = FlashUnit{0, 0, a.M, 0, (int)blockIdx.z, f.splits, (int)blockIdx.y, 0};
     u.slot = u.tile * f.splits;
     plan_range(a.shared, u.splits, u.split, kb, ke);
     key += kb;
     id = key < ke ? c.entry(0, key >> c.shift) : -1;  // requested together with the positions
     int most = -1;  // the last position of any of the tile's rows
-    for (int i = u.tile * BQ + lane; i < min((u.tile + 1) * BQ, u.n * G); i += 64) most = max(most, a.pos[i / G]);
+    for (int i = u.tile * BQ + lane; i < min((u.tile + 1) * BQ, u.n * G); i += 64) most = max(most, a.pos[plan_token(i, a.magic)]);
     end = max(min(wave_most(most), a.shared - 1), -1) + 1;
   } else {
-    if (!flash_unit<BQ>(a, cap, f, blockIdx.x / a.Hkv, lane, u)) return;
-    end = plan_tile_end(u.pos, u.n, u.tile, G, BQ, cap);
+    if (!flash_unit<BQ>(a, cap, f, blockIdx.y, lane, u)) return;
+    end = plan_tile_end(u.pos, u.n, u.tile, G, a.magic, BQ, cap);
     plan_range(end, u.splits, u.split, kb, ke);
     key += kb;
     id = key < ke ? c.entry(u.b, key >> c.shift) : -1;
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   // this lane's row and the last key it sees
   const int pr = u.tile * BQ + rg * 32 + fr;
   const bool row = pr < u.n * G;
-  const int token = row ? pr / G : 0, h = hk * G + (row ? pr - token * G : 0);
+  const int token = row ? plan_token(pr, a.magic) : 0, h = hk * G + (row ? pr - token * G : 0);
   const int64_t qrow = u.row0 + token;
   int qpos = -1;
   if (row) qpos = PREFIX ? min(a.pos[token], a.shared - 1) : (int)min((int64_t)u.pos + token, (int64_t)cap - 1);
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   const int groups = min(RG, (u.n * G - u.tile * BQ + 31) / 32), jg = wave % groups, P = NW / groups, part = wave / groups;
   const int jr = jg * 32 + fr, jpr = u.tile * BQ + jr;  // the lane's row here
   const bool jrow = jpr < u.n * G;
-  const int jtoken = jrow ? jpr / G : 0, jh = hk * G + (jrow ? jpr - jtoken * G : 0);
+  const int jtoken = jrow ? plan_token(jpr, a.magic) : 0, jh = hk * G + (jrow ? jpr - jtoken * G : 0);
   f16* const jout = a.out + (int64_t)(u.row0 + jtoken) * a.ldo + jh * D + 4 * fk;
   int n = u.splits, at = u.split, step = 1;
   for (int level = 0;; level++, at /= kFan, n = (n + kFan - 1) / kFan, step *= kFan) {
@@ -658,14 +660,14 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
   constexpr int NT = NWV * 64;
   typedef typename std::conditional<DL == 8, u32x4, u32x2>::type VT;
   __shared__ StepSmem<GC, D, NWV, OWN> sh;
-  // split-major blocks: a pair's used splits come first in dispatch order
-  const int nhb = a.B * a.Hkv, G = a.Hq / a.Hkv, page = 1 << c.shift;
-  const int split = blockIdx.x / nhb, hk = blockIdx.x % a.Hkv, b = (blockIdx.x % nhb) / a.Hkv;
+  // grid (Hkv, B, S): a pair's used splits come first in dispatch order
+  const int G = a.G, page = 1 << c.shift, split = blockIdx.z, hk = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = step_keys(a, c.capacity(), b, OWN ? a.shared : 0);
   const int S_eff = splits_used(len, f.S, f.S1);
   if (split >= S_eff) return;
-  const int chunk = (((len + S_eff - 1) / S_eff) + 7) & ~7;  // the groups of 8 keys start on multiples of 8
+  // (the groups of 8 keys start on multiples of 8)
+  const int chunk = ((len < kPlanDiv ? plan_div(len + S_eff - 1, S_eff) : (len + S_eff - 1) / S_eff) + 7) & ~7;
   const int base = OWN ? a.shared : 0;
   const int start = base + split * chunk, end = base + min(len, (split + 1) * chunk);
 
@@ -1000,7 +1002,7 @@ size_t flash_slot_bytes(int RG, int D) { return (size_t)32 * RG * (D + 2) * 4; }
 // tiles are too many to be split.
 int flash_slots(int M, int G, int Hkv, int RG, int cus) {
   const int least = plan_tiles(M, G, 32 * RG);
-  return plan_budget(least, Hkv, cus) ? max(2 * cus / Hkv, 1) : 0;
+  return plan_budget(least, Hkv, cus, cus / Hkv, 2 * cus / Hkv) ? max(2 * cus / Hkv, 1) : 0;
 }
 
 // Row tiles that the rows can make: every sequence with rows has at most one part-filled tile.
@@ -1052,24 +1054,26 @@ int flash_fits(K kern, int threads, size_t lds, const char* who) {
 
 template <int D, int RG>
 int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
-  const int G = a.Hq / a.Hkv, cap = c.W << c.shift;
+  const int G = a.G, cap = c.W << c.shift;
   FlashPlan f{};
-  const int slots = cap > kPlanMinSplit ? flash_slots(a.M, G, a.Hkv, RG, cus) : 0;
+  const int slots = cap > kPlanMinSplit * kPlanTile ? flash_slots(a.M, G, a.Hkv, RG, cus) : 0;
   if (slots) {
     f.slots = slots;
     f.cus = cus;
+    f.b1 = cus / a.Hkv;
+    f.b2 = 2 * cus / a.Hkv;
     f.counters = (int*)work;
     f.ml = (float*)((char*)work + kWorkHead);
     f.po = f.ml + (size_t)slots * a.Hkv * 2 * 32 * RG;
   }
-  const int64_t blocks = max(flash_tiles(a.M, a.B, G, RG), (int64_t)slots) * a.Hkv;
+  const int64_t units = max(flash_tiles(a.M, a.B, G, RG), (int64_t)slots);
   // (the tiles of any start, also one that gives the same rows to every sequence, are counted in int)
-  if (blocks > INT32_MAX || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
+  if (units > 65535 || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
     HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
   const auto kern = attn_pages_kernel<D, RG, false>;
   const size_t lds = FpSmem<D, RG>::kBytes;
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
+  hipLaunchKernelGGL(kern, dim3(a.Hkv, (unsigned)units), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
   return 0;
 }
@@ -1077,10 +1081,9 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
 template <int D, bool OWN>
 int step_launch(const AttnArgs& a, const PagedCache& c, const StepPlan& f, const FlashPlan& pf, int BQ, bool wide,
                 hipStream_t s, const char* who) {
-  const int64_t blocks = (int64_t)f.S * a.B * a.Hkv;
-  if (blocks > INT32_MAX) HI_FAIL("%s: %d sequences of %d kv heads are too many", who, a.B, a.Hkv);
-  const dim3 grid((unsigned)blocks);
-  const int G = a.Hq / a.Hkv;
+  if (a.B > 65535) HI_FAIL("%s: %d sequences (at most 65535)", who, a.B);
+  const dim3 grid(a.Hkv, a.B, f.S);
+  const int G = a.G;
   if (G > 8) hipLaunchKernelGGL((attn_step_kernel<16, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
   else if (G > 4) {
     if (wide) hipLaunchKernelGGL((attn_step_kernel<8, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f, pf, BQ);
@@ -1097,7 +1100,7 @@ template <int D>
 int step_run(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
   StepPlan f;
   bool wide;
-  step_splits(a.B, a.Hkv, a.Hq / a.Hkv, cus, f, wide);
+  step_splits(a.B, a.Hkv, a.G, cus, f, wide);
   f.counters = (int*)work;
   f.ml = (float*)((char*)work + kWorkHead);
   f.po = f.ml + step_ml(f, a.B, a.Hq);
@@ -1114,7 +1117,7 @@ size_t shared_bytes(int B, int Hq, int Hkv, int D, int cus) {
 
 template <int D, int RG>
 int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
-  const int G = a.Hq / a.Hkv, T = plan_tiles(a.M, G, 32 * RG);
+  const int G = a.G, T = plan_tiles(a.M, G, 32 * RG);
   StepPlan st;
   bool wide;
   step_splits(a.B, a.Hkv, G, cus, st, wide);
@@ -1126,12 +1129,11 @@ int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, h
   f.slots = T * f.splits;
   f.ml = st.po + (size_t)a.B * a.Hq * st.S * D;
   f.po = f.ml + (size_t)f.slots * a.Hkv * 2 * 32 * RG;
-  const int64_t blocks = (int64_t)f.slots * a.Hkv;
-  if (blocks > INT32_MAX) HI_FAIL("%s: %d sequences are too many", who, a.B);
+  if (a.B > 65535) HI_FAIL("%s: %d sequences (at most 65535)", who, a.B);
   const auto kern = attn_pages_kernel<D, RG, true>;
   const size_t lds = FpSmem<D, RG>::kBytes;
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(128 * RG), lds, s, a, c, f);
+  hipLaunchKernelGGL(kern, dim3(a.Hkv, f.splits, T), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
   return step_launch<D, true>(a, c, st, f, 32 * RG, wide, s, who);
 }
@@ -1149,7 +1151,7 @@ int attn_check(const char* who, const void* q, int ldq, const int* pos, const vo
 }
 
 int attn_run(const AttnArgs& a, const PagedCache& c, int D, int cus, void* work, hipStream_t s, const char* who) {
-  const int G = a.Hq / a.Hkv;
+  const int G = a.G;
   if (a.start) {
     const bool small = flash_row_groups(a.M, a.B, G) == 2;
     return D == 64 ? (small ? flash_launch<64, 2>(a, c, cus, work, s, who) : flash_launch<64, 4>(a, c, cus, work, s, who))
@@ -1233,7 +1235,8 @@ HI_EXPORT int hi_attn_paged(const void* q, int ldq, const void* kp, const void* 
     HI_FAIL("%s: work of %zu bytes (at least %zu, 16-byte aligned)", who, work_bytes, need);
   const HiDevice* d = hi_device();
   if (!d) return -2;
-  const AttnArgs a{(const f16*)q, ldq, (f16*)out, ldo, lse, start, pos, M, B, Hq, Hkv, 0, 1.4426950408889634f / sqrtf((float)D)};
+  const AttnArgs a{(const f16*)q, ldq, (f16*)out, ldo, lse, start, pos, M, B, Hq, Hkv, 0, Hq / Hkv, plan_magic(Hq / Hkv),
+                   1.4426950408889634f / sqrtf((float)D)};
   return attn_run(a, c, D, d->cus, work, (hipStream_t)stream, who);
 }
 
@@ -1258,6 +1261,7 @@ HI_EXPORT int hi_attn_shared(const void* q, int ldq, const void* kp, const void*
     HI_FAIL("%s: work of %zu bytes (at least %zu, 16-byte aligned)", who, work_bytes, need);
   const HiDevice* d = hi_device();
   if (!d) return -2;
-  const AttnArgs a{(const f16*)q, ldq, (f16*)out, ldo, lse, nullptr, pos, B, B, Hq, Hkv, shared, 1.4426950408889634f / sqrtf((float)D)};
+  const AttnArgs a{(const f16*)q, ldq, (f16*)out, ldo, lse, nullptr, pos, B, B, Hq, Hkv, shared, Hq / Hkv, plan_magic(Hq / Hkv),
+                   1.4426950408889634f / sqrtf((float)D)};
   return attn_run(a, c, D, d->cus, work, (hipStream_t)stream, who);
 }

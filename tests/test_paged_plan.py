@@ -23,26 +23,26 @@ extern "C" int cut(const int* start, const int* pos, int B, int M, int G, int BQ
     const int n = plan_rows(start[b], start[b + 1], M), t = plan_tiles(n, G, BQ), e = plan_end(pos[b], n, cap);
     T += t;
     work += (uint32_t)t * plan_key_tiles(e);
-    if (t) longest = std::max(longest, e);
+    if (t) longest = std::max(longest, plan_key_tiles(e));
   }
   int L = kPlanNoSplit;
-  const int budget = slots ? plan_budget(T, Hkv, cus) : 0;
+  const int budget = slots ? plan_budget(T, Hkv, cus, cus / Hkv, 2 * cus / Hkv) : 0;
   if (budget > 0)
     for (L = plan_length(work, budget); L < longest; L = plan_longer(L)) {
       int units = 0;
       for (int b = 0; b < B; b++) {
         const int n = plan_rows(start[b], start[b + 1], M);
-        units += plan_tiles(n, G, BQ) * plan_splits(plan_end(pos[b], n, cap), L);
+        units += plan_tiles(n, G, BQ) * plan_splits(plan_key_tiles(plan_end(pos[b], n, cap)), L);
       }
       if (units <= std::min(budget, slots)) break;
     }
   int n_out = 0, slot = 0;
   for (int b = 0; b < B; b++) {
-    const int n = plan_rows(start[b], start[b + 1], M), t = plan_tiles(n, G, BQ), s = plan_splits(plan_end(pos[b], n, cap), L);
+    const int n = plan_rows(start[b], start[b + 1], M), t = plan_tiles(n, G, BQ), s = plan_splits(plan_key_tiles(plan_end(pos[b], n, cap)), L);
     for (int i = 0; i < t * s; i++) {
       const int tile = t - 1 - i / s, split = i % s;
       int kb, ke;
-      plan_range(plan_tile_end(pos[b], n, tile, G, BQ, cap), s, split, kb, ke);
+      plan_range(plan_tile_end(pos[b], n, tile, G, plan_magic(G), BQ, cap), s, split, kb, ke);
       if (n_out == room) return -1;
       int* o = out + 7 * n_out++;
       o[0] = b, o[1] = tile, o[2] = split, o[3] = kb, o[4] = ke, o[5] = s > 1 ? slot + tile * s + split : -1, o[6] = s;
@@ -51,7 +51,8 @@ extern "C" int cut(const int* start, const int* pos, int B, int M, int G, int BQ
   }
   return n_out;
 }
-extern "C" int budget_of(int T, int Hkv, int cus) { return plan_budget(T, Hkv, cus); }
+extern "C" int budget_of(int T, int Hkv, int cus) { return plan_budget(T, Hkv, cus, cus / Hkv, 2 * cus / Hkv); }
+extern "C" int token_of(int r, int G) { return plan_token(r, plan_magic(G)); }
 extern "C" int tiles_of(int n, int G, int BQ) { return plan_tiles(n, G, BQ); }
 """
 
@@ -119,6 +120,14 @@ def test_bad_start_stays_in_bounds(plan, start):
     units, tiles, slots = cut(plan, start, [100, 5000, 2**31 - 1], 6, 4, 64, 8, 8192)
     for b, tile, split, kb, ke, slot, s in units:
         assert 0 <= kb <= ke <= 8192 and slot < slots
+
+
+def test_token_is_exact(plan):
+    r = random.Random(0)
+    for G in range(1, 17):
+        for _ in range(3000):
+            n = r.choice([r.randint(0, 300), r.randint(0, 1 << 27), (1 << 27) - r.randint(1, 40)])
+            assert plan.token_of(n, G) == n // G
 
 
 def test_one_sequence_fills_the_gpu(plan):
