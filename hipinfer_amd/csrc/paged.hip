@@ -626,7 +626,8 @@ __device__ __forceinline__ void join_parts(float& M, float& L, f32x4& O, const f
 // keys that are not there become -inf, their V rows zeros.
 // OWN: the keys behind a shared prefix, whose own splits' results (FlashPlan) are joined in when a pair's are.
 struct StepPlan {
-  int S, S1;      // splits of a pair: the launch's, and those that give every CU its blocks (splits_used)
+  int S, S1;      // splits of a pair: the launch's, and those that give every CU a block (splits_used)
+  int K;          // > 0: a split per K keys instead
   int* counters;  // [B * Hkv], arrivals of a pair's splits
   float *ml, *po; // partial results: [B][Hq][S][2] m and l, [B][Hq][S][D] O
 };
@@ -664,7 +665,7 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
   const int G = a.G, page = 1 << c.shift, split = blockIdx.z, hk = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = step_keys(a, c.capacity(), b, OWN ? a.shared : 0);
-  const int S_eff = splits_used(len, f.S, f.S1);
+  const int S_eff = f.K > 0 ? max(1, min(f.S, plan_div(len + f.K - 1, f.K))) : splits_used(len, f.S, f.S1);
   if (split >= S_eff) return;
   // (the groups of 8 keys start on multiples of 8)
   const int chunk = ((len < kPlanDiv ? plan_div(len + S_eff - 1, S_eff) : (len + S_eff - 1) / S_eff) + 7) & ~7;
@@ -1013,16 +1014,32 @@ size_t flash_bytes(int M, int G, int Hkv, int RG, int D, int cus) {
   return (size_t)flash_slots(M, G, Hkv, RG, cus) * Hkv * flash_slot_bytes(RG, D);
 }
 
-// The work buffer begins with the arrival counters, in every call: one buffer may serve calls of all forms. Pairs with more
-// than one split count there, which are fewer than two for each CU (decode_splits), or slots, two for each CU at most.
+// The work buffer begins with the arrival counters, in every call: one buffer may serve calls of all forms. Pairs (sequence, kv
+// head) with more than one split count there, or slots, two for each CU at most.
 constexpr int kCounters = 4096;
 constexpr size_t kWorkHead = kCounters * 4;
 
+// Splits of a decode step's pairs. With at most an eighth as many pairs as CUs, blocks of 8 waves and the slot cache's rule
+// (decode_split.h): the step is a chain of latencies. With more, blocks of 4 waves and a split per 256 keys (pairs for a
+// quarter of the CUs), 320 (for one a CU) or 768: a batch of mixed lengths ends with its longest blocks, while every split
+// costs its part's way through memory; equal lengths lose 1 to 3 %. Measured against that rule for all, us: 100 sequences of
+// 50 to 2000 keys, 12/2 heads of 128, 35.7 -> 28.0; 31 of 1 to 300, 32/8 of 128, 11.4 -> 8.5; 120 of 1 to 700, 32/4 of 64, 15.3
+// -> 12.3; 30 of 500 to 4000, 32/8 of 128, 65.3 -> 60.4; 48 of 100 to 2000 46.8 -> 46.8; 16 of 4097 52.3 -> 54.0. (192, 320
+// or 352 keys for the first two and 704 or 1024 for the last: within 3 % over 17 batches, 288 and 12 splits worse.) From two
+// pairs a CU on, a split per 4096 keys only, so that one long sequence does not hold up the batch: 64 of 1000 keys lose 12 %
+// by a second split. A sequence's splits depend on the batch's size, not on the other lengths.
 void step_splits(int B, int Hkv, int G, int cus, StepPlan& f, bool& wide) {
-  f.S1 = decode_splits(B, Hkv, cus);
-  wide = G <= 8 && f.S1 >= kDaWideSplits;
-  if (wide) f.S = f.S1 = decode_splits_wide(B, Hkv, cus);
-  else f.S = decode_splits_max(B, Hkv, f.S1, cus);
+  const int64_t pairs = (int64_t)B * Hkv;
+  f.K = 0;
+  wide = G <= 8 && decode_splits(B, Hkv, cus) >= kDaWideSplits;
+  if (wide) {
+    f.S = f.S1 = decode_splits_wide(B, Hkv, cus);
+    return;
+  }
+  f.S1 = 1;
+  f.S = pairs > kCounters ? 1 : (int)min((int64_t)8, 4 * kCounters / pairs);
+  if (pairs < 2 * cus) f.S = max(f.S, decode_splits(B, Hkv, cus));
+  f.K = 4 * pairs <= cus ? 256 : pairs <= cus ? 320 : pairs < 2 * cus ? 768 : 4096;
 }
 // Floats of the partial results' m and l, a multiple of 4 (O is read in 16-byte pieces).
 size_t step_ml(const StepPlan& f, int B, int Hq) { return ((size_t)B * Hq * f.S * 2 + 3) & ~(size_t)3; }
