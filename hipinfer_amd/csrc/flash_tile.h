@@ -6,6 +6,8 @@
 //   issue_k(i, st), issue_v(i, st)               DMA instruction i of the next K (V) tile into stage st
 //   advance()                                    called once before the DMA of each K tile but the first
 //   before_barrier(), after_barrier()            called around the prologue's barrier, before n_full is read
+//   kGuard, odd_tile                             whether infinities and NaN in V are taken out of masked tiles, and the first
+//                                                tile where any were (INT_MAX)
 //   enter_masked(t), hidden(t, kt, e)            whether the lane's query does not see element e of key block kt of tile t
 //   xor32(v)                                     lane l ^ 32's v
 //   m_i, l_i, o                                  the row's reference max (-inf), the lane's share of its sum (0), O^T (0)
@@ -68,6 +70,34 @@
       pf[e >> 3][(e & 7) + 1] = (f16)p1;
     }
     l_i += sum0 + sum1;
+  };
+
+  // Infinities and NaN in the V rows of a masked tile t: a row that does not see them has weight 0 there, and 0 times either is
+  // NaN. They leave the fragments, and the kernel gives them to the rows that do see them.
+  auto guard = [&](int t, f16x8 (&vf)[2][DT]) __attribute__((always_inline)) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int ss = 0; ss < 2; ss++)
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) {
+        const u32x4 w = __builtin_bit_cast(u32x4, vf[ss][dt]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) odd |= (w[i] & 0x7fff7fffu) + 0x04000400u;  // an exponent of ones carries into the sign
+      }
+    if (!__any((odd & 0x80008000u) != 0)) return;
+    odd_tile = min(odd_tile, t);
+#pragma unroll
+    for (int ss = 0; ss < 2; ss++)
+#pragma unroll
+      for (int dt = 0; dt < DT; dt++) {
+        u32x4 w = __builtin_bit_cast(u32x4, vf[ss][dt]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if ((w[i] & 0x7c00u) == 0x7c00u) w[i] &= 0xffff0000u;
+          if ((w[i] & 0x7c000000u) == 0x7c000000u) w[i] &= 0x0000ffffu;
+        }
+        vf[ss][dt] = __builtin_bit_cast(f16x8, w);
+      }
   };
 
   // One key tile t (stage t & 1, given as a constant in the main loop): the softmax and P.V of its
@@ -199,9 +229,11 @@
     }
     softmax(sc[0], m_use, pf);
     load_v(st, 0, vf);
+    if constexpr (MASK && kGuard) guard(t, vf);
     pv(vf, pf);
     softmax(sc[1], m_use, pl);
     load_v(st, 1, vl);
+    if constexpr (MASK && kGuard) guard(t, vl);
     if constexpr (NEXT) {
       __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
 #pragma unroll

@@ -451,7 +451,29 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
       return k0 <= most && k0 < kv_end;
     };
 
+    constexpr bool kGuard = true;
+    int odd_tile = INT32_MAX;
 #include "flash_tile.h"
+    // the infinities and NaN of the masked tiles, key by key (rare: fp16 overflow in a V row)
+#pragma unroll 1
+    for (int ot = odd_tile; ot < nt; ot++) {
+      const int k0 = kb + ot * kFpBKV + kFpKPW * kh;
+#pragma unroll 1
+      for (int k = k0; k < min(k0 + kFpKPW, kv_end); k++) {
+        const int vid = c.entry(tb, k >> c.shift);
+        if (!c.has(vid)) continue;
+        const f16* vrow = c.vp + vid * c.stride + ((int64_t)hk * page + (k & (page - 1))) * D + 4 * fk;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const f16x4 x = *reinterpret_cast<const f16x4*>(vrow + dt * 32 + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (k <= qpos && !(__builtin_fabsf((float)x[e]) < __builtin_huge_valf())) o[dt][4 * g + e] += (float)x[e];
+          }
+      }
+    }
   }
 
   // ---- merge the two key halves of each row group: the second wave hands (m, l, O) over

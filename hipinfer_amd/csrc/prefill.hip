@@ -131,6 +131,8 @@ __global__ void __launch_bounds__(128 * RG)
     return t * kFpBKV + kFpKPW * kh + 32 * kt + 8 * (e >> 2) + 4 * fk + (e & 3) > qpos;
   };
   auto enter_masked = [](int) {};
+  constexpr bool kGuard = false;
+  int odd_tile = 0;
   auto advance = [] {};
   auto before_barrier = [] {};
   auto after_barrier = [] {};

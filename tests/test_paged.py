@@ -225,6 +225,50 @@ def test_infinite_logits(hi, D):
     assert np.isfinite(out).all()
 
 
+def same_where_finite(name, got, want):
+    """Within the tolerance where the result is finite, the same infinity where it is one, NaN where it is."""
+    out, tol, _ = want
+    got = got.astype(np.float64)
+    assert np.array_equal(np.isnan(got), np.isnan(out)), f"{name}: NaN in {np.argwhere(np.isnan(got) != np.isnan(out))[:4]}"
+    big = np.isinf(out)
+    assert np.array_equal(got[big], out[big]), name
+    fine = np.isfinite(out)
+    assert (np.abs(got[fine] - out[fine]) <= tol[fine]).all(), name
+
+
+@pytest.mark.parametrize("D,G,Hkv", HEADS, ids=IDS)
+@pytest.mark.parametrize("form", ["ragged", "shared"])
+def test_later_infinities(hi, D, G, Hkv, form):
+    """Infinities and NaN in the V rows, and in the K rows, of positions that a row does not see do not reach it; in V rows
+    that it sees they give what the sum gives."""
+    Hq, page, n, p0 = Hkv * G, 16, 150, 90
+    total = p0 + n if form == "ragged" else 8192
+    c = Cache(55 + G, [total], Hkv, D, page)
+    r = rng(56)
+    spots = r.choice(np.arange(p0 + 20, p0 + n - 5), 9, replace=False)
+    for i, p in enumerate(sorted(spots)):
+        c.v[c.table[0, p // page], :, p % page, (7 * i) % D] = [np.inf, -np.inf, np.nan][i % 3]
+    c.v[c.table[0, max(spots) // page], :, max(spots) % page, 7 * 2 % D] = np.inf
+    last = p0 + n - 3
+    c.k[c.table[0, last // page], :, last % page, :] = np.inf
+    if form == "ragged":
+        q = r.standard_normal((n, Hq * D)).astype(np.float16)
+        k, v, table = c.cuda()
+        got = host(hi.attn_paged(dev(q), k, v, table, dev(np.array([p0], np.int32)), Hq, Hkv,
+                                 start=dev(np.array([0, n], np.int32))))
+        at = [(0, p0 + t) for t in range(n - 3)]
+        same_where_finite("ragged", got[:n - 3], attend(c, at, q[:n - 3], Hq))
+        assert np.isnan(got[n - 3:]).all(), "rows that see the infinite key"
+        return
+    B = 60  # sequences whose last position lies in the shared part, among them some that see each of the spots
+    at = [(0, int(p)) for p in r.integers(p0, last, B)]
+    c.table = np.repeat(c.table, B, 0)
+    q = r.standard_normal((B, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    got = host(hi.attn_shared(dev(q), k, v, table, dev(np.array([p for _, p in at], np.int32)), total, Hq, Hkv))
+    same_where_finite("shared", got, attend(c, at, q, Hq))
+
+
 # ------------------------------------------------------------------ ragged batches
 RAGGED = [  # rows of each sequence, cached positions before them
     ([5, 5, 5], [100, 0, 1000]),
