@@ -892,25 +892,27 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
         for (int k = 0; k < 16; k++) v0[e][k] = ld_coherent(pp + (int64_t)min(k, S_eff - 1) * D);
       }
     }
-    for (int i = tid; i < G * S_eff; i += NT) {
-      const int g = i / S_eff, s = i - g * S_eff;
-      const float* pp = f.ml + ((pair + g) * f.S + s) * 2;
-      sh.sm[g][s] = ld_coherent(pp);
-      sh.sw[g][s] = ld_coherent(pp + 1);
-    }
-    __syncthreads();
-    for (int g = wave; g < G; g += NWV) {  // S_eff is at most a wave's lanes
-      const float ms = lane < S_eff ? sh.sm[g][lane] : -__builtin_huge_valf(), ls = lane < S_eff ? sh.sw[g][lane] : 0.f;
-      const float M = wave_max(ms);
-      const float e = ms == -__builtin_huge_valf() ? 0.f : exp2f(ms - M);
-      const float L = wave_sum(ls * e);
-      if (lane < S_eff) sh.sw[g][lane] = e;
-      if (lane == 0) {
-        sh.tm[g] = M;
-        sh.tl[g] = L;
+    if constexpr (!OWN) {
+      for (int i = tid; i < G * S_eff; i += NT) {
+        const int g = i / S_eff, s = i - g * S_eff;
+        const float* pp = f.ml + ((pair + g) * f.S + s) * 2;
+        sh.sm[g][s] = ld_coherent(pp);
+        sh.sw[g][s] = ld_coherent(pp + 1);
       }
+      __syncthreads();
+      for (int g = wave; g < G; g += NWV) {  // S_eff is at most a wave's lanes
+        const float ms = lane < S_eff ? sh.sm[g][lane] : -__builtin_huge_valf(), ls = lane < S_eff ? sh.sw[g][lane] : 0.f;
+        const float M = wave_max(ms);
+        const float e = ms == -__builtin_huge_valf() ? 0.f : exp2f(ms - M);
+        const float L = wave_sum(ls * e);
+        if (lane < S_eff) sh.sw[g][lane] = e;
+        if (lane == 0) {
+          sh.tm[g] = M;
+          sh.tl[g] = L;
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
   // splits s0 .. s0 + 15 of element (g, d)
   auto sum16 = [&](int g, const float (&v)[16], int s0, float& O) {
@@ -956,24 +958,24 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
         const int64_t slot = (int64_t)tile * pf.splits * a.Hkv + hk;
         const float* ml = pf.ml + slot * 2 * BQ + at;
         const float* po = pf.po + (slot * BQ + at) * D + d;
-        if (part == 0) {  // the sequence's own keys
-          if (single) {
+        if (single) {  // the sequence's own keys
+          if (part == 0) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               float v;
               block_sum(g, d + e, M, L, v);
               O[e] = v;
             }
-          } else {
-            M = sh.tm[g];
-            L = sh.tl[g];
+          }
+        } else {
 #pragma unroll 1
-            for (int s = 0; s < S_eff; s++) {
-              const float w = sh.sw[g][s];
-              const float* pp = f.po + ((pair + g) * f.S + s) * D + d;
+          for (int s = part; s < S_eff; s += P) {
+            const int64_t own = (pair + g) * f.S + s;
+            const float ms[1] = {ld_coherent(f.ml + 2 * own)}, ls[1] = {ld_coherent(f.ml + 2 * own + 1)};
+            f32x4 os[1];
 #pragma unroll
-              for (int e = 0; e < 4; e++) O[e] = __builtin_fmaf(ld_coherent(pp + e), w, O[e]);
-            }
+            for (int e = 0; e < 4; e++) os[0][e] = ld_coherent(f.po + own * D + d + e);
+            join_parts(M, L, O, ms, ls, os, 1);
           }
         }
 #pragma unroll 1
