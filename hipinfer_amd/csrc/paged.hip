@@ -285,8 +285,9 @@ struct PartBuffer {
   }
 };
 
+// One block: kv head hk of unit `unit`, or with PREFIX split `unit` of row tile `tile` of the shared prefix.
 template <int D, int RG, bool PREFIX>
-__global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedCache c, FlashPlan f) {
+__device__ __forceinline__ void pages_block(const AttnArgs& a, const PagedCache& c, const FlashPlan& f, int hk, int unit, int tile) {
   constexpr int NW = 2 * RG, BQ = 32 * RG;
   constexpr int CPR = D / 8;                   // 16-byte chunks per key row
   constexpr int IPW = kFpBKV * CPR / 64 / NW;  // DMA instructions per wave per tile and operand
@@ -308,14 +309,13 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   const int rg = wave % RG, kh = wave / RG;     // row group, key half
   const int fr = lane & 31, fk = lane >> 5;
   const int G = a.G, page = 1 << c.shift, cap = c.capacity();
-  const int hk = blockIdx.x;                    // grid (Hkv, units): a kv head's blocks on as few XCDs as there can be
   FlashUnit u;
   int end;     // keys that some row of the tile sees
   int kb, ke;  // the split's
   // of the next key tile to be located: this lane's group of 8 keys, and its page
   int key = wave * KPW + 8 * (lane & (NG - 1)), id;
   if constexpr (PREFIX) {
-    u = FlashUnit{0, 0, a.M, 0, (int)blockIdx.z, f.splits, (int)blockIdx.y, 0};
+    u = FlashUnit{0, 0, a.M, 0, tile, f.splits, unit, 0};
     u.slot = u.tile * f.splits;
     plan_range(a.shared, u.splits, u.split, kb, ke);
     key += kb;
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
     for (int i = u.tile * BQ + lane; i < min((u.tile + 1) * BQ, u.n * G); i += 64) most = max(most, a.pos[plan_token(i, a.magic)]);
     end = max(min(wave_most(most), a.shared - 1), -1) + 1;
   } else {
-    if (!flash_unit<BQ>(a, cap, f, blockIdx.y, lane, u)) return;
+    if (!flash_unit<BQ>(a, cap, f, unit, lane, u)) return;
     end = plan_tile_end(u.pos, u.n, u.tile, G, a.magic, BQ, cap);
     plan_range(end, u.splits, u.split, kb, ke);
     key += kb;
@@ -614,6 +614,12 @@ __global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedC
   }
 }
 
+// grid (Hkv, units): a kv head's blocks are on as few XCDs as there can be
+template <int D, int RG>
+__global__ void __launch_bounds__(128 * RG) attn_pages_kernel(AttnArgs a, PagedCache c, FlashPlan f) {
+  pages_block<D, RG, false>(a, c, f, blockIdx.x, blockIdx.y, 0);
+}
+
 // Joins N parts (m, l, O) to the running (M, L, O), which is relative to M (-inf: no key yet); parts from `count` on are
 // left out.
 template <int N>
@@ -646,7 +652,7 @@ __device__ __forceinline__ void join_parts(float& M, float& L, f32x4& O, const f
 // one 64-bit address each for K and V per tile, from entries requested a tile ahead. What the slot kernel leaves to the
 // buffer bounds is done in registers, in a wave's last tile and in tiles with an entry that is no page only: logits of
 // keys that are not there become -inf, their V rows zeros.
-// OWN: the keys behind a shared prefix, whose own splits' results (FlashPlan) are joined in when a pair's are.
+// OWN: the keys behind a shared prefix; every split leaves its part for attn_parts_kernel.
 struct StepPlan {
   int S, S1;      // splits of a pair: the launch's, and those that give every CU a block (splits_used)
   int K;          // > 0: a split per K keys instead
@@ -659,35 +665,48 @@ __device__ __forceinline__ int step_keys(const AttnArgs& a, int cap, int b, int 
   return plan_end(a.pos[b], 1, cap) > base ? plan_end(a.pos[b], 1, cap) - base : 0;
 }
 
-template <int NT>
-struct OwnSmem {
-  float m[NT], l[NT];
-  f32x4 o[NT];
-};
-
-template <int GC, int D, int NWV, bool OWN>
+template <int GC, int D, int NWV>
 struct StepSmem {
   float wo[NWV][GC][D];
   float wm[NWV][GC], wl[NWV][GC];
   float sm[GC][kDecodeMaxSplits], sw[GC][kDecodeMaxSplits];
   float tm[GC], tl[GC];
   int is_last;
-  OwnSmem<OWN ? NWV * 64 : 1> own;
 };
 
+// Element d of head g over a block's waves.
+template <int GC, int D, int NWV>
+__device__ __forceinline__ void step_sum(const StepSmem<GC, D, NWV>& sh, int g, int d, float& M, float& L, float& O) {
+  M = -__builtin_huge_valf();
+#pragma unroll
+  for (int w = 0; w < NWV; w++) M = fmaxf(M, sh.wm[w][g]);
+  L = O = 0.f;
+#pragma unroll
+  for (int w = 0; w < NWV; w++) {
+    const float e = sh.wm[w][g] == -__builtin_huge_valf() ? 0.f : exp2f(sh.wm[w][g] - M);
+    L = __builtin_fmaf(sh.wl[w][g], e, L);
+    O = __builtin_fmaf(sh.wo[w][g][d], e, O);
+  }
+}
+
+// Splits that a run of len keys is cut into.
+__device__ __forceinline__ int step_used(const StepPlan& f, int len) {
+  return f.K > 0 ? max(1, min(f.S, plan_div(len + f.K - 1, f.K))) : splits_used(len, f.S, f.S1);
+}
+
+// One block: split `split` of sequence b and kv head hk. With `keep` a sequence's only part is left in the waves' LDS (step_sum).
 template <int GC, int D, int NWV, bool OWN>
-__global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, PagedCache c, StepPlan f, FlashPlan pf, int BQ) {
+__device__ __forceinline__ void step_block(const AttnArgs& a, const PagedCache& c, const StepPlan& f,
+                                           StepSmem<GC, D, NWV>& sh, int hk, int b, int split, bool keep = false) {
   constexpr int KS = D / 32;               // k steps of a logits product
   constexpr int DL = D / 16;               // V dims (and P.V products) per lane
   constexpr int BK = NWV * kDaTile;        // keys per block pass
   constexpr int NT = NWV * 64;
   typedef typename std::conditional<DL == 8, u32x4, u32x2>::type VT;
-  __shared__ StepSmem<GC, D, NWV, OWN> sh;
-  // grid (Hkv, B, S): a pair's used splits come first in dispatch order
-  const int G = a.G, page = 1 << c.shift, split = blockIdx.z, hk = blockIdx.x, b = blockIdx.y;
+  const int G = a.G, page = 1 << c.shift;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = step_keys(a, c.capacity(), b, OWN ? a.shared : 0);
-  const int S_eff = f.K > 0 ? max(1, min(f.S, plan_div(len + f.K - 1, f.K))) : splits_used(len, f.S, f.S1);
+  const int S_eff = step_used(f, len);
   if (split >= S_eff) return;
   // (the groups of 8 keys start on multiples of 8)
   const int chunk = ((len < kPlanDiv ? plan_div(len + S_eff - 1, S_eff) : (len + S_eff - 1) / S_eff) + 7) & ~7;
@@ -830,46 +849,32 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
   }
   __syncthreads();
   const bool single = S_eff == 1;
+  if (OWN && keep && single) return;
   const int64_t pair = (int64_t)b * a.Hq + hk * G;  // of head 0 of the group; its partials start at pair * S
-  // element d of head g over the block's waves
-  auto block_sum = [&](int g, int d, float& M, float& L, float& O) {
-    M = -__builtin_huge_valf();
-#pragma unroll
-    for (int w = 0; w < NWV; w++) M = fmaxf(M, sh.wm[w][g]);
-    L = O = 0.f;
-#pragma unroll
-    for (int w = 0; w < NWV; w++) {
-      const float e = sh.wm[w][g] == -__builtin_huge_valf() ? 0.f : exp2f(sh.wm[w][g] - M);
-      L = __builtin_fmaf(sh.wl[w][g], e, L);
-      O = __builtin_fmaf(sh.wo[w][g][d], e, O);
-    }
-  };
   auto store = [&](int g, int d, float M, float L, float O) {
     a.out[(int64_t)b * a.ldo + (hk * G + g) * D + d] = (f16)(L == 0.f ? 0.f : O / L);
     if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
   };
-  if (!single || !OWN) {
-    for (int i = tid; i < G * D; i += NT) {
-      const int g = i / D, d = i % D;
-      float M, L, O;
-      block_sum(g, d, M, L, O);
-      if (single) {
-        store(g, d, M, L, O);
-      } else {
-        const int64_t at = (pair + g) * f.S + split;
-        st_coherent(f.po + at * D + d, O);
-        if (d == 0) {
-          st_coherent(f.ml + 2 * at, M);
-          st_coherent(f.ml + 2 * at + 1, L);
-        }
+  for (int i = tid; i < G * D; i += NT) {
+    const int g = i / D, d = i % D;
+    float M, L, O;
+    step_sum(sh, g, d, M, L, O);
+    const int64_t at = (pair + g) * f.S + split;
+    if (!OWN && single) {
+      store(g, d, M, L, O);
+    } else {
+      st_coherent(f.po + at * D + d, O);
+      if (d == 0) {
+        st_coherent(f.ml + 2 * at, M);
+        st_coherent(f.ml + 2 * at + 1, L);
       }
     }
-    if (single) return;
   }
+  if (OWN || single) return;
   constexpr int EPT = (GC * D + NT - 1) / NT;  // output elements per thread
-  constexpr bool AHEAD = !OWN && GC <= 8;      // (16 heads would not fit the registers)
+  constexpr bool AHEAD = GC <= 8;      // (16 heads would not fit the registers)
   float v0[EPT][16];
-  if (!single) {
+  {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partial stores are complete
     __syncthreads();
     if (tid == 0) {
@@ -892,7 +897,7 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
         for (int k = 0; k < 16; k++) v0[e][k] = ld_coherent(pp + (int64_t)min(k, S_eff - 1) * D);
       }
     }
-    if constexpr (!OWN) {
+    {
       for (int i = tid; i < G * S_eff; i += NT) {
         const int g = i / S_eff, s = i - g * S_eff;
         const float* pp = f.ml + ((pair + g) * f.S + s) * 2;
@@ -924,7 +929,7 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
 #pragma unroll
     for (int k = 0; k < 16; k++) v[k] = ld_coherent(pp + (int64_t)min(s0 + k, S_eff - 1) * D);
   };
-  if constexpr (!OWN) {
+  {
 #pragma unroll
     for (int e = 0; e < EPT; e++) {
       const int i = tid + e * NT;
@@ -940,82 +945,164 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
         store(g, d, sh.tm[g], sh.tl[g], O);
       }
     }
-  } else {
-    // With the prefix's parts: a thread takes 4 dims of a head, and where there are more threads than those, every P-th part,
-    // 8 requested at once; the P threads' results are joined through LDS.
-    constexpr int D4 = D / 4;
-    const int items = G * D4, P = items < NT ? NT / items : 1;
-    const int64_t sm = (int64_t)a.Hkv * 2 * BQ, so = (int64_t)a.Hkv * BQ * D;
+  }
+}
+
+// grid (Hkv, B, S): a pair's used splits come first in dispatch order
+template <int GC, int D, int NWV>
+__global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, PagedCache c, StepPlan f) {
+  __shared__ StepSmem<GC, D, NWV> sh;
+  step_block<GC, D, NWV, false>(a, c, f, sh, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// ---- a shared prefix
+//
+// Its parts (pages_block) and the sequences' own keys (step_block) are computed apart and joined. Where the prefix leaves half
+// of the GPU idle, both run in one launch, and a launch for the joins follows; else the own keys run in a second launch,
+// whose blocks join.
+constexpr int kPartThreads = 256;
+struct PartSmem {
+  float m[kPartThreads], l[kPartThreads];
+  f32x4 o[kPartThreads];
+};
+
+// Joins the prefix's parts and the `own` parts of sequence b, kv head hk. A thread takes 4 dims of a head, and where there are
+// more threads than those, every P-th part, 8 requested at once; the P threads' results are joined through LDS. SAME: the
+// own parts come of this launch; an only one is asked of sum(g, d, M, L, O).
+template <int D, bool SAME, typename Sum>
+__device__ __forceinline__ void join_block(const AttnArgs& a, const FlashPlan& f, const StepPlan& st, int BQ, PartSmem& sh, int hk,
+                                           int b, int own, Sum sum) {
+  constexpr int D4 = D / 4, NT = kPartThreads;
+  const int G = a.G, tid = threadIdx.x, S = f.splits;
+  const int items = G * D4, P = items < NT ? NT / items : 1;
+  const int64_t dm = (int64_t)a.Hkv * 2 * BQ, dn = (int64_t)a.Hkv * BQ * D;
 #pragma unroll 1
-    for (int i0 = 0; i0 < items; i0 += NT) {
-      const int part = items < NT ? tid / items : 0, item = items < NT ? tid - part * items : i0 + tid;
-      const bool active = part < P && item < items;
-      const int g = item / D4, d = 4 * (item % D4);
-      float M = -__builtin_huge_valf(), L = 0.f;
-      f32x4 O = {0.f, 0.f, 0.f, 0.f};
-      if (active) {
-        const int pr = b * G + g, tile = pr / BQ, at = pr - tile * BQ;
-        const int64_t slot = (int64_t)tile * pf.splits * a.Hkv + hk;
-        const float* ml = pf.ml + slot * 2 * BQ + at;
-        const float* po = pf.po + (slot * BQ + at) * D + d;
-        if (single) {  // the sequence's own keys
-          if (part == 0) {
+  for (int i0 = 0; i0 < items; i0 += NT) {
+    const int part = items < NT ? tid / items : 0, item = items < NT ? tid - part * items : i0 + tid;
+    const bool active = part < P && item < items;
+    const int g = item / D4, d = 4 * (item % D4);
+    float M = -__builtin_huge_valf(), L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    if (active) {
+      const int pr = b * G + g, tile = pr / BQ, at = pr - tile * BQ;
+      const int64_t slot = (int64_t)tile * S * a.Hkv + hk, mine = ((int64_t)b * a.Hq + hk * G + g) * st.S;
+      const float* ml = f.ml + slot * 2 * BQ + at;
+      const float* po = f.po + (slot * BQ + at) * D + d;
+      if (SAME && own == 1) {
+        if (part == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              float v;
-              block_sum(g, d + e, M, L, v);
-              O[e] = v;
-            }
-          }
-        } else {
-#pragma unroll 1
-          for (int s = part; s < S_eff; s += P) {
-            const int64_t own = (pair + g) * f.S + s;
-            const float ms[1] = {ld_coherent(f.ml + 2 * own)}, ls[1] = {ld_coherent(f.ml + 2 * own + 1)};
-            f32x4 os[1];
-#pragma unroll
-            for (int e = 0; e < 4; e++) os[0][e] = ld_coherent(f.po + own * D + d + e);
-            join_parts(M, L, O, ms, ls, os, 1);
+          for (int e = 0; e < 4; e++) {
+            float v;
+            sum(g, d + e, M, L, v);
+            O[e] = v;
           }
         }
+      } else {
 #pragma unroll 1
-        for (int s0 = part; s0 < pf.splits; s0 += 8 * P) {
-          float ms[8], ls[8];
-          f32x4 os[8];
+        for (int s = part; s < own; s += P) {
+          const float* p = st.ml + 2 * (mine + s);
+          const float* q = st.po + (mine + s) * D + d;
+          const float ms[1] = {SAME ? ld_coherent(p) : p[0]}, ls[1] = {SAME ? ld_coherent(p + 1) : p[1]};
+          f32x4 os[1];
 #pragma unroll
-          for (int k = 0; k < 8; k++) {
-            const int s = min(s0 + k * P, pf.splits - 1);
-            ms[k] = ml[s * sm];
-            ls[k] = ml[s * sm + BQ];
-            os[k] = *reinterpret_cast<const f32x4*>(po + s * so);
-          }
-          join_parts(M, L, O, ms, ls, os, (pf.splits - s0 + P - 1) / P);
+          for (int e = 0; e < 4; e++) os[0][e] = SAME ? ld_coherent(q + e) : q[e];
+          join_parts(M, L, O, ms, ls, os, 1);
         }
       }
-      if (P > 1) {
-        __syncthreads();
-        if (active && part > 0) {
-          sh.own.m[tid] = M;
-          sh.own.l[tid] = L;
-          sh.own.o[tid] = O;
-        }
-        __syncthreads();
-        if (active && part == 0)
-          for (int p = 1; p < P; p++) {
-            const float ms[1] = {sh.own.m[p * items + item]}, ls[1] = {sh.own.l[p * items + item]};
-            const f32x4 os[1] = {sh.own.o[p * items + item]};
-            join_parts(M, L, O, ms, ls, os, 1);
-          }
-      }
-      if (active && part == 0) {
-        f16x4 v;
+#pragma unroll 1
+      for (int s0 = part; s0 < S; s0 += 8 * P) {
+        float ms[8], ls[8];
+        f32x4 os[8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = (f16)(L == 0.f ? 0.f : O[e] / L);
-        *reinterpret_cast<f16x4*>(a.out + (int64_t)b * a.ldo + (hk * G + g) * D + d) = v;
-        if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
+        for (int k = 0; k < 8; k++) {
+          const int s = min(s0 + k * P, S - 1);
+          ms[k] = ml[s * dm];
+          ls[k] = ml[s * dm + BQ];
+          os[k] = *reinterpret_cast<const f32x4*>(po + s * dn);
+        }
+        join_parts(M, L, O, ms, ls, os, (S - s0 + P - 1) / P);
       }
     }
+    if (P > 1) {
+      __syncthreads();
+      sh.m[tid] = M;
+      sh.l[tid] = L;
+      sh.o[tid] = O;
+      __syncthreads();
+      if (active && part == 0)
+        for (int p = 1; p < P; p++) {
+          const float ms[1] = {sh.m[p * items + item]}, ls[1] = {sh.l[p * items + item]};
+          const f32x4 os[1] = {sh.o[p * items + item]};
+          join_parts(M, L, O, ms, ls, os, 1);
+        }
+    }
+    if (active && part == 0) {
+      f16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = (f16)(L == 0.f ? 0.f : O[e] / L);
+      *reinterpret_cast<f16x4*>(a.out + (int64_t)b * a.ldo + (hk * G + g) * D + d) = v;
+      if (a.lse && d == 0) a.lse[(int64_t)(hk * G + g) * a.M + b] = M + log2f(L);
+    }
   }
+}
+
+// grid (Hkv, prefix blocks + own blocks): the prefix's splits x tiles first, then (with both kinds in one launch) blocks
+// that take the sequences' splits in turn, sequence by sequence and split by split.
+template <int GC, int D, int RG>
+__global__ void __launch_bounds__(128 * RG) attn_prefix_kernel(AttnArgs a, PagedCache c, FlashPlan f, StepPlan st, int tiles) {
+  const int np = f.splits * tiles, y = blockIdx.y;
+  if (y < np) {
+    const int split = tiles == 1 ? y : y / tiles;
+    pages_block<D, RG, true>(a, c, f, blockIdx.x, split, y - split * tiles);
+    return;
+  }
+  extern __shared__ u32x4 fp_smem[];
+  auto& sh = *reinterpret_cast<StepSmem<GC, D, 2 * RG>*>(fp_smem);
+  const int step = gridDim.y - np;
+  int b = y - np, split = 0;
+  for (;; b += step) {
+    while (b >= a.B) {
+      b -= a.B;
+      split++;
+    }
+    if (split >= st.S) break;
+    // (turned by split: the same blocks would get the long sequences' splits again)
+    const int turned = b + split * (a.B / 2 + 1) % a.B;
+    step_block<GC, D, 2 * RG, true>(a, c, st, sh, blockIdx.x, turned < a.B ? turned : turned - a.B, split);
+    __syncthreads();  // the block's LDS is used again
+  }
+}
+
+// After it, where it took the sequences' splits too: grid (Hkv, B).
+template <int D>
+__global__ void __launch_bounds__(kPartThreads) attn_parts_kernel(AttnArgs a, int cap, FlashPlan f, StepPlan st, int BQ) {
+  __shared__ PartSmem sh;
+  join_block<D, false>(a, f, st, BQ, sh, blockIdx.x, blockIdx.y, step_used(st, step_keys(a, cap, blockIdx.y, a.shared)),
+                       [](int, int, float&, float&, float&) {});
+}
+
+// Else: grid (Hkv, B, S).
+template <int GC, int D>
+__global__ void __launch_bounds__(kPartThreads, 3) attn_own_kernel(AttnArgs a, PagedCache c, FlashPlan f, StepPlan st, int BQ) {
+  __shared__ StepSmem<GC, D, 4> sh;
+  __shared__ PartSmem ps;
+  const int hk = blockIdx.x, b = blockIdx.y, split = blockIdx.z;
+  const int own = step_used(st, step_keys(a, c.capacity(), b, a.shared));
+  if (split >= own) return;
+  step_block<GC, D, 4, true>(a, c, st, sh, hk, b, split, true);
+  if (own > 1) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partial stores are complete
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int* ctr = st.counters + b * a.Hkv + hk;
+      sh.is_last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == own - 1;
+      if (sh.is_last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next launch
+    }
+    __syncthreads();
+    if (!sh.is_last) return;
+  }
+  join_block<D, true>(a, f, st, BQ, ps, hk, b, own,
+                      [&](int g, int d, float& M, float& L, float& O) { step_sum(sh, g, d, M, L, O); });
 }
 
 // Row groups per block: 4 (128 packed rows), or 2 where a sequence has 64 packed rows or less on average.
@@ -1069,19 +1156,25 @@ void step_splits(int B, int Hkv, int G, int cus, StepPlan& f, bool& wide) {
 size_t step_ml(const StepPlan& f, int B, int Hq) { return ((size_t)B * Hq * f.S * 2 + 3) & ~(size_t)3; }
 size_t step_bytes(const StepPlan& f, int B, int Hq, int D) { return (step_ml(f, B, Hq) + (size_t)B * Hq * f.S * D) * 4; }
 
-// Splits of a prefix of `shared` positions for T row tiles: a block for each CU.
-int prefix_splits(int T, int Hkv, int shared, int cus) {
-  return max(1, min(cus / max(1, T * Hkv), max((shared + 255) / 256, min(8, (shared + 127) / 128))));
+// Splits of a prefix of `shared` positions for T row tiles, and whether the own keys go into the same launch (`mixed`): where
+// half of the CUs are through with the prefix in 12 key tiles, the other half takes the own keys; beyond that the prefix needs
+// all of them, and the own keys are faster in small blocks after it. Apart / mixed, us, 32/8 heads of 128: 32 sequences
+// after 8192 with 300 own keys 33.2 / 25.3, 8 after 8192 23.7 / 18.5, 32 after 16384 (8 tiles) with 30 32.0 / 29.2, 64 after
+// 32768 (32 tiles) with 200 66.9 / 81.5, 8 after 32768 (16 tiles) with 300 42.4 / 44.1.
+int prefix_splits(int T, int Hkv, int shared, int cus, bool& mixed) {
+  const int te = plan_key_tiles(shared), half = max(1, cus / 2 / max(1, T * Hkv)), S = max(1, min(half, te / 4));
+  mixed = 2 * T * Hkv <= cus && (te + S - 1) / S <= 12;
+  return mixed ? S : max(1, min(cus / max(1, T * Hkv), (te + 1) / 2));
 }
 
-// Whether a decode step that reads the prefix again for every sequence is faster. Its re-reads mostly hit the caches, at 12
-// TB/s; sharing costs 10 us (a launch more, the parts' way through memory) and the prefix once, at 6 TB/s or 500 TFLOP/s.
-// Measured with 2 to 64 sequences after prefixes of 512 to 32768, 20 or 300 keys of their own, in 32/8 and 12/2 heads of
-// 128 and 32/4 of 64: 1 % above the faster of the two on average (us, sharing / re-reading: 8 after 2048, 32/8 of 128, 17.1 /
-// 14.2; after 8192 24.4 / 28.4; 32 after 8192 30.5 / 81.1; 4 after 16384 25.4 / 27.5).
+// Whether a decode step that reads the prefix again for every sequence is faster. Its re-reads mostly hit the caches, at 14
+// TB/s; reading it once costs 5 us (a second launch, the parts' way through memory) and the prefix at 8 TB/s. Measured with 2
+// to 64 sequences after prefixes of 512 to 32768, 20 or 300 keys of their own, in 32/8 and 12/2 heads of 128 and 32/4 of
+// 64: 0.5 % above the faster of the two on average (us, once / again, 300 own keys, 32/8 of 128: 4 after 4096 16.6 / 14.1,
+// after 16384 23.4 / 27.8; 8 after 2048 16.7 / 15.0, after 4096 17.4 / 19.9; 32 after 1024 22.8 / 25.1, after 4096 23.2 / 52.1).
 bool prefix_reread(const AttnArgs& a, int D) {
-  const double mb = 4e-6 * a.shared * a.Hkv * D, mflop = 4e-6 * D * a.Hq * a.shared * a.B;
-  return a.B * mb / 12 < 10 + fmax(mb / 6, mflop / 500);
+  const double mb = 4e-6 * a.shared * a.Hkv * D;
+  return a.B * mb / 14 < 5 + mb / 8;
 }
 
 // Largest grid's blocks and what a kernel's LDS limit needs; 0, or a negative code.
@@ -1111,7 +1204,7 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
   // (the tiles of any start, also one that gives the same rows to every sequence, are counted in int)
   if (units > 65535 || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
     HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
-  const auto kern = attn_pages_kernel<D, RG, false>;
+  const auto kern = attn_pages_kernel<D, RG>;
   const size_t lds = FpSmem<D, RG>::kBytes;
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
   hipLaunchKernelGGL(kern, dim3(a.Hkv, (unsigned)units), dim3(128 * RG), lds, s, a, c, f);
@@ -1119,64 +1212,87 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
   return 0;
 }
 
-template <int D, bool OWN>
-int step_launch(const AttnArgs& a, const PagedCache& c, const StepPlan& f, const FlashPlan& pf, int BQ, bool wide,
-                hipStream_t s, const char* who) {
-  if (a.B > 65535) HI_FAIL("%s: %d sequences (at most 65535)", who, a.B);
-  const dim3 grid(a.Hkv, a.B, f.S);
-  const int G = a.G;
-  if (G > 8) hipLaunchKernelGGL((attn_step_kernel<16, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
-  else if (G > 4) {
-    if (wide) hipLaunchKernelGGL((attn_step_kernel<8, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f, pf, BQ);
-    else hipLaunchKernelGGL((attn_step_kernel<8, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
-  } else {
-    if (wide) hipLaunchKernelGGL((attn_step_kernel<4, D, 8, OWN>), grid, dim3(512), 0, s, a, c, f, pf, BQ);
-    else hipLaunchKernelGGL((attn_step_kernel<4, D, 4, OWN>), grid, dim3(256), 0, s, a, c, f, pf, BQ);
-  }
-  HI_TRY(hipGetLastError());
-  return 0;
-}
-
 template <int D>
 int step_run(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
+  if (a.B > 65535) HI_FAIL("%s: %d sequences (at most 65535)", who, a.B);
   StepPlan f;
   bool wide;
   step_splits(a.B, a.Hkv, a.G, cus, f, wide);
   f.counters = (int*)work;
   f.ml = (float*)((char*)work + kWorkHead);
   f.po = f.ml + step_ml(f, a.B, a.Hq);
-  return step_launch<D, false>(a, c, f, FlashPlan{}, 0, wide, s, who);
+  const dim3 grid(a.Hkv, a.B, f.S);
+  const int G = a.G;
+  if (G > 8) hipLaunchKernelGGL((attn_step_kernel<16, D, 4>), grid, dim3(256), 0, s, a, c, f);
+  else if (G > 4) {
+    if (wide) hipLaunchKernelGGL((attn_step_kernel<8, D, 8>), grid, dim3(512), 0, s, a, c, f);
+    else hipLaunchKernelGGL((attn_step_kernel<8, D, 4>), grid, dim3(256), 0, s, a, c, f);
+  } else {
+    if (wide) hipLaunchKernelGGL((attn_step_kernel<4, D, 8>), grid, dim3(512), 0, s, a, c, f);
+    else hipLaunchKernelGGL((attn_step_kernel<4, D, 4>), grid, dim3(256), 0, s, a, c, f);
+  }
+  HI_TRY(hipGetLastError());
+  return 0;
+}
+
+// Splits of the sequences' own keys behind a shared prefix. In the prefix's launch, one per 512 keys (256 in blocks of 4
+// waves), up to 8; in their own, as any decode step in blocks of 4 waves.
+void own_splits(int B, int Hkv, int RG, int cus, bool mixed, StepPlan& f) {
+  bool wide;
+  step_splits(B, Hkv, 16, cus, f, wide);  // (more than 8 heads a group: never blocks of 8 waves)
+  if (!mixed) return;
+  f.S = 8;
+  f.K = RG == 2 ? 256 : 512;
 }
 
 size_t shared_bytes(int B, int Hq, int Hkv, int D, int cus) {
+  size_t most = 0;
   StepPlan st;
   bool wide;
-  step_splits(B, Hkv, Hq / Hkv, cus, st, wide);
+  step_splits(B, Hkv, Hq / Hkv, cus, st, wide);  // the prefix read again for every sequence
+  most = step_bytes(st, B, Hq, D);
   const int RG = flash_row_groups(B, 1, Hq / Hkv), T = plan_tiles(B, Hq / Hkv, 32 * RG);
-  return step_bytes(st, B, Hq, D) + (size_t)T * max(1, cus / max(1, T * Hkv)) * Hkv * flash_slot_bytes(RG, D);
+  for (const bool mixed : {false, true}) {
+    own_splits(B, Hkv, RG, cus, mixed, st);
+    most = max(most, step_bytes(st, B, Hq, D) + (size_t)T * max(1, cus / max(1, T * Hkv)) * Hkv * flash_slot_bytes(RG, D));
+  }
+  return most;
 }
 
 template <int D, int RG>
 int shared_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
-  const int G = a.G, T = plan_tiles(a.M, G, 32 * RG);
+  const int G = a.G, T = plan_tiles(a.M, G, 32 * RG), BQ = 32 * RG;
+  if (a.B > 65535) HI_FAIL("%s: %d sequences (at most 65535)", who, a.B);
+  bool mixed;
+  FlashPlan f{};
+  f.splits = prefix_splits(T, a.Hkv, a.shared, cus, mixed);
+  f.slots = T * f.splits;
   StepPlan st;
-  bool wide;
-  step_splits(a.B, a.Hkv, G, cus, st, wide);
+  own_splits(a.B, a.Hkv, RG, cus, mixed, st);
+  if (mixed) st.S = max(1, min(st.S, ((c.W << c.shift) - a.shared + st.K - 1) / st.K));
   st.counters = (int*)work;
   st.ml = (float*)((char*)work + kWorkHead);
   st.po = st.ml + step_ml(st, a.B, a.Hq);
-  FlashPlan f{};
-  f.splits = prefix_splits(T, a.Hkv, a.shared, cus);
-  f.slots = T * f.splits;
   f.ml = st.po + (size_t)a.B * a.Hq * st.S * D;
-  f.po = f.ml + (size_t)f.slots * a.Hkv * 2 * 32 * RG;
-  if (a.B > 65535) HI_FAIL("%s: %d sequences (at most 65535)", who, a.B);
-  const auto kern = attn_pages_kernel<D, RG, true>;
+  f.po = f.ml + (size_t)f.slots * a.Hkv * 2 * BQ;
+  // twice the blocks that the prefix leaves room for (two blocks a CU at D = 64): fewer or more are slower
+  const int room = (D == 64 ? 2 : 1) * cus - f.slots * a.Hkv, own = mixed ? max(1, min(a.B * st.S, 2 * room / a.Hkv)) : 0;
+  const auto kern = G > 8 ? attn_prefix_kernel<16, D, RG> : G > 4 ? attn_prefix_kernel<8, D, RG> : attn_prefix_kernel<4, D, RG>;
   const size_t lds = FpSmem<D, RG>::kBytes;
+  static_assert(sizeof(StepSmem<16, D, 2 * RG>) <= FpSmem<D, RG>::kBytes, "both kinds of blocks fit the LDS");
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
-  hipLaunchKernelGGL(kern, dim3(a.Hkv, f.splits, T), dim3(128 * RG), lds, s, a, c, f);
+  hipLaunchKernelGGL(kern, dim3(a.Hkv, f.slots + own), dim3(128 * RG), lds, s, a, c, f, st, T);
   HI_TRY(hipGetLastError());
-  return step_launch<D, true>(a, c, st, f, 32 * RG, wide, s, who);
+  if (mixed) {
+    hipLaunchKernelGGL((attn_parts_kernel<D>), dim3(a.Hkv, a.B), dim3(kPartThreads), 0, s, a, c.W << c.shift, f, st, BQ);
+  } else {
+    const dim3 grid(a.Hkv, a.B, st.S);
+    if (G > 8) hipLaunchKernelGGL((attn_own_kernel<16, D>), grid, dim3(kPartThreads), 0, s, a, c, f, st, BQ);
+    else if (G > 4) hipLaunchKernelGGL((attn_own_kernel<8, D>), grid, dim3(kPartThreads), 0, s, a, c, f, st, BQ);
+    else hipLaunchKernelGGL((attn_own_kernel<4, D>), grid, dim3(kPartThreads), 0, s, a, c, f, st, BQ);
+  }
+  HI_TRY(hipGetLastError());
+  return 0;
 }
 
 int attn_check(const char* who, const void* q, int ldq, const int* pos, const void* out, int ldo, const float* lse, int M,

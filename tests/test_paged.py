@@ -713,6 +713,36 @@ def test_captured_and_grown(hi, form):
         pos.copy_(torch.minimum(pos * 2 + 1, limit))
 
 
+def test_pages_behind_4_gib(hi):
+    """Page ids whose byte and element offsets pass 32 bits: the same bits as the same pages in a small cache."""
+    D, G, Hkv, page, B = 128, 4, 8, 16, 3
+    Hq, lens = Hkv * G, [700, 33, 1500]
+    c = Cache(170, lens, Hkv, D, page, shared=32)
+    k, v, table = c.cuda()
+    N = 140000  # 4.6 GB each
+    kf, vf = (torch.empty(N, Hkv, page, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    far = torch.from_numpy(rng(171).permutation(N - 131100)[:c.pages].astype(np.int64) + 131100).cuda()
+    kf[far], vf[far] = k, v
+    tf = torch.where(table >= 0, far[table.clamp(min=0).long()].int(), table)
+    q = dev(rng(172).standard_normal((B, Hq * D)).astype(np.float16))
+    pos = dev(np.array(lens, np.int32) - 1)
+    assert torch.equal(hi.attn_paged(q, k, v, table, pos, Hq, Hkv), hi.attn_paged(q, kf, vf, tf, pos, Hq, Hkv))
+    q = dev(rng(173).standard_normal((60, Hq * D)).astype(np.float16))
+    start, at = dev(np.array([0, 20, 30, 60], np.int32)), dev(np.array(lens, np.int32) - np.array([20, 10, 30], np.int32))
+    assert torch.equal(hi.attn_paged(q, k, v, table, at, Hq, Hkv, start=start),
+                       hi.attn_paged(q, kf, vf, tf, at, Hq, Hkv, start=start))
+    big = 64  # enough rows for the prefix to be read once
+    tables = [t[2:3].repeat(big, 1).contiguous() for t in (table, tf)]
+    q = dev(rng(174).standard_normal((big, Hq * D)).astype(np.float16))
+    pos = torch.full((big,), 1499, dtype=torch.int32, device="cuda")
+    assert torch.equal(hi.attn_shared(q, k, v, tables[0], pos, 1488, Hq, Hkv), hi.attn_shared(q, kf, vf, tables[1], pos, 1488, Hq, Hkv))
+    qkv, cs, _ = rope_case(175, 5, 1, Hq, Hkv, D, D, page, 1600, False)
+    seq, pos = dev(np.array([2, 0, 2, 1, 2], np.int32)), dev(np.array([1499, 40, 3, 32, 700], np.int32))
+    for kk, vv, tt in ((k, v, table), (kf, vf, tf)):
+        hi.rope_cache_paged(dev(qkv), Hq, Hkv, dev(cs), kk, vv, tt, pos, seq=seq)
+    assert torch.equal(k.view(torch.int16), kf[far].view(torch.int16)) and torch.equal(v.view(torch.int16), vf[far].view(torch.int16))
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals(hi):
     D, Hq, Hkv, page, B = 128, 4, 2, 16, 3
