@@ -66,7 +66,8 @@ __global__ void __launch_bounds__(256) rope_paged_any_kernel(RopePagedArgs a, Pa
 
 // 16-byte accesses: a step turns 8 pairs (the 8 elements at d and the 8 at d + rot / 2, or 8 interleaved ones: 4 pairs) or
 // copies 8 elements; block per row, a thread per step up to 512. `per` steps a q or k head, `turns` of them rotate. The row is
-// requested before its place is known (position, table entry and cs row are a chain of three loads).
+// requested before its place is known (position, table entry and cs row are a chain of three loads). 2048 rows of 32/8 heads
+// of 128 10.2 us, 5.1 TB/s, what a large copy reaches (the kernel above 15.5); one row 2.3 us, the chain (5.2).
 template <typename CS, bool INTER>
 __global__ void __launch_bounds__(512) rope_paged_kernel(RopePagedArgs a, PagedCache c, int per, int turns) {
   constexpr int NP = INTER ? 4 : 8;  // pairs of a step
@@ -154,8 +155,11 @@ struct AttnArgs {
 //    the masked tile for all of its keys, and hides them there.
 // Where the row tiles are fewer than the GPU's CUs, their keys are split (paged_plan.h). A split stores its unnormalised O, m
 // and l in fp32, in the lanes' order; of each kFan splits of a tile the block that arrives last joins them, of each kFan such
-// groups the last again, until one block has the tile. Nobody waits. Against a launch of its own for the joins: 8 x 5 rows
-// after 700 to 4000 keys XXX us, 7 prompt chunks of 1 to 411 rows XXX.
+// groups the last again, until one block has the tile. Nobody waits. A launch of its own for the joins, us: 8 x 5 rows after
+// 700 to 4000 keys 23.3 (here 23.2), 7 prompt chunks of 1 to 411 rows 28.9 (here 26.3), and 3 more for every small batch.
+// What bounds it: 2048 rows after 4096 positions (32/8 heads of 128) 176 us, 975 TFLOP/s, as the slot cache's kernel; few rows:
+// their keys' bytes (8 x 5 rows: 10 of 23 us at 7 TB/s, partly from the last-level cache), and a chain of about 12 us around
+// them: start and pos, the plan, the table, the first K tile (2 to 3 us), the parts' stores, arrival and join (5 us).
 struct FlashPlan {
   float *ml, *po;  // partial results: [slot][2][BQ] m and l, O [slot][RG][D / 8][64][4], a prefix's [slot][BQ][D]
   int slots;       // slots there are, each of all kv heads
@@ -376,7 +380,7 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const PagedCache&
     int kn[NG], vn[NG];
     auto fetch = [&] { id = key < kv_end ? c.entry(tb, key >> c.shift) : -1; };
     auto take = [&] {
-      const bool ok = c.has(id);
+      const bool ok = c.has(id) && key < kv_end;
       const int64_t off = ok ? (id * c.stride + ((int64_t)hk * page + (key & (page - 1))) * D) * 2 : 0;
       const int n = ok ? min(8, kv_end - key) * D * 2 : 0;
 #pragma unroll
@@ -652,7 +656,9 @@ __device__ __forceinline__ void join_parts(float& M, float& L, f32x4& O, const f
 // one 64-bit address each for K and V per tile, from entries requested a tile ahead. What the slot kernel leaves to the
 // buffer bounds is done in registers, in a wave's last tile and in tiles with an entry that is no page only: logits of
 // keys that are not there become -inf, their V rows zeros.
-// OWN: the keys behind a shared prefix; every split leaves its part for attn_parts_kernel.
+// Measured: 64 sequences of 1000 keys, 32/8 heads of 128, 48.0 us (5.5 TB/s; slots 47.2), 48 of 100 to 2000 46.3 (4.5 TB/s;
+// slots 43.5), one of 4001 9.9 (slots 9.4: the table is one more load in the chain from the position to K).
+// OWN: the keys behind a shared prefix; a split leaves its part for join_block.
 struct StepPlan {
   int S, S1;      // splits of a pair: the launch's, and those that give every CU a block (splits_used)
   int K;          // > 0: a split per K keys instead

@@ -420,18 +420,15 @@ def flash_prefill_lse(q, kc, vc, T, p0, Hq, Hkv, out=None, lse=None):
 # ------------------------------------------------------------------ paged key/value cache
 # These wrappers are half of a small call's time, so their checks read each property once (60 to 90 ns each) and the common
 # case is one comparison; what fails is looked at again for the message.
-_F16, _F32, _I32 = torch.float16, torch.float32, torch.int32
+_F16, _F32, _I32, _U8 = torch.float16, torch.float32, torch.int32, torch.uint8
+_current_gpu = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _gpu(what, *tensors):
-    """The current device, on which every tensor (None aside) has to be: the library launches there."""
-    gpu = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != gpu:
-            raise ValueError(f"hipinfer_amd.{what}: tensors on {tensors[0].device} and {t.device}")
-    if gpu < 0 or gpu != torch._C._cuda_getDevice():
-        raise ValueError(f"hipinfer_amd.{what}: tensors must live on the current GPU (got {tensors[0].device})")
-    return gpu
+def _elsewhere(what, *tensors):
+    """The error for tensors (None aside) that are not all on the current GPU, where the library launches."""
+    raise ValueError(f"hipinfer_amd.{what}: tensors must live on the current GPU, got "
+                     f"{sorted({str(t.device) for t in tensors if t is not None})}")
 
 
 def _paged(what, kp, vp, table, Hkv):
@@ -461,13 +458,12 @@ def _paged(what, kp, vp, table, Hkv):
 
 def _rows_of(what, name, t, M, width):
     """An fp16 [M, >= width] tensor of contiguous rows; returns its row stride (a single row's is its width)."""
-    shape = t.shape
+    shape, steps = t.shape, t.stride()
     if t.dtype is not _F16 or len(shape) != 2 or shape[0] != M or shape[1] < width:
         raise ValueError(f"hipinfer_amd.{what}: {name} must be fp16 [{M}, {width}], got {t.dtype} {tuple(shape)}")
-    step, one = t.stride()
-    if one != 1 and shape[1] > 1:
+    if steps[1] != 1 and shape[1] > 1:
         raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous")
-    return step if M > 1 else shape[1]
+    return steps[0] if M > 1 else shape[1]
 
 
 def _vector(what, name, t, n):
@@ -490,7 +486,11 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
     A row that has no place is left out, its q too: a negative position (padding), one behind its table row or cs,
     a seq outside the table, a page id outside [0, pages). Rows of one call must have places of their own."""
     what = "rope_cache_paged"
-    gpu = _gpu(what, qkv, cs, kp, vp, table, pos, seq, q_out)
+    gpu = qkv.get_device()
+    if not (gpu == kp.get_device() == vp.get_device() == table.get_device() == pos.get_device() == cs.get_device()) or \
+            (seq is not None and seq.get_device() != gpu) or (q_out is not None and q_out.get_device() != gpu) or \
+            gpu < 0 or gpu != _current_gpu():
+        _elsewhere(what, qkv, cs, kp, vp, table, pos, seq, q_out)
     cache, B, D = _paged(what, kp, vp, table, Hkv)
     M = qkv.shape[0]
     ldq = _rows_of(what, "qkv", qkv, M, (Hq + 2 * Hkv) * D)
@@ -508,23 +508,26 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
         ldo = _rows_of(what, "q_out", q_out, M, Hq * D)
     check_rc(lib.hi_rope_cache_paged(qkv.data_ptr(), ldq, q_out.data_ptr(), ldo, M, Hq, Hkv, D, cs.data_ptr(), cshape[0],
                                      wide, 2 * cshape[1], interleaved, _addr(seq), pos.data_ptr(), *cache, B,
-                                     torch._C._cuda_getCurrentRawStream(gpu)), what)
+                                     _raw_stream(gpu)), what)
 
 
-def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work):
+def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu):
     """Checks what attn_paged and attn_shared have in common; returns the cache's arguments, M, B, D, q's row stride, out
     and its row stride."""
     cache, B, D = _paged(what, kp, vp, table, Hkv)
-    M = q.shape[0]
-    ldq = _rows_of(what, "q", q, M, Hq * D)
+    M, width = q.shape[0], Hq * D
+    ldq = _rows_of(what, "q", q, M, width)
     _vector(what, "pos", pos, B)
     if out is None:
-        out = _alloc_rows(q, M, Hq * D)
-    ldo = _rows_of(what, "out", out, M, Hq * D)
-    if lse is not None and (lse.dtype is not _F32 or lse.shape != (Hq, M) or not lse.is_contiguous()):
-        raise ValueError(f"hipinfer_amd.{what}: lse must be packed fp32 [{Hq}, {M}]")
-    if work is not None and (work.dtype is not torch.uint8 or not work.is_contiguous()):
-        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8")
+        out, ldo = _alloc_rows(q, M, width), width
+    else:
+        ldo = _rows_of(what, "out", out, M, width)
+        if out.get_device() != gpu:
+            _elsewhere(what, q, out)
+    if lse is not None and (lse.dtype is not _F32 or lse.shape != (Hq, M) or not lse.is_contiguous() or lse.get_device() != gpu):
+        raise ValueError(f"hipinfer_amd.{what}: lse must be packed fp32 [{Hq}, {M}] on the current GPU")
+    if work is not None and (work.dtype is not _U8 or not work.is_contiguous() or work.get_device() != gpu):
+        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8 on the current GPU")
     return cache, M, B, D, ldq, out, ldo
 
 
@@ -556,16 +559,21 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     base-2 log-sum-exp of each row's scaled logits (-inf without keys). `work` (attn_paged_work) can be kept
     across calls; everything the call reads of pos, start and table is read on the device, so it can be captured."""
     what = "attn_paged"
-    gpu = _gpu(what, q, kp, vp, table, pos, start, out, lse, work)
-    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
+    gpu = q.get_device()
+    if not (gpu == kp.get_device() == vp.get_device() == table.get_device() == pos.get_device()) or gpu < 0 or \
+            gpu != _current_gpu():
+        _elsewhere(what, q, kp, vp, table, pos)
+    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu)
     if start is not None:
         _vector(what, "start", start, B + 1)
+        if start.get_device() != gpu:
+            _elsewhere(what, q, start)
     elif M != B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences (one row each without start)")
     if work is None:
         work = attn_paged_work(M, B, Hq, Hkv, D, start is not None)
     check_rc(lib.hi_attn_paged(q.data_ptr(), ldq, *cache, _addr(start), pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), M,
-                               B, Hq, Hkv, D, work.data_ptr(), work.numel(), torch._C._cuda_getCurrentRawStream(gpu)), what)
+                               B, Hq, Hkv, D, work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
     return out
 
 
@@ -580,14 +588,17 @@ def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work
     result as attn_paged where every row of table begins with those pages; a sequence may also be shorter than the
     shared part."""
     what = "attn_shared"
-    gpu = _gpu(what, q, kp, vp, table, pos, out, lse, work)
-    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work)
+    gpu = q.get_device()
+    if not (gpu == kp.get_device() == vp.get_device() == table.get_device() == pos.get_device()) or gpu < 0 or \
+            gpu != _current_gpu():
+        _elsewhere(what, q, kp, vp, table, pos)
+    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu)
     if M != B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences")
     if work is None:
         work = attn_shared_work(B, Hq, Hkv, D)
     check_rc(lib.hi_attn_shared(q.data_ptr(), ldq, *cache, shared, pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), B, Hq,
-                                Hkv, D, work.data_ptr(), work.numel(), torch._C._cuda_getCurrentRawStream(gpu)), what)
+                                Hkv, D, work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
     return out
 
 
