@@ -30,7 +30,7 @@ inline int paged_cache(const char* who, const void* kp, const void* vp, long lon
   if ((int64_t)Hkv * page * D * 2 > INT32_MAX) HI_FAIL("%s: a page of over 2 GiB", who);
   if (page_stride % 8 || (pages > 1 && page_stride < (int64_t)Hkv * page * D))
     HI_FAIL("%s: page stride %lld (a multiple of 8, at least Hkv * page * D)", who, page_stride);
-  if (!kp || !vp || !table || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)table & 3))
+  if (!kp || !vp || (!table && B > 0) || ((uintptr_t)kp & 15) || ((uintptr_t)vp & 15) || ((uintptr_t)table & 3))
     HI_FAIL("%s: kp and vp must be 16-byte aligned, table 4-byte aligned, none null", who);
   int shift = 0;
   while ((1 << shift) < page) shift++;

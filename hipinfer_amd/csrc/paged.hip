@@ -1389,10 +1389,11 @@ HI_EXPORT int hi_attn_paged(const void* q, int ldq, const void* kp, const void* 
   const char* who = "hi_attn_paged";
   PagedCache c;
   if (paged_cache(who, kp, vp, page_stride, pages, page, table, ldt, W, B, Hkv, D, c)) return -1;
+  if (B == 0 && (M == 0 || start)) return 0;  // rows of no sequence
   if (attn_check(who, q, ldq, pos, out, ldo, lse, M, Hq, Hkv, D)) return -1;
   if (!start && M != B) HI_FAIL("%s: %d rows for %d sequences (one each without start)", who, M, B);
   if ((uintptr_t)start & 3) HI_FAIL("%s: start must be 4-byte aligned", who);
-  if (M == 0 || B == 0) return 0;
+  if (M == 0) return 0;
   const size_t need = hi_attn_paged_work_bytes(M, B, Hq, Hkv, D, start != nullptr);
   if (!work || ((uintptr_t)work & 15) || work_bytes < need)
     HI_FAIL("%s: work of %zu bytes (at least %zu, 16-byte aligned)", who, work_bytes, need);
@@ -1415,10 +1416,10 @@ HI_EXPORT int hi_attn_shared(const void* q, int ldq, const void* kp, const void*
   const char* who = "hi_attn_shared";
   PagedCache c;
   if (paged_cache(who, kp, vp, page_stride, pages, page, table, ldt, W, B, Hkv, D, c)) return -1;
+  if (B == 0) return 0;
   if (attn_check(who, q, ldq, pos, out, ldo, lse, B, Hq, Hkv, D)) return -1;
   if (shared < 0 || shared % page || shared > (int64_t)W * page)
     HI_FAIL("%s: %d shared positions (whole pages of %d, at most the table's %d)", who, shared, page, W);
-  if (B == 0) return 0;
   const size_t need = hi_attn_shared_work_bytes(B, Hq, Hkv, D);
   if (!work || ((uintptr_t)work & 15) || work_bytes < need)
     HI_FAIL("%s: work of %zu bytes (at least %zu, 16-byte aligned)", who, work_bytes, need);

@@ -796,6 +796,13 @@ def test_refusals(hi):
     refused(R, qkv, Hq, Hkv, cs, k, v, table, pos, q_out=q[:2])
     refused(R, qkv, Hq, Hkv, cs, k, v, table, pos, seq=pos[:2])
     refused(R, qkv.float(), Hq, Hkv, cs, k, v, table, pos)
-    # no rows: nothing to do
+    # no rows, or no sequences: nothing to do
+    empty = dict(kp=k, vp=v, table=table[:0], pos=pos[:0], Hq=Hq, Hkv=Hkv)
+    assert A(torch.zeros(0, Hq * D, **half), **empty).shape == (0, Hq * D)
+    assert S(torch.zeros(0, Hq * D, **half), shared=16, **empty).shape == (0, Hq * D)
+    R(qkv[:0], Hq, Hkv, cs, k, v, table[:0], pos[:0])
+    kept = torch.full((3, Hq * D), 7.0, **half)
+    A(q, start=start[:1], out=kept, **empty)
+    assert (kept == 7).all()
     none = torch.zeros(0, Hq * D, **half)
     assert A(none, k, v, table, pos, Hq, Hkv, start=torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, Hq * D)
