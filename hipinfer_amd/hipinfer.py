@@ -555,9 +555,10 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     decrease). A row at position p sees keys 0 .. p, at most those its table row holds; keys whose page id lies outside
     [0, pages) are left out. A row that sees no key (pos -1: padding) gives zeros.
 
-    Returns out [M, Hq*D]; rows that belong to no sequence are left as they were. lse [Hq, M] fp32, if given, receives the
-    base-2 log-sum-exp of each row's scaled logits (-inf without keys). `work` (attn_paged_work) can be kept
-    across calls; everything the call reads of pos, start and table is read on the device, so it can be captured."""
+    Returns out [M, Hq*D], which may be q itself; rows that belong to no sequence are left as they were (in a new out, as
+    allocated). lse [Hq, M] fp32, if given, receives the base-2 log-sum-exp of each row's scaled logits (-inf without
+    keys). `work` (attn_paged_work) can be kept across calls; everything the call reads of pos, start and table is read on the
+    device, so it can be captured."""
     what = "attn_paged"
     gpu = q.get_device()
     if not (gpu == kp.get_device() == vp.get_device() == table.get_device() == pos.get_device()) or gpu < 0 or \
@@ -595,6 +596,8 @@ def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work
     cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu)
     if M != B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences")
+    if not 0 <= shared <= cache[4] * cache[7]:  # also what would wrap in a C int
+        raise ValueError(f"hipinfer_amd.{what}: {shared} shared positions, the table holds {cache[4] * cache[7]}")
     if work is None:
         work = attn_shared_work(B, Hq, Hkv, D)
     check_rc(lib.hi_attn_shared(q.data_ptr(), ldq, *cache, shared, pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), B, Hq,

@@ -743,6 +743,60 @@ def test_pages_behind_4_gib(hi):
     assert torch.equal(k.view(torch.int16), kf[far].view(torch.int16)) and torch.equal(v.view(torch.int16), vf[far].view(torch.int16))
 
 
+@pytest.mark.parametrize("form", ["decode", "ragged", "shared", "reread"])
+def test_out_in_place(hi, form):
+    """out = q, a slice of the QKV rows that rope_cache_paged rotated in place: the same bits as into new rows, and the rest
+    of the rows untouched."""
+    D, Hq, Hkv, page = 128, 8, 2, 16
+    rows = [3, 40, 1, 0, 17] if form == "ragged" else [1] * (40 if form == "shared" else 9)
+    B, M, shared = len(rows), sum(rows), {"shared": 4096, "reread": 64}.get(form, 0)
+    before = [shared + 37 * b for b in range(B)]
+    if form == "ragged":
+        before = [2500, 900, 5000, 10, 0]
+    c = Cache(190, [p + n for p, n in zip(before, rows)], Hkv, D, page, shared=shared)
+    for b in range(1, B):
+        c.table[b, :shared // page] = c.table[0, :shared // page]
+    k, v, table = c.cuda()
+    pos = dev(np.array(before, np.int32))
+    qkv = dev(rng(191).standard_normal((M, (Hq + 2 * Hkv) * D)).astype(np.float16))
+    q, kept = qkv[:, :Hq * D], qkv[:, Hq * D:].clone()
+    start = dev(np.cumsum([0] + rows).astype(np.int32))
+
+    def run(out):
+        if shared:
+            return hi.attn_shared(q, k, v, table, pos, shared, Hq, Hkv, out=out)
+        return hi.attn_paged(q, k, v, table, pos, Hq, Hkv, start=start if form == "ragged" else None, out=out)
+
+    want = run(None)
+    assert run(q) is q
+    assert torch.equal(q, want) and torch.equal(qkv[:, Hq * D:], kept)
+
+
+def test_two_streams(hi):
+    """Calls on two streams at once, a work buffer each: as one after the other."""
+    D, Hq, Hkv, page = 128, 32, 8, 16
+    lens = [4000, 700, 2500, 90]
+    c = Cache(195, lens, Hkv, D, page)
+    k, v, table = c.cuda()
+    pos, at = dev(np.array(lens, np.int32) - 1), dev(np.array(lens, np.int32) - 20)
+    start = dev(np.arange(0, 81, 20).astype(np.int32))
+    q1, q2 = (dev(rng(196 + i).standard_normal((n, Hq * D)).astype(np.float16)) for i, n in enumerate((4, 80)))
+    w1, w2 = hi.attn_paged_work(4, 4, Hq, Hkv, D), hi.attn_paged_work(80, 4, Hq, Hkv, D, ragged=True)
+    one = hi.attn_paged(q1, k, v, table, pos, Hq, Hkv, work=w1)
+    two = hi.attn_paged(q2, k, v, table, at, Hq, Hkv, start=start, work=w2)
+    a, b = [torch.empty_like(one) for _ in range(20)], [torch.empty_like(two) for _ in range(20)]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for x, y in zip(a, b):
+        with torch.cuda.stream(s1):
+            hi.attn_paged(q1, k, v, table, pos, Hq, Hkv, out=x, work=w1)
+        with torch.cuda.stream(s2):
+            hi.attn_paged(q2, k, v, table, at, Hq, Hkv, start=start, out=y, work=w2)
+    torch.cuda.synchronize()
+    for x, y in zip(a, b):
+        assert torch.equal(x, one) and torch.equal(y, two)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals(hi):
     D, Hq, Hkv, page, B = 128, 4, 2, 16, 3
@@ -806,3 +860,14 @@ def test_refusals(hi):
     assert (kept == 7).all()
     none = torch.zeros(0, Hq * D, **half)
     assert A(none, k, v, table, pos, Hq, Hkv, start=torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, Hq * D)
+
+
+def test_refused_shared_beyond_32_bits(hi):
+    """A `shared` that a C int would take for another number."""
+    D, Hq, Hkv, page = 128, 4, 2, 16
+    c = Cache(180, [40, 40], Hkv, D, page)
+    k, v, table = c.cuda()
+    q, pos = torch.zeros(2, Hq * D, dtype=torch.float16, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for shared in (2**32, 2**32 + 16, -2**32):
+        with pytest.raises(ValueError):
+            hi.attn_shared(q, k, v, table, pos, shared, Hq, Hkv)
