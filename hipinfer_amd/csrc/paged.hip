@@ -155,15 +155,16 @@ struct AttnArgs {
 //    the masked tile for all of its keys, and hides them there.
 // Where the row tiles are fewer than the GPU's CUs, their keys are split (paged_plan.h). A split stores its unnormalised O, m
 // and l in fp32, in the lanes' order; of each kFan splits of a tile the block that arrives last joins them, of each kFan such
-// groups the last again, until one block has the tile. Nobody waits. A launch of its own for the joins, us: 8 x 5 rows after
-// 700 to 4000 keys 23.3 (here 23.2), 7 prompt chunks of 1 to 411 rows 28.9 (here 26.3), and 3 more for every small batch.
-// What bounds it: 2048 rows after 4096 positions (32/8 heads of 128) 176 us, 975 TFLOP/s, as the slot cache's kernel; few rows:
-// their keys' bytes (8 x 5 rows: 10 of 23 us at 7 TB/s, partly from the last-level cache), and a chain of about 12 us around
-// them: start and pos, the plan, the table, the first K tile (2 to 3 us), the parts' stores, arrival and join (5 us).
+// groups the last again, until one block has the tile. Nobody waits. A launch of its own for the joins, us: 7 prompt
+// chunks of 1 to 411 rows 28.9 (here 26.3), and 3 more for every small batch.
+// What bounds it: 2048 rows after 4096 positions (32/8 heads of 128) 176 us, 975 TFLOP/s, as the slot cache's kernel; smaller
+// batches a chain of about 12 us around their tiles: start and pos, the plan, the table, the first K tile (2 to 3 us), the
+// parts' stores, arrival and join (5 us). Few rows: attn_rows_kernel.
 struct FlashPlan {
   float *ml, *po;  // partial results: [slot][2][BQ] m and l, O [slot][RG][D / 8][64][4], a prefix's [slot][BQ][D]
   int slots;       // slots there are, each of all kv heads
   int cus, b1, b2; // > 0: split over that many; plan_budget's quotients
+  int least, fan;  // key tiles that a split has at least, splits that a tile has at most (0: any)
   int splits;      // of the shared prefix
   int* counters;   // [slots * Hkv], arrivals of a tile's splits
 };
@@ -235,7 +236,9 @@ __device__ __forceinline__ bool flash_unit(const AttnArgs& a, int cap, const Fla
     const int budget = plan_budget(T, a.Hkv, f.cus, f.b1, f.b2);
     if (budget > 0) {
       longest = wave_most(longest);
-      for (L = plan_length((uint32_t)wave_total((int)work), budget); L < longest; L = plan_longer(L)) {
+      L = plan_length((uint32_t)wave_total((int)work), budget, f.least);
+      if (f.fan > 0) L = max(L, plan_div(longest + f.fan - 1, f.fan));
+      for (; L < longest; L = plan_longer(L)) {
         int units = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
           const Seq s = b0 ? seq(b0 + lane) : first;
@@ -961,6 +964,344 @@ __global__ void __launch_bounds__(NWV * 64, 3) attn_step_kernel(AttnArgs a, Page
   step_block<GC, D, NWV, false>(a, c, f, sh, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
+// ---- few rows
+//
+// Runs of a few rows (decoding sequences, drafted tokens to verify, short chunks; row_columns): the step's products with packed
+// rows (token, head of the group) as columns, NC blocks of 16, so that K and V fragments feed NC products each. The keys
+// behind a row are hidden in the tiles that hold them, and infinities and NaN among their V rows go to the rows that see them
+// as in flash_tile.h. Block = (row tile, kv head, split); of a tile's splits the block that arrives last joins all. Two
+// blocks of 8 waves would not fit a CU's registers: there is a unit for every CU, by the plan of all lengths; many tiles
+// have blocks of 4 waves and a step's splits, which need no plan.
+// What bounds it: small batches the chain of a step (one row after 4000 11.9 us, a plan's 1 to 2 more than attn_step_kernel);
+// 48 rows after 100 to 2000 45.5 us, 4.6 TB/s; 8 x 5 rows after 700 to 4000 21.1, 3.7 TB/s, its 256 blocks' first tiles
+// (4 us) and the joins (4 us) around 12 us of keys.
+template <int D, int NC, int NWV>
+struct RowsSmem {
+  float wo[NWV][16 * NC][D + 4];  // (+ 4: the 16 columns' stores on distinct banks)
+  float wm[NWV][16 * NC], wl[NWV][16 * NC];
+  int is_last;
+};
+
+// Unit `at` of the batch's row tiles, each of them as many units as its sequence's keys have splits: blocks without work come
+// last, where they keep no other from a CU. u.slot is the tile's number. False if there are not so many.
+template <int COLS>
+__device__ __forceinline__ bool rows_unit(const AttnArgs& a, int cap, const StepPlan& f, int at, int lane, FlashUnit& u) {
+  int before = 0, slot = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    int row0 = 0, rows = 0, pos = 0;
+    if (b < a.B) {
+      const int s0 = a.start[b], s1 = a.start[b + 1];
+      pos = a.pos[b];
+      row0 = plan_first(s0, a.M);
+      rows = plan_rows(s0, s1, a.M);
+    }
+    const int tiles = plan_tiles(rows, a.G, COLS), splits = step_used(f, plan_end(pos, rows, cap)), n = tiles * splits;
+    const int upto = wave_scan(n, lane), slots = wave_scan(tiles, lane);
+    const uint64_t hit = __ballot(before + upto > at);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      auto take = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      const int i = at - before - (take(upto) - take(n));
+      u = FlashUnit{b0 + l, take(row0), take(rows), take(pos), 0, take(splits), 0, 0};
+      u.tile = u.splits == 1 ? i : plan_div(i, u.splits);
+      u.split = i - u.tile * u.splits;
+      u.slot = slot + take(slots) - take(tiles) + u.tile;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+    slot += __builtin_amdgcn_readlane(slots, 63);
+  }
+  return false;
+}
+
+template <int D, int NC, int NWV>
+__global__ void __launch_bounds__(NWV * 64, NC == 1 ? 3 : 2) attn_rows_kernel(AttnArgs a, PagedCache c, StepPlan f, FlashPlan fp, int tiles) {
+  constexpr int KS = D / 32;               // k steps of a logits product
+  constexpr int DL = D / 16;               // V dims (and P.V products) per lane
+  constexpr int BK = NWV * kDaTile;        // keys per block pass
+  constexpr int NT = NWV * 64, COLS = 16 * NC, D4 = D / 4;
+  typedef typename std::conditional<DL == 8, u32x4, u32x2>::type VT;
+  extern __shared__ u32x4 fp_smem[];
+  auto& sh = *reinterpret_cast<RowsSmem<D, NC, NWV>*>(fp_smem);
+  const int G = a.G, page = 1 << c.shift, cap = c.capacity();
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int hk = blockIdx.x;
+  FlashUnit u;
+  int counter;
+  if constexpr (NWV == 8) {
+    if (!flash_unit<COLS>(a, cap, fp, blockIdx.y, lane, u)) return;
+    if (u.splits > 1 && u.slot + u.split >= fp.slots) return;  // (not reached: the plan stays within the slots)
+    counter = u.slot;
+  } else {
+    if (!rows_unit<COLS>(a, cap, f, blockIdx.y, lane, u)) return;
+    // (a start that decreases may have more tiles, or units, than there are: such tiles are left out whole)
+    if (u.slot >= tiles || (int)blockIdx.y - u.split + u.splits > (int)gridDim.y) return;
+    counter = u.slot;
+    u.slot *= f.S;
+  }
+  const int len = plan_tile_end(u.pos, u.n, u.tile, G, a.magic, COLS, cap);
+  const int S_eff = u.splits, split = u.split;
+  const int chunk = ((len < kPlanDiv ? plan_div(len + S_eff - 1, S_eff) : (len + S_eff - 1) / S_eff) + 7) & ~7;
+  const int start = split * chunk, end = min(len, start + chunk);
+  const int first = u.tile * COLS, cols = min(COLS, u.n * G - first);  // packed rows of the tile
+
+  const int r = lane & 15, fk = lane >> 4;
+  const int kg = 8 * (r >> 2), vg = 8 * fk;  // the lane's key groups in a tile (step_block)
+  const f16* const kl = c.kp + ((int64_t)hk * page + (r & 3)) * D + 8 * fk;
+  const f16* const vl = c.vp + (int64_t)hk * page * D + DL * r;
+  auto entry = [&](int key) { return key < end ? c.entry(u.b, key >> c.shift) : -1; };
+  auto place = [&](int id, int key) { return c.has(id) ? id * c.stride + (int64_t)(key & (page - 1)) * D : (int64_t)0; };
+  // the last key that the lane's columns see (-1 without a row), and the keys that every row of the tile sees
+  int qpos[NC];
+  const f16* qg[NC];
+#pragma unroll
+  for (int x = 0; x < NC; x++) {
+    const int pr = first + 16 * x + r, token = plan_token(min(pr, first + cols - 1), a.magic);
+    qpos[x] = 16 * x + r < cols ? (int)min((int64_t)u.pos + token, (int64_t)cap - 1) : -1;
+    qg[x] = a.q + (int64_t)(u.row0 + token) * a.ldq + (hk * G + min(pr, first + cols - 1) - token * G) * D + 8 * fk;
+  }
+  const int common = min(end, plan_end(u.pos, plan_token(first, a.magic) + 1, cap));
+  u32x4 kf[2][KS];
+  VT vf[8];
+  auto load_k = [&](int64_t at) {
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int s = 0; s < KS; s++) kf[x][s] = *reinterpret_cast<const u32x4*>(kl + at + 4 * x * D + 32 * s);
+  };
+  auto load_v = [&](int64_t at) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) vf[i] = *reinterpret_cast<const VT*>(vl + at + i * D);
+  };
+  const int t_first = start + wave * kDaTile;
+  float m[NC], l[NC];  // of the lane's columns; l over this lane's keys only
+  f32x4 o[NC][DL];     // O^T: dim DL (4 fk + i) + n of column 16 x + r in o[x][n][i]
+#pragma unroll
+  for (int x = 0; x < NC; x++) {
+    m[x] = -__builtin_huge_valf();
+    l[x] = 0.f;
+#pragma unroll
+    for (int n = 0; n < DL; n++) o[x][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (t_first < end) {
+    int kid = entry(t_first + kg), vid = entry(t_first + vg);
+    bool there = c.has(vid);  // this lane's V group of the tile lies on a page
+    bool whole = __all(there) && t_first + kDaTile <= common;
+    int64_t va = place(vid, t_first + vg);
+    load_k(place(kid, t_first + kg));
+    __builtin_amdgcn_sched_barrier(0);
+    u32x4 qf[NC][KS];
+#pragma unroll
+    for (int x = 0; x < NC; x++)
+#pragma unroll
+      for (int s = 0; s < KS; s++) qf[x][s] = *reinterpret_cast<const u32x4*>(qg[x] + 32 * s);
+    load_v(va);
+    kid = entry(t_first + BK + kg);
+    vid = entry(t_first + BK + vg);
+    int odd_tile = INT32_MAX;  // the first masked tile with infinities or NaN in V
+    auto tile = [&](int t0, auto maskc, auto lastc) {
+      constexpr bool MASK = decltype(maskc)::value, LAST = decltype(lastc)::value;
+      f32x4 sc[NC][2];
+#pragma unroll
+      for (int x = 0; x < NC; x++)
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          sc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < KS; s++)
+            sc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[y][s]),
+                                                              __builtin_bit_cast(f16x8, qf[x][s]), sc[x][y], 0, 0, 0);
+        }
+      const bool was = there;
+      if constexpr (!LAST) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(place(kid, t0 + BK + kg));
+        there = c.has(vid);
+        whole = __all(there) && t0 + BK + kDaTile <= common;
+        va = place(vid, t0 + BK + vg);
+        kid = entry(t0 + 2 * BK + kg);
+        vid = entry(t0 + 2 * BK + vg);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      f16x8 ph[NC];
+#pragma unroll
+      for (int x = 0; x < NC; x++) {
+        float p[8];
+        float mx = -__builtin_huge_valf();
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          p[k] = sc[x][k >> 2][k & 3] * a.scale_log2;
+          if (MASK && !(was && t0 + vg + k < end && t0 + vg + k <= qpos[x])) p[k] = -__builtin_huge_valf();
+          mx = fmaxf(mx, p[k]);
+        }
+        const float m_old = m[x];
+        m[x] = fmaxf(m[x], rows_reduce<true>(mx));
+        const float mn = m[x] == -__builtin_huge_valf() ? 0.f : m[x];  // no key seen: all weights are 0
+        const float alpha = __builtin_amdgcn_exp2f(m_old - mn);
+        float ps = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          p[k] = __builtin_amdgcn_exp2f(p[k] - mn);
+          ps += p[k];
+          ph[x][k] = (f16)p[k];
+        }
+        l[x] = __builtin_fmaf(l[x], alpha, ps);
+#pragma unroll
+        for (int n = 0; n < DL; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[x][n][i] *= alpha;
+      }
+      if constexpr (MASK) {
+        // rows behind the end are zeros; infinities and NaN, which a row that does not see their key would turn to
+        // NaN, are taken out and given to the rows that see them after the loop
+        uint32_t odd = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          if (!(was && t0 + vg + k < end)) vf[k] = VT{};
+#pragma unroll
+          for (int i = 0; i < DL / 2; i++) odd |= (vf[k][i] & 0x7fff7fffu) + 0x04000400u;  // an exponent of ones carries
+        }
+        if (__any((odd & 0x80008000u) != 0)) {
+          odd_tile = min(odd_tile, t0);
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+#pragma unroll
+            for (int i = 0; i < DL / 2; i++) {
+              if ((vf[k][i] & 0x7c00u) == 0x7c00u) vf[k][i] &= 0xffff0000u;
+              if ((vf[k][i] & 0x7c000000u) == 0x7c000000u) vf[k][i] &= 0x0000ffffu;
+            }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < DL; n++) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          w[k] = __builtin_amdgcn_perm(vf[2 * k + 1][n >> 1], vf[2 * k][n >> 1], n & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int x = 0; x < NC; x++)
+          o[x][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), ph[x], o[x][n], 0, 0, 0);
+      }
+      if constexpr (!LAST) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(va);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    int t0 = t_first;
+    for (; t0 + BK < end; t0 += BK) {
+      if (whole) tile(t0, no, no);
+      else tile(t0, yes, no);
+    }
+    tile(t0, yes, yes);
+#pragma unroll 1
+    for (int t = odd_tile; t < end; t += BK)
+#pragma unroll 1
+      for (int k = t; k < min(t + kDaTile, end); k++) {
+        const int id = c.entry(u.b, k >> c.shift);
+        if (!c.has(id)) continue;
+        const f16* vrow = c.vp + id * c.stride + ((int64_t)hk * page + (k & (page - 1))) * D + 4 * DL * fk;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int n = 0; n < DL; n++) {
+            const float v = (float)vrow[DL * i + n];
+            if (!(__builtin_fabsf(v) < __builtin_huge_valf()))
+#pragma unroll
+              for (int x = 0; x < NC; x++)
+                if (k <= qpos[x]) o[x][n][i] += v;
+          }
+      }
+  }
+
+  // ---- merge the block's waves (a wave without keys has m = -inf and weight 0)
+#pragma unroll
+  for (int x = 0; x < NC; x++) {
+    l[x] = rows_reduce<false>(l[x]);
+    if (16 * x + r >= cols) continue;
+    if (fk == 0) {
+      sh.wm[wave][16 * x + r] = m[x];
+      sh.wl[wave][16 * x + r] = l[x];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int n = 0; n < DL; n += 4)
+        *reinterpret_cast<f32x4*>(&sh.wo[wave][16 * x + r][DL * (4 * fk + i) + n]) =
+            f32x4{o[x][n][i], o[x][n + 1][i], o[x][n + 2][i], o[x][n + 3][i]};
+  }
+  __syncthreads();
+  auto store = [&](int col, int d, float M, float L, f32x4 O) {
+    const int token = plan_token(first + col, a.magic), h = hk * G + first + col - token * G;
+    f16x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = (f16)(L == 0.f ? 0.f : O[e] / L);
+    *reinterpret_cast<f16x4*>(a.out + (int64_t)(u.row0 + token) * a.ldo + h * D + d) = v;
+    if (a.lse && d == 0) a.lse[(int64_t)h * a.M + u.row0 + token] = M + log2f(L);
+  };
+  const bool single = S_eff == 1;
+  const int64_t part0 = (int64_t)u.slot * a.Hkv + hk;  // split 0's part; the others follow Hkv parts apart
+  const PartBuffer po(f.po, (size_t)(NWV == 8 ? fp.slots : tiles * f.S) * a.Hkv * COLS * D * 4);
+  for (int i = tid; i < cols * D4; i += NT) {
+    const int col = i / D4, d = 4 * (i % D4);
+    float M = -__builtin_huge_valf(), L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    float ms[NWV], ls[NWV];
+    f32x4 os[NWV];
+#pragma unroll
+    for (int w = 0; w < NWV; w++) {
+      ms[w] = sh.wm[w][col];
+      ls[w] = sh.wl[w][col];
+      os[w] = *reinterpret_cast<const f32x4*>(&sh.wo[w][col][d]);
+    }
+    join_parts(M, L, O, ms, ls, os, NWV);
+    if (single) {
+      store(col, d, M, L, O);
+    } else {
+      const int64_t part = part0 + (int64_t)split * a.Hkv;
+      po.store(part * (COLS * D4) + i, O);
+      if (d == 0) {
+        st_coherent(f.ml + part * 2 * COLS + col, M);
+        st_coherent(f.ml + part * 2 * COLS + COLS + col, L);
+      }
+    }
+  }
+  if (single) return;
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this thread's partial stores are complete
+  __syncthreads();
+  if (tid == 0) {
+    int* ctr = f.counters + counter * a.Hkv + hk;
+    sh.is_last = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == S_eff - 1;
+    if (sh.is_last) __hip_atomic_store(ctr, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next launch
+  }
+  __syncthreads();
+  if (!sh.is_last) return;
+  // ---- the last block joins the splits, in their order, 8 requested at once
+  for (int i = tid; i < cols * D4; i += NT) {
+    const int col = i / D4, d = 4 * (i % D4);
+    float M = -__builtin_huge_valf(), L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int s0 = 0; s0 < S_eff; s0 += 8) {
+      float ms[8], ls[8];
+      f32x4 os[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const int64_t part = part0 + (int64_t)min(s0 + k, S_eff - 1) * a.Hkv;
+        ms[k] = ld_coherent(f.ml + part * 2 * COLS + col);
+        ls[k] = ld_coherent(f.ml + part * 2 * COLS + COLS + col);
+        os[k] = po.load(part * (COLS * D4) + i);
+      }
+      join_parts(M, L, O, ms, ls, os, S_eff - s0);
+    }
+    store(col, d, M, L, O);
+  }
+}
+
 // ---- a shared prefix
 //
 // Its parts (pages_block) and the sequences' own keys (step_block) are computed apart and joined. Where the prefix leaves half
@@ -1162,6 +1503,39 @@ void step_splits(int B, int Hkv, int G, int cus, StepPlan& f, bool& wide) {
 size_t step_ml(const StepPlan& f, int B, int Hq) { return ((size_t)B * Hq * f.S * 2 + 3) & ~(size_t)3; }
 size_t step_bytes(const StepPlan& f, int B, int Hq, int D) { return (step_ml(f, B, Hq) + (size_t)B * Hq * f.S * D) * 4; }
 
+constexpr int kRowsMinSplit = 1;  // key tiles
+constexpr int kRowsFan = 32;      // the block that arrives last joins all splits of a tile
+
+// Column blocks of 16 packed rows of the kernel for few rows, or 0: the row tiles of pages_block. It has no stages to fill and
+// one level of joins, but reads a run's keys once per 32 packed rows instead of 64 or 128. So it takes
+//  * batches of a tile per sequence (on average, with no run of more than 384 packed rows while every sequence has a row):
+//    pages / rows, us, 32/8 heads of 128: 1 row after 4000 18.0 / 11.9, 48 after 100 to 2000 57.4 / 45.5, 8 x 5 rows after 700
+//    to 4000 23.4 / 21.1, 64 x 2 after 1000 60.1 / 49.7, 63 after 1000 and 65 after 16000 245 / 156, 31 after 500 and 97 (388
+//    packed) after 8000 59.0 / 89.6;
+//  * and where the tiles are at most half as many as CUs and can read 1536 keys for each CU in all, going by the table's
+//    width: 32 rows after 1000 21.3 / 14.0, after 8000 30.4 / 22.9, 100 after 4000 27.3 / 32.4, 64 after 16000 40.6 / 53.2,
+//    32 after 32000 48.5 / 60.5; 12/2 heads of 128, 19 after 1881 22.7 / 14.5, 250 after 1000 22.8 / 18.1.
+int row_columns(int M, int B, int G, int Hkv, int64_t cap, int cus) {
+  const int tiles = plan_tiles(M, G, 32);
+  const bool one = (int64_t)M * G <= 32 * (int64_t)B && (int64_t)(M - min(B, M) + 1) * G <= 384;
+  const bool few = 2 * (int64_t)max(min(B, M), tiles) * Hkv <= cus && tiles * Hkv * cap <= 1536 * (int64_t)cus;
+  return !one && !few ? 0 : (int64_t)M * G <= 16 * (int64_t)B ? 1 : 2;
+}
+// Its row tiles (at most), and how they are split. Up to a tile for every second CU, blocks of 8 waves and flash_unit's plan
+// (slots > 0), which knows all lengths; beyond, blocks of 4 waves and a step's splits.
+int64_t rows_plan(int M, int B, int G, int Hkv, int NC, int cus, StepPlan& f, int& slots) {
+  const int most = max(min(B, M), plan_tiles(M, G, 16 * NC));
+  const int64_t tiles = B == 1 ? most : (int64_t)M * G / (16 * NC) + min(B, M);
+  bool wide;
+  step_splits(most, Hkv, 16, cus, f, wide);  // (16 heads: never blocks of 8 waves)
+  if (tiles * Hkv > kCounters) f.S = 1;
+  slots = 2 * (int64_t)most * Hkv <= cus ? 2 * cus / Hkv : 0;
+  return tiles;
+}
+size_t rows_bytes(const StepPlan& f, int64_t tiles, int slots, int Hkv, int NC, int D) {
+  return (slots ? slots : f.S == 1 ? 0 : (size_t)tiles * f.S) * Hkv * 16 * NC * (D + 2) * 4;
+}
+
 // Splits of a prefix of `shared` positions for T row tiles, and whether the own keys go into the same launch (`mixed`): where
 // half of the CUs are through with the prefix in 12 key tiles, the other half takes the own keys; beyond that the prefix needs
 // all of them, and the own keys are faster in small blocks after it. Apart / mixed, us, 32/8 heads of 128: 32 sequences
@@ -1200,6 +1574,7 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
   if (slots) {
     f.slots = slots;
     f.cus = cus;
+    f.least = kPlanMinSplit;
     f.b1 = cus / a.Hkv;
     f.b2 = 2 * cus / a.Hkv;
     f.counters = (int*)work;
@@ -1216,6 +1591,36 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
   hipLaunchKernelGGL(kern, dim3(a.Hkv, (unsigned)units), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());
   return 0;
+}
+
+template <int D, int NC, int NWV>
+int rows_launch(const AttnArgs& a, const PagedCache& c, const StepPlan& f, const FlashPlan& fp, int64_t tiles, int64_t units,
+                hipStream_t s, const char* who) {
+  if (units > 65535 || (int64_t)a.B * plan_tiles(a.M, a.G, 16 * NC) * f.S > INT32_MAX)  // as flash_launch
+    HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
+  const auto kern = attn_rows_kernel<D, NC, NWV>;
+  const size_t lds = sizeof(RowsSmem<D, NC, NWV>);
+  if (const int rc = flash_fits(kern, NWV * 64, lds, who)) return rc;
+  hipLaunchKernelGGL(kern, dim3(a.Hkv, (unsigned)units), dim3(NWV * 64), lds, s, a, c, f, fp, (int)tiles);
+  HI_TRY(hipGetLastError());
+  return 0;
+}
+
+template <int D, int NC>
+int rows_run(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStream_t s, const char* who) {
+  StepPlan f;
+  FlashPlan fp{};
+  const int64_t tiles = rows_plan(a.M, a.B, a.G, a.Hkv, NC, cus, f, fp.slots);
+  f.counters = (int*)work;
+  f.ml = (float*)((char*)work + kWorkHead);
+  f.po = f.ml + (fp.slots ? fp.slots : (size_t)tiles * f.S) * a.Hkv * 2 * 16 * NC;
+  if (!fp.slots) return rows_launch<D, NC, 4>(a, c, f, fp, tiles, tiles * f.S, s, who);
+  fp.cus = cus;
+  fp.b1 = cus / a.Hkv;
+  fp.b2 = 2 * cus / a.Hkv;
+  fp.least = kRowsMinSplit;
+  fp.fan = kRowsFan;
+  return rows_launch<D, NC, 8>(a, c, f, fp, tiles, max(tiles, (int64_t)fp.slots), s, who);
 }
 
 template <int D>
@@ -1316,6 +1721,9 @@ int attn_check(const char* who, const void* q, int ldq, const int* pos, const vo
 int attn_run(const AttnArgs& a, const PagedCache& c, int D, int cus, void* work, hipStream_t s, const char* who) {
   const int G = a.G;
   if (a.start) {
+    const int NC = row_columns(a.M, a.B, G, a.Hkv, (int64_t)c.W << c.shift, cus);
+    if (NC == 1) return D == 64 ? rows_run<64, 1>(a, c, cus, work, s, who) : rows_run<128, 1>(a, c, cus, work, s, who);
+    if (NC == 2) return D == 64 ? rows_run<64, 2>(a, c, cus, work, s, who) : rows_run<128, 2>(a, c, cus, work, s, who);
     const bool small = flash_row_groups(a.M, a.B, G) == 2;
     return D == 64 ? (small ? flash_launch<64, 2>(a, c, cus, work, s, who) : flash_launch<64, 4>(a, c, cus, work, s, who))
                    : (small ? flash_launch<128, 2>(a, c, cus, work, s, who) : flash_launch<128, 4>(a, c, cus, work, s, who));
@@ -1374,8 +1782,15 @@ HI_EXPORT size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, 
   if (!d || !work_sizes(M, B, Hq, Hkv, D)) return 0;
   if (M == 0 || B == 0) return kWorkHead;
   if (ragged) {
-    const int RG = flash_row_groups(M, B, Hq / Hkv);
-    return kWorkHead + flash_bytes(M, Hq / Hkv, Hkv, RG, D, d->cus);
+    const int G = Hq / Hkv, NC = row_columns(M, B, G, Hkv, 1, d->cus);  // a wider table may take the other kernel
+    size_t rows = 0;
+    if (NC) {
+      StepPlan f;
+      int slots;
+      const int64_t tiles = rows_plan(M, B, G, Hkv, NC, d->cus, f, slots);
+      rows = rows_bytes(f, tiles, slots, Hkv, NC, D);
+    }
+    return kWorkHead + max(rows, flash_bytes(M, G, Hkv, flash_row_groups(M, B, G), D, d->cus));
   }
   StepPlan f;
   bool wide;

@@ -62,12 +62,12 @@ PLAN_HD int plan_budget(int T, int Hkv, int cus, int b1, int b2) {
 }
 // The first split length to try for `work` key tiles over all row tiles (a row tile counts its sequence's), and the next
 // longer one while the splits are more than the budget.
-PLAN_HD int plan_length(uint32_t work, int budget) {
+PLAN_HD int plan_length(uint32_t work, int budget, int least = kPlanMinSplit) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const int l = (int)((float)work * __builtin_amdgcn_rcpf((float)budget)) + 1;
 #else
   const int l = (int)((float)work / (float)budget) + 1;
 #endif
-  return l < kPlanMinSplit ? kPlanMinSplit : l;
+  return l < least ? least : l;
 }
 PLAN_HD int plan_longer(int L) { return L + L / 8 + 1; }

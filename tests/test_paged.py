@@ -304,6 +304,56 @@ def test_ragged(hi, D, G, Hkv, rows, before):
     compare_lse("ragged", L[:, pad:M + pad], want)
 
 
+FEW = [  # few rows a sequence: one or two blocks of 16 columns, one split and many, tiles that share a sequence
+    ([1], [650]), ([2], [4001]), ([1, 1, 2, 1, 3, 1], [5, 700, 33, 3000, 0, 64]), ([1] * 40, [37 * b for b in range(40)]),
+    ([4, 0, 1, 0, 3], [1030, 5, 9000, 0, 257]), ([8, 1, 1, 1, 1, 1, 1, 1], [123, 0, 1, 2, 31, 32, 33, 2000]),
+    ([2] * 90, [(61 * b) % 1500 for b in range(90)]), ([1] * 600, [b % 97 for b in range(600)]),
+]
+
+
+@pytest.mark.parametrize("D,G,Hkv", HEADS, ids=IDS)
+@pytest.mark.parametrize("rows,before", FEW, ids=[f"B{len(r)}-{sum(r)}rows" for r, _ in FEW])
+def test_few_rows(hi, D, G, Hkv, rows, before):
+    """Runs of few rows, with entries that are no page, unwritten rows behind the last key and a kept work buffer."""
+    page = [8, 16, 64][(D + G + len(rows)) % 3]
+    c = Cache(200 + G + len(rows), [p + n for p, n in zip(before, rows)], Hkv, D, page, layout=["joint", "strided", "packed"][G % 3])
+    for b in range(0, len(rows), 3):
+        if before[b] > 3 * page:
+            c.table[b, 1] = c.table[b, before[b] // page - 1] = [-1, 2**31 - 1, -2**31][b % 3]
+    M, Hq = sum(rows), Hkv * G
+    q = rng(201).standard_normal((M, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    start, pos = dev(np.cumsum([0] + rows).astype(np.int32)), dev(np.array(before, np.int32))
+    lse = torch.empty(Hq, M, device="cuda")
+    work = hi.attn_paged_work(M, len(rows), Hq, Hkv, D, ragged=True)
+    got = [host(hi.attn_paged(dev(q), k, v, table, pos, Hq, Hkv, start=start, lse=lse, work=work)) for _ in range(2)]
+    want = attend(c, [(b, p + t) for b, (p, n) in enumerate(zip(before, rows)) for t in range(n)], q, Hq)
+    compare("few rows", got[0], want)
+    compare_lse("few rows", host(lse), want)
+    assert np.array_equal(bits(got[0]), bits(got[1])), "a kept work buffer"
+    assert (host(work)[:hi.ATTN_COUNTER_BYTES] == 0).all()
+
+
+@pytest.mark.parametrize("D,G,Hkv", HEADS, ids=IDS)
+def test_few_rows_infinities(hi, D, G, Hkv):
+    """An infinite (and a NaN) V row at each of the positions of a run: only the rows from it on see it."""
+    page, B, n, p0 = 16, 40, 2, 611
+    for spot in (p0, p0 + 1, 300, 575, 576):
+        c = Cache(210 + spot, [p0 + n] * B, Hkv, D, page)
+        for b in range(B):
+            c.v[c.table[b, spot // page], :, spot % page] = [np.inf, -np.inf, np.nan][b % 3]
+        q = rng(211).standard_normal((B * n, Hkv * G * D)).astype(np.float16)
+        k, v, table = c.cuda()
+        start = dev(np.arange(0, B * n + 1, n).astype(np.int32))
+        got = host(hi.attn_paged(dev(q), k, v, table, dev(np.full(B, p0, np.int32)), Hkv * G, Hkv, start=start))
+        for t in range(n):
+            rows = np.arange(t, B * n, n)
+            if p0 + t >= spot:
+                assert (~np.isfinite(got[rows])).all(), "rows that see it"
+            else:
+                compare("rows before it", got[rows], attend(c, [(b, p0 + t) for b in range(B)], q[rows], Hkv * G))
+
+
 @pytest.mark.parametrize("T,p0,D,G,Hkv", [(700, 0, 64, 8, 4), (1000, 333, 128, 4, 8)])
 def test_ragged_one_chunk(hi, T, p0, D, G, Hkv):
     """A prompt chunk over pages is the chunk over a cache slot; the two kernels agree to both their tolerances."""
