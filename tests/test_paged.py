@@ -354,6 +354,31 @@ def test_few_rows_infinities(hi, D, G, Hkv):
                 compare("rows before it", got[rows], attend(c, [(b, p0 + t) for b in range(B)], q[rows], Hkv * G))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,before,Hkv,G", [
+    ([10] * 20, [(173 * b) % 2600 for b in range(20)], 8, 4),  # tiles of 64 packed rows, some split
+    ([16], [40000], 8, 4), ([16], [200001], 1, 4), ([100], [30000], 1, 8), ([40], [60000], 2, 6),  # levels of joins
+], ids=["B20", "16-Hkv8", "16-Hkv1", "100-Hkv1", "40-Hkv2"])
+def test_row_tiles(hi, D, rows, before, Hkv, G):
+    """Runs that are too many, or whose contexts are too long, for the kernel of few rows."""
+    page, Hq, M = 16, Hkv * G, sum(rows)
+    c = Cache(220 + M + D, [p + n for p, n in zip(before, rows)], Hkv, D, page)
+    c.table[-1, 1] = -1
+    q = rng(221).standard_normal((M, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    start, pos = dev(np.cumsum([0] + rows).astype(np.int32)), dev(np.array(before, np.int32))
+    lse = torch.empty(Hq, M, device="cuda")
+    work = hi.attn_paged_work(M, len(rows), Hq, Hkv, D, ragged=True)
+    got = [host(hi.attn_paged(dev(q), k, v, table, pos, Hq, Hkv, start=start, lse=lse, work=work)) for _ in range(2)]
+    at = [(b, p + t) for b, (p, n) in enumerate(zip(before, rows)) for t in range(n)]
+    some = list(range(0, M, 1 if M * max(before) < 10**6 else 13)) + [M - 1]
+    out, tol, want = attend(c, [at[m] for m in some], q[some], Hq)
+    compare("row tiles", got[0][some], (out, tol, want))
+    compare_lse("row tiles", host(lse)[:, some], (out, tol, want))
+    assert np.array_equal(bits(got[0]), bits(got[1])), "a kept work buffer"
+    assert (host(work)[:hi.ATTN_COUNTER_BYTES] == 0).all()
+
+
 @pytest.mark.parametrize("T,p0,D,G,Hkv", [(700, 0, 64, 8, 4), (1000, 333, 128, 4, 8)])
 def test_ragged_one_chunk(hi, T, p0, D, G, Hkv):
     """A prompt chunk over pages is the chunk over a cache slot; the two kernels agree to both their tolerances."""
