@@ -559,8 +559,9 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const PagedCache&
     __syncthreads();
     if (*flag == 0) return;
     const bool done = n <= kFan;
+    float m = -__builtin_huge_valf(), l = 0.f;
     if (part < P) {
-      float w[kFan], ls[kFan], m = -__builtin_huge_valf(), l = 0.f;
+      float w[kFan], ls[kFan];
 #pragma unroll
       for (int k = 0; k < kFan; k++) {
         const float* p = f.ml + (s0 + min(k, size - 1) * ds) * 2 * BQ + jr;
@@ -608,13 +609,16 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const PagedCache&
           }
         }
       }
-      if (part == 0 && fk == 0) {
-        if (!done) {
-          st_coherent(f.ml + s0 * 2 * BQ + jr, m);
-          st_coherent(f.ml + s0 * 2 * BQ + BQ + jr, l);
-        } else if (a.lse && jrow) {
-          a.lse[(int64_t)jh * a.M + u.row0 + jtoken] = m + log2f(l);
-        }
+    }
+    // every wave of a row group has read the first member's m and l before the joined ones take their place (O's chunks are
+    // each read and written by one wave)
+    if (!done) __syncthreads();
+    if (part == 0 && fk == 0) {
+      if (!done) {
+        st_coherent(f.ml + s0 * 2 * BQ + jr, m);
+        st_coherent(f.ml + s0 * 2 * BQ + BQ + jr, l);
+      } else if (a.lse && jrow) {
+        a.lse[(int64_t)jh * a.M + u.row0 + jtoken] = m + log2f(l);
       }
     }
     if (done) return;
