@@ -5,6 +5,7 @@
 #include "flash.h"
 #include "paged.h"
 #include "paged_plan.h"
+#include "row_overlap.h"
 
 namespace {
 
@@ -1719,6 +1720,8 @@ int attn_check(const char* who, const void* q, int ldq, const int* pos, const vo
     HI_FAIL("%s: q must be 16-byte aligned with ldq %% 8 == 0 and ldq >= Hq * D, pos 4-byte aligned, none null", who);
   if (((uintptr_t)out & 7) || ldo % 4 || ldo < Hq * D) HI_FAIL("%s: out must be 8-byte aligned, ldo %% 4 == 0, ldo >= Hq * D", who);
   if ((uintptr_t)lse & 3) HI_FAIL("%s: lse must be 4-byte aligned", who);
+  if (!in_place_or_apart(q, 2 * (int64_t)ldq, 2 * (int64_t)Hq * D, out, 2 * (int64_t)ldo, 2 * (int64_t)Hq * D, M))
+    HI_FAIL("%s: out must be q (with its row stride) or apart from it", who);
   return 0;
 }
 
@@ -1761,6 +1764,8 @@ HI_EXPORT int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int
   if (!qkv || !q_out || (rot && !cs) || !pos || ldq < (Hq + 2 * Hkv) * D || ldqo < Hq * D || ((uintptr_t)qkv & 1) ||
       ((uintptr_t)q_out & 1) || ((uintptr_t)cs & (cs_f32 ? 7 : 3)) || ((uintptr_t)pos & 3) || ((uintptr_t)seq & 3))
     HI_FAIL("%s: a null or misaligned pointer, ldq < (Hq + 2 Hkv) D or q_out's row stride < Hq D", who);
+  if (!in_place_or_apart(qkv, 2 * (int64_t)ldq, 2 * (int64_t)(Hq + 2 * Hkv) * D, q_out, 2 * (int64_t)ldqo, 2 * (int64_t)Hq * D, M))
+    HI_FAIL("%s: q_out must be qkv (with its row stride) or apart from it", who);
   if (!hi_device()) return -2;
   const RopePagedArgs a{(f16*)qkv, ldq, (f16*)q_out, ldqo, Hq, Hkv, D, rot, cs_rows, B, cs, seq, pos};
   const hipStream_t s = (hipStream_t)stream;

@@ -555,7 +555,7 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     decrease). A row at position p sees keys 0 .. p, at most those its table row holds; keys whose page id lies outside
     [0, pages) are left out. A row that sees no key (pos -1: padding) gives zeros.
 
-    Returns out [M, Hq*D], which may be q itself; rows that belong to no sequence are left as they were (in a new out, as
+    Returns out [M, Hq*D], which may be q itself, else shares no memory with it; rows that belong to no sequence are left as they were (in a new out, as
     allocated). lse [Hq, M] fp32, if given, receives the base-2 log-sum-exp of each row's scaled logits (-inf without
     keys). `work` (attn_paged_work) can be kept across calls; everything the call reads of pos, start and table is read on the
     device, so it can be captured."""

@@ -166,7 +166,8 @@ int hi_flash_prefill_lse(const void* q, int ldq, const void* kc, const void* vc,
  * page id outside [0, pages) is no page. kp, vp 16-byte aligned.
  *
  * Rotates and stores M rows qkv [M, ldq] = [q (Hq*D) | k (Hkv*D) | v (Hkv*D)], row m at position pos[m] of sequence
- * seq[m] (m when seq is NULL; then M <= B): q to q_out [M, ldqo] (qkv itself: in place), k to kp, v to vp. The first rot
+ * seq[m] (m when seq is NULL; then M <= B): q to q_out [M, ldqo] (qkv itself with ldqo == ldq: in place; else rows that
+ * meet qkv's are refused), k to kp, v to vp. The first rot
  * elements of a head are rotated in pairs (j, j + rot/2), or (2j, 2j + 1) when interleaved != 0, by cs [cs_rows][rot/2]
  * (cos, sin), fp32 when cs_f32 != 0, else fp16; one rounding per result. Rows without a place (pos < 0, behind the
  * table or cs, seq outside [0, B), no page) are left out entirely. */
@@ -181,7 +182,8 @@ size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged
 /* Causal attention over the paged cache: start NULL, row b of q [M, ldq] at position pos[b] of sequence b (M == B); else
  * rows start[b] .. start[b + 1] - 1 at positions pos[b], pos[b] + 1, ... of sequence b (start [B + 1], not
  * decreasing). A row at position p sees keys 0 .. p that its table row and the pages hold; a row without any gives 0 and
- * lse -inf. Rows of no sequence are left as they were. Hq / Hkv in 1..16, query head h reads kv head h / (Hq / Hkv). lse
+ * lse -inf. Rows of no sequence are left as they were. Hq / Hkv in 1..16, query head h reads kv head h / (Hq / Hkv). out
+ * [M, ldo] may be q itself with ldo == ldq; else rows that meet q's are refused. lse
  * [Hq][M] fp32 (base-2 log-sum-exp of the scaled logits) or NULL. work: work_bytes >= hi_attn_paged_work_bytes(...),
  * 16-byte aligned; launches that share it must not run concurrently. */
 int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,
