@@ -705,7 +705,7 @@ __device__ __forceinline__ void step_sum(const StepSmem<GC, D, NWV>& sh, int g, 
 
 // Splits that a run of len keys is cut into.
 __device__ __forceinline__ int step_used(const StepPlan& f, int len) {
-  return f.K > 0 ? max(1, min(f.S, plan_div(len + f.K - 1, f.K))) : splits_used(len, f.S, f.S1);
+  return f.K > 0 ? plan_step_splits(len, f.K, f.S) : splits_used(len, f.S, f.S1);
 }
 
 // One block: split `split` of sequence b and kv head hk. With `keep` a sequence's only part is left in the waves' LDS (step_sum).

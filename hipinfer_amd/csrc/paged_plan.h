@@ -1,5 +1,5 @@
-// How attention over ragged row runs is cut into blocks: row tiles, and splits of a tile's keys. Plain integer arithmetic of
-// one sequence at a time, used by the kernels (summed over a wave's lanes) and compiled for the host by its test.
+// How attention over ragged row runs is cut into blocks: row tiles, and splits of a tile's keys. Plain arithmetic of one
+// sequence at a time, used by the kernels (summed over a wave's lanes) and compiled for the host by its tests.
 #pragma once
 #include <cstdint>
 
@@ -7,6 +7,12 @@
 #define PLAN_HD __host__ __device__ __forceinline__
 #else
 #define PLAN_HD inline
+#endif
+// 1 / b in fp32, off by 2^-23 of it at most: the hardware's estimate, on the host the division (a test puts in its neighbours)
+#if defined(__HIP_DEVICE_COMPILE__)
+#define PLAN_RCP(b) __builtin_amdgcn_rcpf(b)
+#elif !defined(PLAN_RCP)
+#define PLAN_RCP(b) (1.0f / (b))
 #endif
 
 constexpr int kPlanTile = 128;          // keys of a tile: splits are whole tiles, and their lengths count them
@@ -17,12 +23,8 @@ constexpr int kPlanNoSplit = 1 << 24;   // more tiles than the 2^30 keys that a 
 // division is some 30 instructions, and a plan's are on the way of every block.
 constexpr int kPlanDiv = 1 << 22;  // an `a` that every b >= 1 is fine with
 PLAN_HD int plan_div(int a, int b) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b)), r = a - q * b;
+  const int q = (int)((float)a * PLAN_RCP((float)b)), r = a - q * b;
   return q + (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
-#else
-  return a / b;
-#endif
 }
 
 // Rows of a sequence: start values are cut to the M rows there are.
@@ -46,6 +48,10 @@ PLAN_HD int plan_tile_end(int pos, int n, int tile, int G, uint32_t magic, int B
   return plan_end(pos, plan_token(rows - 1, magic) + 1, cap);
 }
 PLAN_HD int plan_key_tiles(int end) { return (end + kPlanTile - 1) / kPlanTile; }
+// Splits of len keys, K of them each, at most S.
+PLAN_HD int plan_step_splits(int len, int K, int S) {
+  return len > (S - 1) * K ? S : len <= K ? 1 : plan_div(len + K - 1, K);
+}
 // Splits of a sequence with te key tiles.
 PLAN_HD int plan_splits(int te, int L) { return te <= L ? 1 : plan_div(te + L - 1, L); }
 // Keys [kb, ke) of split `split` of s of a row tile with `end` keys; the last ones can be empty.
@@ -63,11 +69,7 @@ PLAN_HD int plan_budget(int T, int Hkv, int cus, int b1, int b2) {
 // The first split length to try for `work` key tiles over all row tiles (a row tile counts its sequence's), and the next
 // longer one while the splits are more than the budget.
 PLAN_HD int plan_length(uint32_t work, int budget, int least = kPlanMinSplit) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const int l = (int)((float)work * __builtin_amdgcn_rcpf((float)budget)) + 1;
-#else
-  const int l = (int)((float)work / (float)budget) + 1;
-#endif
+  const int l = (int)((float)work * PLAN_RCP((float)budget)) + 1;
   return l < least ? least : l;
 }
 PLAN_HD int plan_longer(int L) { return L + L / 8 + 1; }
