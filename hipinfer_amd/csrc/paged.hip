@@ -1,6 +1,8 @@
 // Serving from a paged key/value cache: rotation and cache write of projected rows (hi_rope_cache_paged), attention over
 // the pages (hi_attn_paged) and attention of a batch whose sequences share their first positions (hi_attn_shared).
 // The cache and its table: paged.h.
+#include <algorithm>
+
 #include "decode_split.h"
 #include "flash.h"
 #include "paged.h"
@@ -1500,7 +1502,7 @@ void step_splits(int B, int Hkv, int G, int cus, StepPlan& f, bool& wide) {
     return;
   }
   f.S1 = 1;
-  f.S = pairs > kCounters ? 1 : (int)min((int64_t)8, 4 * kCounters / pairs);
+  f.S = pairs > kCounters ? 1 : (int)std::min((int64_t)8, 4 * kCounters / pairs);
   if (pairs < 2 * cus) f.S = max(f.S, decode_splits(B, Hkv, cus));
   f.K = 4 * pairs <= cus ? 256 : pairs <= cus ? 320 : pairs < 2 * cus ? 768 : 4096;
 }
@@ -1586,7 +1588,7 @@ int flash_launch(const AttnArgs& a, const PagedCache& c, int cus, void* work, hi
     f.ml = (float*)((char*)work + kWorkHead);
     f.po = f.ml + (size_t)slots * a.Hkv * 2 * 32 * RG;
   }
-  const int64_t units = max(flash_tiles(a.M, a.B, G, RG), (int64_t)slots);
+  const int64_t units = std::max(flash_tiles(a.M, a.B, G, RG), (int64_t)slots);
   // (the tiles of any start, also one that gives the same rows to every sequence, are counted in int)
   if (units > 65535 || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
     HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
@@ -1625,7 +1627,7 @@ int rows_run(const AttnArgs& a, const PagedCache& c, int cus, void* work, hipStr
   fp.b2 = 2 * cus / a.Hkv;
   fp.least = kRowsMinSplit;
   fp.fan = kRowsFan;
-  return rows_launch<D, NC, 8>(a, c, f, fp, tiles, max(tiles, (int64_t)fp.slots), s, who);
+  return rows_launch<D, NC, 8>(a, c, f, fp, tiles, std::max(tiles, (int64_t)fp.slots), s, who);
 }
 
 template <int D>
@@ -1670,7 +1672,8 @@ size_t shared_bytes(int B, int Hq, int Hkv, int D, int cus) {
   const int RG = flash_row_groups(B, 1, Hq / Hkv), T = plan_tiles(B, Hq / Hkv, 32 * RG);
   for (const bool mixed : {false, true}) {
     own_splits(B, Hkv, RG, cus, mixed, st);
-    most = max(most, step_bytes(st, B, Hq, D) + (size_t)T * max(1, cus / max(1, T * Hkv)) * Hkv * flash_slot_bytes(RG, D));
+    // (std::max: the host's plain max is one of ints)
+    most = std::max(most, step_bytes(st, B, Hq, D) + (size_t)T * max(1, cus / max(1, T * Hkv)) * Hkv * flash_slot_bytes(RG, D));
   }
   return most;
 }
@@ -1799,7 +1802,7 @@ HI_EXPORT size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, 
       const int64_t tiles = rows_plan(M, B, G, Hkv, NC, d->cus, f, slots);
       rows = rows_bytes(f, tiles, slots, Hkv, NC, D);
     }
-    return kWorkHead + max(rows, flash_bytes(M, G, Hkv, flash_row_groups(M, B, G), D, d->cus));
+    return kWorkHead + std::max(rows, flash_bytes(M, G, Hkv, flash_row_groups(M, B, G), D, d->cus));
   }
   StepPlan f;
   bool wide;

@@ -32,3 +32,11 @@ def test_joins_of_joined_parts(hi, D, Hkv, G, n, p0):  # noqa: F811
         again = hi.attn_paged(qd, k, v, table, pos, Hq, Hkv, start=start, work=work)
         assert torch.equal(again.view(torch.int16), first.view(torch.int16))
     assert (work[:hi.ATTN_COUNTER_BYTES] == 0).all()
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D", [(65535, 64, 8, 128), (65535, 32, 8, 128), (4096, 300, 300, 64), (30000, 48, 8, 128)])
+def test_work_beyond_2_gib(hi, B, Hq, Hkv, D):  # noqa: F811
+    """Own parts of every row and the prefix's parts, of at least a split each, have their place however many rows there are."""
+    part = 4 * (D + 2)
+    assert hi.lib.hi_attn_shared_work_bytes(B, Hq, Hkv, D) >= hi.ATTN_COUNTER_BYTES + 2 * B * Hq * part
+    assert hi.lib.hi_attn_paged_work_bytes(B, B, Hq, Hkv, D, 0) >= hi.ATTN_COUNTER_BYTES + B * Hq * part
