@@ -1746,6 +1746,55 @@ int attn_run(const AttnArgs& a, const PagedCache& c, int D, int cus, void* work,
   return D == 64 ? step_run<64>(a, c, cus, work, s, who) : step_run<128>(a, c, cus, work, s, who);
 }
 
+// What a call's parts need behind the counters. More rows or sequences may need less: the splits get fewer.
+size_t paged_bytes(int M, int B, int Hq, int Hkv, int D, bool ragged, int cus) {
+  StepPlan f;
+  if (!ragged) {
+    bool wide;
+    step_splits(B, Hkv, Hq / Hkv, cus, f, wide);
+    return step_bytes(f, B, Hq, D);
+  }
+  const int G = Hq / Hkv, NC = row_columns(M, B, G, Hkv, 1, cus);  // a wider table may take the other kernel
+  size_t rows = 0;
+  if (NC) {
+    int slots;
+    const int64_t tiles = rows_plan(M, B, G, Hkv, NC, cus, f, slots);
+    rows = rows_bytes(f, tiles, slots, Hkv, NC, D);
+  }
+  return std::max(rows, flash_bytes(M, G, Hkv, flash_row_groups(M, B, G), D, cus));
+}
+
+// What any call of at most M rows of at most B sequences needs; ragged: with start or without. Beyond kCounters pairs a step has one
+// split, its need grows with B. Row tiles need the same slots for any M that has some, of 4 row groups once a sequence can have over 64
+// packed rows; so do the few rows' blocks of 8 waves, smaller ones. Their blocks of 4 waves have splits while tiles * Hkv <=
+// kCounters: for every number of sequences with rows (more of them than rows are as many as rows) and NC, the most tiles of those.
+size_t paged_most_bytes(int M, int B, int Hq, int Hkv, int D, bool ragged, int cus) {
+  const int G = Hq / Hkv, few = kCounters / Hkv;
+  const int steps = ragged ? min(M, B) : B;  // a step has as many rows as sequences
+  size_t most = paged_bytes(steps, steps, Hq, Hkv, D, false, cus);
+  for (int b = 1; b <= min(steps, few); b++) most = std::max(most, paged_bytes(b, b, Hq, Hkv, D, false, cus));
+  if (!ragged) return most;
+  most = std::max(most, flash_bytes(1, G, Hkv, (int64_t)M * G > 64 ? 4 : 2, D, cus));
+  for (int b = 1; b <= min(steps, few); b++)
+    for (const int NC : {1, 2}) {
+      StepPlan f;
+      bool wide;
+      step_splits(b, Hkv, 16, cus, f, wide);  // as rows_plan
+      const int64_t rows = std::min((int64_t)M, 16 * NC * (int64_t)b / G);
+      const int64_t tiles = std::min(rows * G / (16 * NC) + b, (int64_t)few);
+      most = std::max(most, rows_bytes(f, tiles, 0, Hkv, NC, D));
+    }
+  return most;
+}
+
+size_t shared_most_bytes(int B, int Hq, int Hkv, int D, int cus) {
+  size_t most = shared_bytes(B, Hq, Hkv, D, cus);
+  // beyond both, one split: the need grows with B
+  const int64_t few = max(kCounters / Hkv, 128 * (cus / Hkv + 1) / (Hq / Hkv) + 1);
+  for (int b = 1; b <= std::min((int64_t)B, few); b++) most = std::max(most, shared_bytes(b, Hq, Hkv, D, cus));
+  return most;
+}
+
 // Sizes of a work buffer's call that the attention can take.
 bool work_sizes(int M, int B, int Hq, int Hkv, int D) {
   return M >= 0 && B >= 0 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 16 && (D == 64 || D == 128) &&
@@ -1792,22 +1841,13 @@ HI_EXPORT int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int
 HI_EXPORT size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged) {
   const HiDevice* d = hi_device();
   if (!d || !work_sizes(M, B, Hq, Hkv, D)) return 0;
-  if (M == 0 || B == 0) return kWorkHead;
-  if (ragged) {
-    const int G = Hq / Hkv, NC = row_columns(M, B, G, Hkv, 1, d->cus);  // a wider table may take the other kernel
-    size_t rows = 0;
-    if (NC) {
-      StepPlan f;
-      int slots;
-      const int64_t tiles = rows_plan(M, B, G, Hkv, NC, d->cus, f, slots);
-      rows = rows_bytes(f, tiles, slots, Hkv, NC, D);
-    }
-    return kWorkHead + std::max(rows, flash_bytes(M, G, Hkv, flash_row_groups(M, B, G), D, d->cus));
-  }
-  StepPlan f;
-  bool wide;
-  step_splits(B, Hkv, Hq / Hkv, d->cus, f, wide);
-  return kWorkHead + step_bytes(f, B, Hq, D);
+  return kWorkHead + (M == 0 || B == 0 ? 0 : paged_bytes(M, B, Hq, Hkv, D, ragged != 0, d->cus));
+}
+
+HI_EXPORT size_t hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ragged) {
+  const HiDevice* d = hi_device();
+  if (!d || !work_sizes(M, B, Hq, Hkv, D)) return 0;
+  return kWorkHead + (M == 0 || B == 0 ? 0 : paged_most_bytes(M, B, Hq, Hkv, D, ragged != 0, d->cus));
 }
 
 HI_EXPORT int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages,
@@ -1835,6 +1875,12 @@ HI_EXPORT size_t hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D) {
   const HiDevice* d = hi_device();
   if (!d || !work_sizes(B, B, Hq, Hkv, D)) return 0;
   return kWorkHead + (B == 0 ? 0 : shared_bytes(B, Hq, Hkv, D, d->cus));
+}
+
+HI_EXPORT size_t hi_attn_shared_work_bytes_max(int B, int Hq, int Hkv, int D) {
+  const HiDevice* d = hi_device();
+  if (!d || !work_sizes(B, B, Hq, Hkv, D)) return 0;
+  return kWorkHead + (B == 0 ? 0 : shared_most_bytes(B, Hq, Hkv, D, d->cus));
 }
 
 HI_EXPORT int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages,

@@ -86,10 +86,12 @@ int hi_rope_cache_paged(ptr qkv, int ldq, ptr q_out, int ldqo, int M, int Hq, in
                         int cs_f32, int rot, int interleaved, ptr seq, ptr pos, ptr kp, ptr vp, i64 page_stride,
                         int pages, int page, ptr table, int ldt, int W, int B, ptr stream);
 size hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged);
+size hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ragged);
 int hi_attn_paged(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
                   ptr start, ptr pos, ptr out, int ldo, ptr lse, int M, int B, int Hq, int Hkv, int D, ptr work,
                   size work_bytes, ptr stream);
 size hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D);
+size hi_attn_shared_work_bytes_max(int B, int Hq, int Hkv, int D);
 int hi_attn_shared(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
                    int shared, ptr pos, ptr out, int ldo, ptr lse, int B, int Hq, int Hkv, int D, ptr work,
                    size work_bytes, ptr stream);
@@ -541,9 +543,10 @@ def _attn_work(what, size):
 
 
 def attn_paged_work(rows, seqs, Hq, Hkv, D, ragged=False):
-    """A work buffer of attn_paged for `rows` rows of `seqs` sequences (ragged: with start). It serves any later call of
-    attn_paged or attn_shared that needs no more bytes; calls that use one buffer must not overlap in time."""
-    return _attn_work("attn_paged_work", lib.hi_attn_paged_work_bytes(rows, seqs, Hq, Hkv, D, int(ragged)))
+    """A work buffer of attn_paged for at most `rows` rows of at most `seqs` sequences (ragged: with start as well as
+    without). It serves any call of attn_paged or attn_shared that needs no more bytes; calls that use one buffer must not
+    overlap in time."""
+    return _attn_work("attn_paged_work", lib.hi_attn_paged_work_bytes_max(rows, seqs, Hq, Hkv, D, int(ragged)))
 
 
 def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, work=None):
@@ -572,15 +575,15 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     elif M != B:
         raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences (one row each without start)")
     if work is None:
-        work = attn_paged_work(M, B, Hq, Hkv, D, start is not None)
+        work = _attn_work(what, lib.hi_attn_paged_work_bytes(M, B, Hq, Hkv, D, int(start is not None)))
     check_rc(lib.hi_attn_paged(q.data_ptr(), ldq, *cache, _addr(start), pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), M,
                                B, Hq, Hkv, D, work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
     return out
 
 
 def attn_shared_work(seqs, Hq, Hkv, D):
-    """A work buffer of attn_shared for `seqs` sequences, as attn_paged_work's."""
-    return _attn_work("attn_shared_work", lib.hi_attn_shared_work_bytes(seqs, Hq, Hkv, D))
+    """A work buffer of attn_shared for at most `seqs` sequences, as attn_paged_work's."""
+    return _attn_work("attn_shared_work", lib.hi_attn_shared_work_bytes_max(seqs, Hq, Hkv, D))
 
 
 def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work=None):
@@ -599,7 +602,7 @@ def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work
     if not 0 <= shared <= cache[4] * cache[7]:  # also what would wrap in a C int
         raise ValueError(f"hipinfer_amd.{what}: {shared} shared positions, the table holds {cache[4] * cache[7]}")
     if work is None:
-        work = attn_shared_work(B, Hq, Hkv, D)
+        work = _attn_work(what, lib.hi_attn_shared_work_bytes(B, Hq, Hkv, D))
     check_rc(lib.hi_attn_shared(q.data_ptr(), ldq, *cache, shared, pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), B, Hq,
                                 Hkv, D, work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
     return out

@@ -179,6 +179,9 @@ int hi_rope_cache_paged(void* qkv, int ldq, void* q_out, int ldqo, int M, int Hq
  * 0 for bad sizes. Its first 16384 bytes are zeroed once by the caller and left zero by every call; one buffer serves
  * calls of hi_attn_paged and hi_attn_shared in turn, of any sizes that it is large enough for. */
 size_t hi_attn_paged_work_bytes(int M, int B, int Hq, int Hkv, int D, int ragged);
+/* Bytes enough for every call of at most M rows of at most B sequences (ragged: with start and without), which
+ * hi_attn_paged_work_bytes(M, B, ...) need not be: larger batches are split less and can need less. */
+size_t hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ragged);
 /* Causal attention over the paged cache: start NULL, row b of q [M, ldq] at position pos[b] of sequence b (M == B); else
  * rows start[b] .. start[b + 1] - 1 at positions pos[b], pos[b] + 1, ... of sequence b (start [B + 1], not
  * decreasing). A row at position p sees keys 0 .. p that its table row and the pages hold; a row without any gives 0 and
@@ -191,6 +194,7 @@ int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long l
                   int M, int B, int Hq, int Hkv, int D, void* work, size_t work_bytes, void* stream);
 /* The same for hi_attn_shared. */
 size_t hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D);
+size_t hi_attn_shared_work_bytes_max(int B, int Hq, int Hkv, int D);
 /* hi_attn_paged without start for B sequences whose first `shared` positions (a multiple of page) are one prefix, read
  * from table row 0's pages once for the batch; later positions are each sequence's own. */
 int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,

@@ -40,3 +40,59 @@ def test_work_beyond_2_gib(hi, B, Hq, Hkv, D):  # noqa: F811
     part = 4 * (D + 2)
     assert hi.lib.hi_attn_shared_work_bytes(B, Hq, Hkv, D) >= hi.ATTN_COUNTER_BYTES + 2 * B * Hq * part
     assert hi.lib.hi_attn_paged_work_bytes(B, B, Hq, Hkv, D, 0) >= hi.ATTN_COUNTER_BYTES + B * Hq * part
+
+
+SIZES = [(32, 8, 128), (12, 2, 128), (32, 4, 64), (16, 1, 128), (7, 7, 64), (80, 80, 64), (300, 300, 64)]  # Hq, Hkv, D
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", SIZES)
+def test_work_of_the_largest_batch(hi, Hq, Hkv, D):  # noqa: F811
+    """A buffer for the largest batch is large enough for every smaller one, of either form."""
+    r, need, shared = rng(310 + Hq), hi.lib.hi_attn_paged_work_bytes, hi.lib.hi_attn_shared_work_bytes
+    for top_rows, top_seqs in [(70, 40), (2048, 8), (2048, 256), (600, 600), (4096, 4096), (3, 900), (1, 1), (9000, 1)]:
+        most = hi.lib.hi_attn_paged_work_bytes_max(top_rows, top_seqs, Hq, Hkv, D, 1)
+        step = hi.lib.hi_attn_paged_work_bytes_max(top_seqs, top_seqs, Hq, Hkv, D, 0)
+        joint = hi.lib.hi_attn_shared_work_bytes_max(top_seqs, Hq, Hkv, D)
+        sizes = [(top_rows, top_seqs)] + [(int(r.integers(1, top_rows + 1)), int(r.integers(1, top_seqs + 1))) for _ in range(2000)]
+        sizes += [(m, b) for b in (1, 2, 3, top_seqs) for m in range(1, top_rows + 1)]
+        sizes += [(m, b) for b in range(1, top_seqs + 1) for m in (b, 2 * b, 16 * b * Hkv // Hq, 32 * b * Hkv // Hq) if 1 <= m <= top_rows]
+        for m, b in sizes:
+            if b <= top_seqs:
+                assert need(m, b, Hq, Hkv, D, 1) <= most, (m, b)
+        for b in range(1, top_seqs + 1):
+            assert need(b, b, Hq, Hkv, D, 0) <= step and shared(b, Hq, Hkv, D) <= joint, b
+            assert b > top_rows or need(b, b, Hq, Hkv, D, 0) <= most, b
+
+
+def test_one_work_buffer_for_smaller_batches(hi):  # noqa: F811
+    """A server's buffers, made once for its largest batch, in calls of fewer rows and sequences: taken, with the same bits as a
+    buffer of the call's own."""
+    def same(a, b):  # (rows behind the cached positions are NaN)
+        return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+    Hq, Hkv, D, page = 32, 8, 128, 16
+    lens = [int(n) for n in rng(320).integers(1, 900, 600)]
+    c = Cache(321, [900] * 24, Hkv, D, page)
+    k, v, rows = c.cuda()
+    table = rows[torch.arange(600, device="cuda") % 24].contiguous()
+    pos = dev(np.array(lens, np.int32) - 1)
+    q = dev(rng(322).standard_normal((2048, Hq * D)).astype(np.float16))
+    works = {"ragged": hi.attn_paged_work(2048, 600, Hq, Hkv, D, ragged=True), "step": hi.attn_paged_work(600, 600, Hq, Hkv, D),
+             "shared": hi.attn_shared_work(600, Hq, Hkv, D)}
+    for B in (600, 513, 512, 511, 64, 8, 1):
+        at = q[:B], k, v, table[:B], pos[:B]
+        want = hi.attn_paged(*at, Hq, Hkv)
+        assert same(hi.attn_paged(*at, Hq, Hkv, work=works["step"]), want)
+        assert same(hi.attn_paged(*at, Hq, Hkv, work=works["ragged"]), want)
+        common = table[:1].expand(B, -1).contiguous()
+        want = hi.attn_shared(q[:B], k, v, common, pos[:B], 640, Hq, Hkv)
+        assert same(hi.attn_shared(q[:B], k, v, common, pos[:B], 640, Hq, Hkv, work=works["shared"]), want)
+        for M in (2048, 2016, 1000, 7 * B, B):
+            if M < B or M > 2048:
+                continue
+            start = torch.linspace(0, M, B + 1).int().cuda()
+            ends = pos[:B].clamp(max=600)
+            want = hi.attn_paged(q[:M], k, v, table[:B], ends, Hq, Hkv, start=start)
+            assert same(hi.attn_paged(q[:M], k, v, table[:B], ends, Hq, Hkv, start=start, work=works["ragged"]), want)
+    for w in works.values():
+        assert (w[:hi.ATTN_COUNTER_BYTES] == 0).all()
