@@ -423,6 +423,7 @@ def flash_prefill_lse(q, kc, vc, T, p0, Hq, Hkv, out=None, lse=None):
 # These wrappers are half of a small call's time, so their checks read each property once (60 to 90 ns each) and the common
 # case is one comparison; what fails is looked at again for the message.
 _F16, _F32, _I32, _U8 = torch.float16, torch.float32, torch.int32, torch.uint8
+_INT_MAX = 2**31 - 1  # ctypes passes a larger number on without its upper bits
 _current_gpu = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -452,8 +453,8 @@ def _paged(what, kp, vp, table, Hkv):
             raise ValueError(f"hipinfer_amd.{what}: kp and vp must have the same page stride")
     B, W = tshape
     ldt, one = table.stride()
-    if one != 1 and W > 1:
-        raise ValueError(f"hipinfer_amd.{what}: table rows must be contiguous")
+    if one != 1 and W > 1 or ldt > _INT_MAX and B > 1:
+        raise ValueError(f"hipinfer_amd.{what}: table rows must be contiguous, at most 2^31 - 1 entries apart")
     return (kp.data_ptr(), vp.data_ptr(), step if pages > 1 else Hkv * page * D, pages, page, table.data_ptr(),
             ldt if B > 1 else W, W), B, D
 
@@ -463,8 +464,8 @@ def _rows_of(what, name, t, M, width):
     shape, steps = t.shape, t.stride()
     if t.dtype is not _F16 or len(shape) != 2 or shape[0] != M or shape[1] < width:
         raise ValueError(f"hipinfer_amd.{what}: {name} must be fp16 [{M}, {width}], got {t.dtype} {tuple(shape)}")
-    if steps[1] != 1 and shape[1] > 1:
-        raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous")
+    if steps[1] != 1 and shape[1] > 1 or steps[0] > _INT_MAX and M > 1:
+        raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous, at most 2^31 - 1 elements apart")
     return steps[0] if M > 1 else shape[1]
 
 
