@@ -96,3 +96,41 @@ def test_one_work_buffer_for_smaller_batches(hi):  # noqa: F811
             assert same(hi.attn_paged(q[:M], k, v, table[:B], ends, Hq, Hkv, start=start, work=works["ragged"]), want)
     for w in works.values():
         assert (w[:hi.ATTN_COUNTER_BYTES] == 0).all()
+
+
+@pytest.mark.parametrize("D,G,Hkv", [(128, 4, 8), (64, 8, 4), (128, 6, 2)], ids=["D128", "D64", "G6"])
+@pytest.mark.parametrize("rows,before", [([32], [1000]), ([100], [900]), ([5] * 8, [700, 64, 0, 1500, 31, 2, 900, 333]),
+                                         ([1, 300, 0, 40], [900, 0, 5, 1200])], ids=["32", "100", "8x5", "mixed"])
+@pytest.mark.parametrize("times", [1, 8, 32])
+def test_runs_in_wide_tables(hi, D, G, Hkv, rows, before, times):  # noqa: F811
+    """A table allocated for the longest context there may be: entries behind a sequence's pages are never followed, whichever
+    kernel the width selects."""
+    Hq, page, M = Hkv * G, 16, sum(rows)
+    lens = [p + n for p, n in zip(before, rows)]
+    need = max(-(-n // page) for n in lens)
+    c = Cache(330 + M, lens, Hkv, D, page, width=need * times, unused=2**31 - 1)
+    q = rng(331).standard_normal((M, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    lse = torch.empty(Hq, M, device="cuda")
+    got = hi.attn_paged(dev(q), k, v, table, dev(np.array(before, np.int32)), Hq, Hkv,
+                        start=dev(np.cumsum([0] + rows).astype(np.int32)), lse=lse)
+    want = attend(c, [(b, p + t) for b, (p, n) in enumerate(zip(before, rows)) for t in range(n)], q, Hq)
+    compare("runs", host(got), want)
+    compare_lse("runs", host(lse), want)
+
+
+@pytest.mark.parametrize("D,G,Hkv", [(128, 4, 8), (64, 8, 4)], ids=["D128", "D64"])
+@pytest.mark.parametrize("shared", [0, 256, 4096])
+@pytest.mark.parametrize("times", [1, 8, 32])
+def test_steps_in_wide_tables(hi, D, G, Hkv, shared, times):  # noqa: F811
+    """A decode step without a prefix, with one that is read again, and with one whose own keys share its launch."""
+    B, Hq, page = 24, Hkv * G, 16
+    lens = [shared + 1 + 29 * b for b in range(B)]
+    need = -(-max(lens) // page)
+    c = Cache(340 + shared, lens, Hkv, D, page, shared=shared, width=need * times, unused=-7)
+    q = rng(341).standard_normal((B, Hq * D)).astype(np.float16)
+    k, v, table = c.cuda()
+    pos = dev(np.array(lens, np.int32) - 1)
+    want = attend(c, [(b, n - 1) for b, n in enumerate(lens)], q, Hq)
+    compare("step", host(hi.attn_paged(dev(q), k, v, table, pos, Hq, Hkv)), want)
+    compare("shared", host(hi.attn_shared(dev(q), k, v, table, pos, shared, Hq, Hkv)), want)
