@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(256) rope_paged_any_kernel(RopePagedArgs a, Pa
 // 16-byte accesses: a step turns 8 pairs (the 8 elements at d and the 8 at d + rot / 2, or 8 interleaved ones: 4 pairs) or
 // copies 8 elements; block per row, a thread per step up to 512. `per` steps a q or k head, `turns` of them rotate. The row is
 // requested before its place is known (position, table entry and cs row are a chain of three loads). 2048 rows of 32/8 heads
-// of 128 10.2 us, 5.1 TB/s, what a large copy reaches (the kernel above 15.5); one row 2.3 us, the chain (5.2).
+// of 128 10.2 us, 5.0 TB/s, what a large copy reaches (the kernel above 15.5); one row 2.3 us, the chain (5.2).
 template <typename CS, bool INTER>
 __global__ void __launch_bounds__(512) rope_paged_kernel(RopePagedArgs a, PagedCache c, int per, int turns) {
   constexpr int NP = INTER ? 4 : 8;  // pairs of a step
@@ -132,6 +132,13 @@ __global__ void __launch_bounds__(512) rope_paged_kernel(RopePagedArgs a, PagedC
 }
 
 // ------------------------------------------------------------------ attention
+//
+// o = sum_k w_k v_k, w_k = 2^(x_k - m) / l, x the logits times log2(e) / sqrt(D). Logits, m, l, O and the parts that splits
+// exchange are fp32. The 2^(x_k - m) are rounded to fp16 for the product with V, as in the slot cache's kernels, for its matrix
+// instructions take no fp32: 2^-11 of each weight at most (the error against 64 bits becomes 2.5e-4 to 2.9e-4 of the result, 2.1e-4
+// with fp32 weights and the result rounded alone), and a weight under 2^-25 of the largest that its wave has seen becomes 0: in all at
+// most 2^-25 sum |v| of the keys.
+// An infinity or NaN in a V row reaches the rows that see its key and no other: as itself, or as NaN where its weight has become 0.
 struct AttnArgs {
   const f16* q;
   int64_t ldq;
@@ -160,7 +167,7 @@ struct AttnArgs {
 // and l in fp32, in the lanes' order; of each kFan splits of a tile the block that arrives last joins them, of each kFan such
 // groups the last again, until one block has the tile. Nobody waits. A launch of its own for the joins, us: 7 prompt
 // chunks of 1 to 411 rows 28.9 (here 26.3), and 3 more for every small batch.
-// What bounds it: 2048 rows after 4096 positions (32/8 heads of 128) 176 us, 975 TFLOP/s, as the slot cache's kernel; smaller
+// What bounds it: 2048 rows after 4096 positions (32/8 heads of 128) 178 us, 965 TFLOP/s (the slot cache's kernel 174); smaller
 // batches a chain of about 12 us around their tiles: start and pos, the plan, the table, the first K tile (2 to 3 us), the
 // parts' stores, arrival and join (5 us). Few rows: attn_rows_kernel.
 struct FlashPlan {
@@ -667,7 +674,7 @@ __device__ __forceinline__ void join_parts(float& M, float& L, f32x4& O, const f
 // buffer bounds is done in registers, in a wave's last tile and in tiles with an entry that is no page only: logits of
 // keys that are not there become -inf, their V rows zeros.
 // Measured: 64 sequences of 1000 keys, 32/8 heads of 128, 48.0 us (5.5 TB/s; slots 47.2), 48 of 100 to 2000 46.3 (4.5 TB/s;
-// slots 43.5), one of 4001 9.9 (slots 9.4: the table is one more load in the chain from the position to K).
+// slots 43.5), one of 4001 10.3 (slots 9.4: the table is one more load in the chain from the position to K).
 // OWN: the keys behind a shared prefix; a split leaves its part for join_block.
 struct StepPlan {
   int S, S1;      // splits of a pair: the launch's, and those that give every CU a block (splits_used)
@@ -1492,7 +1499,8 @@ constexpr size_t kWorkHead = kCounters * 4;
 // -> 12.3; 30 of 500 to 4000, 32/8 of 128, 65.3 -> 60.4; 48 of 100 to 2000 46.8 -> 46.8; 16 of 4097 52.3 -> 54.0. (192, 320
 // or 352 keys for the first two and 704 or 1024 for the last: within 3 % over 17 batches, 288 and 12 splits worse.) From two
 // pairs a CU on, a split per 4096 keys only, so that one long sequence does not hold up the batch: 64 of 1000 keys lose 12 %
-// by a second split. A sequence's splits depend on the batch's size, not on the other lengths.
+// by a second split (beyond kCounters pairs, which have no counters, none). A sequence's splits depend on the batch's
+// size, not on the other lengths.
 void step_splits(int B, int Hkv, int G, int cus, StepPlan& f, bool& wide) {
   const int64_t pairs = (int64_t)B * Hkv;
   f.K = 0;
@@ -1520,7 +1528,8 @@ constexpr int kRowsFan = 32;      // the block that arrives last joins all split
 //    to 4000 23.4 / 21.1, 64 x 2 after 1000 60.1 / 49.7, 63 after 1000 and 65 after 16000 245 / 156, 31 after 500 and 97 (388
 //    packed) after 8000 59.0 / 89.6;
 //  * and where the tiles are at most half as many as CUs and can read 1536 keys for each CU in all, going by the table's
-//    width: 32 rows after 1000 21.3 / 14.0, after 8000 30.4 / 22.9, 100 after 4000 27.3 / 32.4, 64 after 16000 40.6 / 53.2,
+//    width, the one bound that the host has (32 rows after 1000 in tables of 1, 8 and 32 times the width that they
+//    need 13.9, 13.9, 21.1 us; 100 rows 17.4, 21.3, 21.2): 32 rows after 1000 21.3 / 14.0, after 8000 30.4 / 22.9, 100 after 4000 27.3 / 32.4, 64 after 16000 40.6 / 53.2,
 //    32 after 32000 48.5 / 60.5; 12/2 heads of 128, 19 after 1881 22.7 / 14.5, 250 after 1000 22.8 / 18.1.
 int row_columns(int M, int B, int G, int Hkv, int64_t cap, int cus) {
   const int tiles = plan_tiles(M, G, 32);

@@ -557,7 +557,8 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
     int32, a ragged batch: rows start[b] .. start[b + 1] - 1 of q are sequence b's, at positions pos[b], pos[b] + 1, ...
     (prompt chunks, drafted rows to verify, single rows of decoding sequences, in any mixture; start does not
     decrease). A row at position p sees keys 0 .. p, at most those its table row holds; keys whose page id lies outside
-    [0, pages) are left out. A row that sees no key (pos -1: padding) gives zeros.
+    [0, pages) are left out. A row that sees no key (pos -1: padding) gives zeros. With start, short runs are faster in a table
+    that is not much wider than they need (table[:, :W] is one), and a row's last bits depend on the batch it is in.
 
     Returns out [M, Hq*D], which may be q itself, else shares no memory with it; rows that belong to no sequence are left as they were (in a new out, as
     allocated). lse [Hq, M] fp32, if given, receives the base-2 log-sum-exp of each row's scaled logits (-inf without

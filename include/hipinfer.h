@@ -186,7 +186,9 @@ size_t hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ra
  * rows start[b] .. start[b + 1] - 1 at positions pos[b], pos[b] + 1, ... of sequence b (start [B + 1], not
  * decreasing). A row at position p sees keys 0 .. p that its table row and the pages hold; a row without any gives 0 and
  * lse -inf. Rows of no sequence are left as they were. Hq / Hkv in 1..16, query head h reads kv head h / (Hq / Hkv). out
- * [M, ldo] may be q itself with ldo == ldq; else rows that meet q's are refused. lse
+ * [M, ldo] may be q itself with ldo == ldq; else rows that meet q's are refused. With start, the kernel for short runs is
+ * chosen by the table's width W * page among others (W no wider than needed is faster), and a row's keys are split by all
+ * sequences' lengths: its last bits depend on the batch. lse
  * [Hq][M] fp32 (base-2 log-sum-exp of the scaled logits) or NULL. work: work_bytes >= hi_attn_paged_work_bytes(...),
  * 16-byte aligned; launches that share it must not run concurrently. */
 int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,
