@@ -1528,9 +1528,10 @@ constexpr int kRowsFan = 32;      // the block that arrives last joins all split
 //    to 4000 23.4 / 21.1, 64 x 2 after 1000 60.1 / 49.7, 63 after 1000 and 65 after 16000 245 / 156, 31 after 500 and 97 (388
 //    packed) after 8000 59.0 / 89.6;
 //  * and where the tiles are at most half as many as CUs and can read 1536 keys for each CU in all, going by the table's
-//    width, the one bound that the host has (32 rows after 1000 in tables of 1, 8 and 32 times the width that they
-//    need 13.9, 13.9, 21.1 us; 100 rows 17.4, 21.3, 21.2): 32 rows after 1000 21.3 / 14.0, after 8000 30.4 / 22.9, 100 after 4000 27.3 / 32.4, 64 after 16000 40.6 / 53.2,
-//    32 after 32000 48.5 / 60.5; 12/2 heads of 128, 19 after 1881 22.7 / 14.5, 250 after 1000 22.8 / 18.1.
+//    width, the one bound that the host has: 32 rows after 1000 21.3 / 14.0, after 8000 30.4 / 22.9, 100 after 4000 27.3 / 32.4,
+//    64 after 16000 40.6 / 53.2, 32 after 32000 48.5 / 60.5; 12/2 heads of 128, 19 after 1881 22.7 / 14.5, 250 after 1000
+//    22.8 / 18.1. In tables of 1, 8 and 32 times the width that they need, 32 rows after 1000 take 13.9, 13.9 and 21.1, 100 rows
+//    17.4, 21.3 and 21.2.
 int row_columns(int M, int B, int G, int Hkv, int64_t cap, int cus) {
   const int tiles = plan_tiles(M, G, 32);
   const bool one = (int64_t)M * G <= 32 * (int64_t)B && (int64_t)(M - min(B, M) + 1) * G <= 384;

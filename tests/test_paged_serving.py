@@ -134,3 +134,24 @@ def test_steps_in_wide_tables(hi, D, G, Hkv, shared, times):  # noqa: F811
     want = attend(c, [(b, n - 1) for b, n in enumerate(lens)], q, Hq)
     compare("step", host(hi.attn_paged(dev(q), k, v, table, pos, Hq, Hkv)), want)
     compare("shared", host(hi.attn_shared(dev(q), k, v, table, pos, shared, Hq, Hkv)), want)
+
+
+@pytest.mark.parametrize("form", ["shared", "step", "runs"])
+def test_most_sequences(hi, form):  # noqa: F811
+    """As many sequences as a call takes (65535; 30000 runs), with parts beyond 2 GiB: rows from all over the batch are right."""
+    D, G, Hkv, page, B = 128, 8, 8, 16, 30000 if form == "runs" else 65535
+    Hq, shared = Hkv * G, 16
+    c = Cache(350, [48] * 40, Hkv, D, page, shared=shared)
+    k, v, rows = c.cuda()
+    of = torch.arange(B, device="cuda") % 40
+    table = rows[of].contiguous()
+    pos = (torch.arange(B, device="cuda") % 37 + 10).int()
+    q = torch.randn(B, Hq * D, device="cuda", dtype=torch.float16, generator=torch.Generator("cuda").manual_seed(351))
+    if form == "shared":
+        got = hi.attn_shared(q, k, v, table, pos, shared, Hq, Hkv)
+    else:
+        start = torch.arange(B + 1, dtype=torch.int32, device="cuda") if form == "runs" else None
+        got = hi.attn_paged(q, k, v, table, pos, Hq, Hkv, start=start)
+    some = [0, 1, 39, 40, 4095, 4096, 16383, 29999] + ([] if form == "runs" else [32768, 50001, 65534])
+    want = attend(c, [(b % 40, b % 37 + 10) for b in some], host(q[some]), Hq)
+    compare(form, host(got[some]), want)
