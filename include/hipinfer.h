@@ -188,10 +188,10 @@ size_t hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ra
  * lse -inf. Rows of no sequence are left as they were. Hq / Hkv in 1..16, query head h reads kv head h / (Hq / Hkv). out
  * [M, ldo] may be q itself with ldo == ldq; else rows that meet q's are refused. With start, the kernel for short runs is
  * chosen by the table's width W * page among others (W no wider than needed is faster), and a row's keys are split by all
- * sequences' lengths: its last bits depend on the batch. lse
- * [Hq][M] fp32 (base-2 log-sum-exp of the scaled logits) or NULL. Without start at most 65535 sequences; with it at most 65535
- * row tiles, which B + M (Hq / Hkv) / 64 <= 65535, or B <= 32767 runs of one row, never exceed. work: work_bytes >= hi_attn_paged_work_bytes(...),
- * 16-byte aligned; launches that share it must not run concurrently. */
+ * sequences' lengths: its last bits depend on the batch. lse [Hq][M] fp32 (base-2 log-sum-exp of the scaled logits) or
+ * NULL. Without start at most 65535 sequences; with it at most 65535 row tiles, which B <= 32767 runs of one row never
+ * exceed. work: work_bytes >= hi_attn_paged_work_bytes(...), 16-byte aligned; launches that share it must not run
+ * concurrently. */
 int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,
                   const int* table, int ldt, int W, const int* start, const int* pos, void* out, int ldo, float* lse,
                   int M, int B, int Hq, int Hkv, int D, void* work, size_t work_bytes, void* stream);
