@@ -284,13 +284,15 @@ def run(s):
             return s["best"], s["parent"], s["token"]
         if c["op"] == "fork":
             if "work" not in s:
+                s["set"] = hi.cache_set(s["caches"], c["page"])
                 s["work"] = hi.cache_work(s["table"].shape[0], s["parent"].shape[0], s["refs"].shape[0])
-            hi.cache_fork(s["caches"], c["page"], s["table"], s["lens"], s["parent"], s["refs"], grow=1, table_out=s["table_out"],
+            hi.cache_fork(s["set"], s["table"], s["lens"], s["parent"], s["refs"], grow=1, table_out=s["table_out"],
                           lens_out=s["lens_out"], refs_out=s["refs_out"], missing=s["missing"], work=s["work"])
             return s["table_out"], s["lens_out"], s["refs_out"], s["missing"], s["pools"]
         if "work" not in s:
+            s["set"] = hi.cache_set(s["caches"], c["page"])
             s["work"] = hi.cache_work(s["table"].shape[0], 0, s["refs"].shape[0])
-        hi.cache_compact(s["caches"], s["table"], s["refs"], table_out=s["table_out"], refs_out=s["refs_out"], moved=s["moved"],
+        hi.cache_compact(s["set"], s["table"], s["refs"], table_out=s["table_out"], refs_out=s["refs_out"], moved=s["moved"],
                          used=s["used"], work=s["work"])
         return s["table_out"], s["refs_out"], s["moved"], s["used"], s["pools"]
     return {"append": _append_plain, "attn": _attn_plain, "beam": _beam_plain, "fork": _fork_plain,
