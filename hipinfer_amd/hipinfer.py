@@ -95,6 +95,16 @@ size hi_attn_shared_work_bytes_max(int B, int Hq, int Hkv, int D);
 int hi_attn_shared(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
                    int shared, ptr pos, ptr out, int ldo, ptr lse, int B, int Hq, int Hkv, int D, ptr work,
                    size work_bytes, ptr stream);
+size hi_beam_select_work_bytes(int B, int beams, int V, int n);
+int hi_beam_select(ptr logits, i64 ldl, ptr scores, int B, int beams, int V, int n, ptr best, ptr parent, ptr token,
+                   ptr work, size work_bytes, ptr stream);
+size hi_cache_work_bytes(int S, int N, int pages);
+int hi_cache_fork(ptr caches, ptr strides, ptr bytes, ptr runs, int n, int page, ptr table, int ldt, int W, int S, ptr lens,
+                  ptr parent, int N, ptr refs, int pages, int grow, ptr table_out, int ldo, ptr lens_out, ptr refs_out,
+                  ptr missing, ptr work, size work_bytes, ptr stream);
+int hi_cache_compact(ptr caches, ptr strides, ptr bytes, ptr runs, int n, int page, ptr table, int ldt, int W, int S, ptr refs,
+                     int pages, ptr table_out, int ldo, ptr refs_out, ptr moved, ptr used, ptr work, size work_bytes,
+                     ptr stream);
 ptr hi_load(str path, int max_batch, int max_seq, int max_prefill);
 ptr hi_load_tp(str path, int max_batch, int max_seq, int max_prefill, int world, ptr devs);
 void hi_free(ptr e);
@@ -607,6 +617,186 @@ def attn_shared(q, kp, vp, table, pos, shared, Hq, Hkv, out=None, lse=None, work
         work = _attn_work(what, lib.hi_attn_shared_work_bytes(B, Hq, Hkv, D))
     check_rc(lib.hi_attn_shared(q.data_ptr(), ldq, *cache, shared, pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), B, Hq,
                                 Hkv, D, work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
+    return out
+
+
+class CacheSet:
+    """The cache tensors of some layers as the calls that move pages take them (cache_set)."""
+
+    def __init__(self, tensors, page):
+        what = "cache_set"
+        self.tensors, self.page, n = tuple(tensors), page, len(tensors)
+        if page < 1 or page & (page - 1):
+            raise ValueError(f"hipinfer_amd.{what}: page {page} must be a power of two")
+        self.pages = self.tensors[0].shape[0] if n else None
+        self.gpu = self.tensors[0].get_device() if n else None
+        self._ptrs, self._runs = (ctypes.c_void_p * n)(), (ctypes.c_int * n)()
+        self._strides, self._bytes = (ctypes.c_longlong * n)(), (ctypes.c_longlong * n)()
+        for i, t in enumerate(self.tensors):
+            _need(what, t)
+            if t.get_device() != self.gpu:
+                raise ValueError(f"hipinfer_amd.{what}: tensors on several GPUs")
+            if t.dim() not in (2, 4) or t.shape[0] != self.pages or t.numel() == 0 or (t.dim() == 4 and t.shape[2] != page):
+                raise ValueError(f"hipinfer_amd.{what}: tensors must be [pages {self.pages}, heads, page {page}, D] or [pages, "
+                                 f"heads], got {tuple(t.shape)}")
+            if not t[0].is_contiguous():
+                raise ValueError(f"hipinfer_amd.{what}: a page must be packed")
+            size = t.element_size()
+            self._ptrs[i], self._runs[i] = t.data_ptr(), t.shape[1] if t.dim() == 4 else 0
+            self._bytes[i] = t[0].numel() * size
+            self._strides[i] = t.stride(0) * size if self.pages > 1 else self._bytes[i]
+        self._args = (self._ptrs, self._strides, self._bytes, self._runs, n, page)
+
+
+def cache_set(caches, page):
+    """The tensors whose pages cache_fork and cache_compact copy: of each layer kp and vp [pages, heads, page, D], and what else
+    belongs to a page ([pages, heads], as rope_cache_paged8's exponents). All have the same number of pages; a page is
+    packed, pages may be strided. Made once for caches that stay where they are."""
+    return CacheSet(caches, page)
+
+
+def cache_work(seqs, rows, pages):
+    """A work buffer of cache_fork for a table of `seqs` rows and `rows` new ones (rows 0: of cache_compact) in a pool of `pages`;
+    it serves smaller calls too. Calls that use one buffer must not overlap in time."""
+    size = lib.hi_cache_work_bytes(seqs, rows, pages)
+    if size == 0:
+        raise ValueError("hipinfer_amd.cache_work: unsupported sizes")
+    return torch.empty(size, dtype=torch.uint8, device="cuda")
+
+
+def _pool_args(what, caches, table, refs, table_out, refs_out, rows, work, others):
+    """Checks what cache_fork and cache_compact have in common; returns the row strides of table and table_out."""
+    gpu = table.get_device()
+    if gpu < 0 or gpu != _current_gpu() or any(t is not None and t.get_device() != gpu
+                                               for t in (refs, table_out, refs_out, work, *others)):
+        _elsewhere(what, table, refs, table_out, refs_out, work, *others)
+    if not isinstance(caches, CacheSet) or (caches.tensors and (caches.gpu != gpu or caches.pages != refs.shape[0])):
+        raise ValueError(f"hipinfer_amd.{what}: caches must be a cache_set on the current GPU, of as many pages as refs")
+    if refs.dim() != 1:
+        raise ValueError(f"hipinfer_amd.{what}: refs must be int32 [pages], got {tuple(refs.shape)}")
+    for name, t in (("refs", refs), ("refs_out", refs_out)):
+        _vector(what, name, t, refs.shape[0])
+    steps = []
+    for name, t, n in (("table", table, table.shape[0]), ("table_out", table_out, rows)):
+        if t.dtype is not _I32 or t.dim() != 2 or t.shape != (n, table.shape[1]):
+            raise ValueError(f"hipinfer_amd.{what}: {name} must be int32 [{n}, {table.shape[-1]}], got {t.dtype} {tuple(t.shape)}")
+        ld, one = t.stride()
+        if n and one != 1 and t.shape[1] > 1 or n > 1 and not t.shape[1] <= ld <= _INT_MAX:
+            raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous and apart, at most 2^31 - 1 entries")
+        steps.append(ld if n > 1 else t.shape[1])
+    if work is not None and (work.dtype is not _U8 or not work.is_contiguous()):
+        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8")
+    return steps
+
+
+def cache_fork(caches, table, lens, parent, refs, grow=0, table_out=None, lens_out=None, refs_out=None, missing=None,
+               work=None):
+    """Makes N new rows of a page table [S, W], row i the continuation of row parent[i]: the same lens[parent[i]] positions, and
+    pages for `grow` more. Beams after beam_select, several answers to one prompt, sequences that begin (a parent of length 0)
+    or end (a parent that is no row, as -1: an empty row).
+
+    refs [pages] int32 counts who holds a page: a table row that names it counts 1, 0 is free; pages that the caller keeps for
+    itself (a cached prompt) count 1 more. Whole pages are shared with the parent. Of the entries behind them the parent's first
+    child keeps the pages that only its parent holds; the other children, and those that find a shared page there, get free
+    pages, the lowest first, in the order of rows and entries, and the positions held of a part-filled page are copied in
+    all tensors of `caches` (cache_set). What no new row holds loses its count, and is free for the next call. Entries
+    that name no page are taken over as they are found missing (-1 for a whole page).
+
+    Returns (table_out [N, W], lens_out [N]), memory apart from table and lens; refs is updated in place, or refs_out
+    written instead. missing [1] int32, if given, receives how many pages were not to be had: their entries are -1. Everything
+    is read on the device: the call can be captured. At most 8192 rows."""
+    what = "cache_fork"
+    N = parent.shape[0]
+    table_out = torch.empty(N, table.shape[-1], dtype=torch.int32, device=table.device) if table_out is None else table_out
+    lens_out = torch.empty(N, dtype=torch.int32, device=table.device) if lens_out is None else lens_out
+    refs_out = refs if refs_out is None else refs_out
+    ldt, ldo = _pool_args(what, caches, table, refs, table_out, refs_out, N, work, (lens, parent, lens_out, missing))
+    S, W = table.shape
+    _vector(what, "lens", lens, S)
+    _vector(what, "parent", parent, N)
+    _vector(what, "lens_out", lens_out, N)
+    if missing is not None:
+        _vector(what, "missing", missing, 1)
+    if not 0 <= grow <= 1 << 30:
+        raise ValueError(f"hipinfer_amd.{what}: room for {grow} positions")
+    if work is None:
+        work = cache_work(S, N, refs.shape[0])
+    check_rc(lib.hi_cache_fork(*caches._args, table.data_ptr(), ldt, W, S, lens.data_ptr(), parent.data_ptr(), N,
+                               refs.data_ptr(), refs.shape[0], grow, table_out.data_ptr(), ldo, lens_out.data_ptr(),
+                               refs_out.data_ptr(), _addr(missing), work.data_ptr(), work.numel(), _stream()), what)
+    return table_out, lens_out
+
+
+def cache_compact(caches, table, refs, table_out=None, refs_out=None, moved=None, used=None, work=None):
+    """Moves the pages in use (refs > 0) to the front of the pool: with U of them, those at or behind U take the free places
+    before U, both in ascending order, in all tensors of `caches` (cache_set); pages from U on are then free, and a smaller
+    pool can be cut off there. Entries of table [S, W] (-1 for one whose page is free) and refs are renamed, in place or into
+    table_out and refs_out.
+
+    Returns moved [pages] int32, where each page went (-1 for a free one), for tables of the caller's own, and used [1] int32,
+    U. Read on the device: the call can be captured."""
+    what = "cache_compact"
+    table_out = table if table_out is None else table_out
+    refs_out = refs if refs_out is None else refs_out
+    moved = torch.empty_like(refs) if moved is None else moved
+    used = torch.empty(1, dtype=torch.int32, device=refs.device) if used is None else used
+    S = table.shape[0]
+    ldt, ldo = _pool_args(what, caches, table, refs, table_out, refs_out, S, work, (moved, used))
+    _vector(what, "moved", moved, refs.shape[0])
+    _vector(what, "used", used, 1)
+    if work is None:
+        work = cache_work(S, 0, refs.shape[0])
+    check_rc(lib.hi_cache_compact(*caches._args, table.data_ptr(), ldt, table.shape[1], S, refs.data_ptr(), refs.shape[0],
+                                  table_out.data_ptr(), ldo, refs_out.data_ptr(), moved.data_ptr(), used.data_ptr(),
+                                  work.data_ptr(), work.numel(), _stream()), what)
+    return moved, used
+
+
+def beam_select_work(seqs, beams, V, n):
+    """A work buffer of beam_select for those sizes; it serves any call that needs no more bytes. Calls that use one buffer must
+    not overlap in time."""
+    size = lib.hi_beam_select_work_bytes(seqs, beams, V, n)
+    if size == 0:
+        raise ValueError("hipinfer_amd.beam_select_work: unsupported sizes")
+    return torch.empty(size, dtype=torch.uint8, device="cuda")
+
+
+def beam_select(logits, scores, beams, n=None, out=None, work=None):
+    """Beam search's selection: of every sequence's candidates, its `beams` rows of logits [B * beams, V] fp16 by their V tokens,
+    the n (default beams; at most 64) with the best scores, in order: scores[row] fp32 + the token's log-probability.
+    The lowest (beam, token) wins a tie; scores closer than 2^-35 (1 + their distance from the best) are one.
+
+    Returns (best [B, n] fp32, parent [B, n] int32, token [B, n] int32), parent the row of logits (cache_fork's parent). A
+    candidate has no finite score where its logit is -inf, its row's score is not finite (a beam that has ended), or a logit
+    of its row is NaN or +inf; nor do those 2^31 or more below the best count. Places without a candidate hold -inf, -1 and -1.
+    At most 64 beams, beams * V at most 2^24."""
+    what = "beam_select"
+    n = beams if n is None else n
+    R, V = logits.shape if logits.dim() == 2 else (0, 0)
+    if logits.dtype is not _F16 or logits.dim() != 2 or beams < 1 or R % beams:
+        raise ValueError(f"hipinfer_amd.{what}: logits must be fp16 [B * beams {beams}, V], got {logits.dtype} "
+                         f"{tuple(logits.shape)}")
+    B, gpu = R // beams, logits.get_device()
+    ld, one = logits.stride()
+    if one != 1 and V > 1 or R > 1 and ld < V:
+        raise ValueError(f"hipinfer_amd.{what}: rows of logits must be contiguous and apart")
+    if out is None:
+        out = (torch.empty(B, n, device=logits.device), *(torch.empty(B, n, dtype=torch.int32, device=logits.device)
+                                                          for _ in range(2)))
+    best, parent, token = out
+    if gpu < 0 or gpu != _current_gpu() or any(t.get_device() != gpu for t in (scores, *out)) or \
+            (work is not None and work.get_device() != gpu):
+        _elsewhere(what, logits, scores, *out, work)
+    for name, t, dtype, shape in (("scores", scores, _F32, (R,)), ("best", best, _F32, (B, n)), ("parent", parent, _I32, (B, n)),
+                                  ("token", token, _I32, (B, n))):
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"hipinfer_amd.{what}: {name} must be packed {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    if work is None:
+        work = beam_select_work(B, beams, V, n)
+    elif work.dtype is not _U8 or not work.is_contiguous():
+        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8")
+    check_rc(lib.hi_beam_select(logits.data_ptr(), ld if R > 1 else V, scores.data_ptr(), B, beams, V, n, best.data_ptr(),
+                                parent.data_ptr(), token.data_ptr(), work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
     return out
 
 

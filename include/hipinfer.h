@@ -204,6 +204,39 @@ int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long 
                    const int* table, int ldt, int W, int shared, const int* pos, void* out, int ldo, float* lse, int B,
                    int Hq, int Hkv, int D, void* work, size_t work_bytes, void* stream);
 
+/* ---- beam search over a pool of pages. No counterpart in the reference.
+ * Selection: of each of B sequences' candidates, `beams` rows of logits [B * beams, ldl] fp16 by V tokens, the n with the best
+ * scores[row] + log-probability, in order: best [B][n] fp32, parent [B][n] (the row of logits), token [B][n]. The lowest
+ * (beam, token) wins a tie (scores closer than 2^-35 (1 + their distance from the best)); places without a candidate hold
+ * -inf, -1, -1: a logit of -inf, a row whose score is not finite or that holds a NaN or +inf, and what lies 2^31 or more below
+ * the best are none. beams and n 1 to 64, beams * V <= 2^24, B * beams <= 65535. work: hi_beam_select_work_bytes(...) (0 for
+ * bad sizes), 16-byte aligned, no state; launches that share it must not run concurrently. */
+size_t hi_beam_select_work_bytes(int B, int beams, int V, int n);
+int hi_beam_select(const void* logits, long long ldl, const float* scores, int B, int beams, int V, int n, float* best,
+                   int* parent, int* token, void* work, size_t work_bytes, void* stream);
+/* Bytes of the work buffer of hi_cache_fork for tables of S and N rows, and of hi_cache_compact (N = 0); 0 for bad sizes. No
+ * state; launches that share it must not run concurrently. */
+size_t hi_cache_work_bytes(int S, int N, int pages);
+/* N new table rows, row i the continuation of row parent[i] of table [S, ldt] (W entries, pages of `page` positions): lens_out[i] =
+ * lens[parent[i]] positions and pages for `grow` more; a parent outside [0, S) gives an empty row. refs [pages] counts a
+ * page's holders (table entries, and the caller's own), 0 is free. Whole pages are shared; of the entries behind them the first child
+ * keeps those pages whose count is 1, others get free pages (lowest first, in the order of rows and entries; -1, counted in
+ * `missing` if not NULL, when there are none) and the positions held of a part-filled page are copied. refs_out (refs itself,
+ * or apart) has the new counts; pages that they free are handed out by later calls.
+ * The n cache tensors (host arrays): caches[t] with pages strides[t] bytes apart, bytes[t] per page, which are runs[t] runs of
+ * `page` positions (heads), or with runs[t] 0 are copied whole. table_out and lens_out are apart from table and lens. S, N
+ * <= 8192. */
+int hi_cache_fork(void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
+                  const int* table, int ldt, int W, int S, const int* lens, const int* parent, int N, const int* refs,
+                  int pages, int grow, int* table_out, int ldo, int* lens_out, int* refs_out, int* missing, void* work,
+                  size_t work_bytes, void* stream);
+/* Moves the pages in use (refs > 0), U of them, to the front: those at or behind U take the free places before U, both in
+ * order. moved [pages]: where each went (-1: free); table_out (table itself, or apart) the renamed entries, refs_out (likewise)
+ * the moved counts, used (if not NULL) U. */
+int hi_cache_compact(void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
+                     const int* table, int ldt, int W, int S, const int* refs, int pages, int* table_out, int ldo,
+                     int* refs_out, int* moved, int* used, void* work, size_t work_bytes, void* stream);
+
 /* ---- RMSNorm (unfused form of the GEMV prologue; the reference's tests build references with it)
  * y[M, H] = w * fp16(x * rsqrt(mean(x^2) + eps)), rows contiguous. Replaces api.cu:76-79
  * (hi_rmsnorm); hipinfer.py:13. */
