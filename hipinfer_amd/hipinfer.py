@@ -90,6 +90,12 @@ size hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ragg
 int hi_attn_paged(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
                   ptr start, ptr pos, ptr out, int ldo, ptr lse, int M, int B, int Hq, int Hkv, int D, ptr work,
                   size work_bytes, ptr stream);
+int hi_rope_cache_paged8(ptr qkv, int ldq, ptr q_out, int ldqo, int M, int Hq, int Hkv, int D, ptr cs, int cs_rows,
+                         int cs_f32, int rot, int interleaved, ptr start, ptr pos, ptr kp, ptr vp, ptr kexp, ptr vexp,
+                         i64 page_stride, int pages, int page, ptr table, int ldt, int W, int B, ptr stream);
+int hi_attn_paged8(ptr q, int ldq, ptr kp, ptr vp, ptr kexp, ptr vexp, i64 page_stride, int pages, int page, ptr table,
+                   int ldt, int W, ptr start, ptr pos, ptr out, int ldo, ptr lse, int M, int B, int Hq, int Hkv, int D,
+                   ptr work, size work_bytes, ptr stream);
 size hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D);
 size hi_attn_shared_work_bytes_max(int B, int Hq, int Hkv, int D);
 int hi_attn_shared(ptr q, int ldq, ptr kp, ptr vp, i64 page_stride, int pages, int page, ptr table, int ldt, int W,
@@ -433,6 +439,7 @@ def flash_prefill_lse(q, kc, vc, T, p0, Hq, Hkv, out=None, lse=None):
 # These wrappers are half of a small call's time, so their checks read each property once (60 to 90 ns each) and the common
 # case is one comparison; what fails is looked at again for the message.
 _F16, _F32, _I32, _U8 = torch.float16, torch.float32, torch.int32, torch.uint8
+_F8, _I8 = torch.float8_e4m3fn, torch.int8
 _INT_MAX = 2**31 - 1  # ctypes passes a larger number on without its upper bits
 _current_gpu = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -444,13 +451,13 @@ def _elsewhere(what, *tensors):
                      f"{sorted({str(t.device) for t in tensors if t is not None})}")
 
 
-def _paged(what, kp, vp, table, Hkv):
+def _paged(what, kp, vp, table, Hkv, dtype=_F16):
     """Checks a paged cache kp / vp [pages, Hkv, page, D] and its table [B, W]; returns the cache's arguments of a library
     call, B and D."""
     shape, steps, tshape = kp.shape, kp.stride(), table.shape
-    if len(shape) != 4 or kp.dtype is not _F16 or vp.dtype is not _F16 or vp.shape != shape or shape[1] != Hkv:
-        raise ValueError(f"hipinfer_amd.{what}: kp and vp must be fp16 [pages, Hkv {Hkv}, page, D], got {kp.dtype} "
-                         f"{tuple(shape)} and {vp.dtype} {tuple(vp.shape)}")
+    if len(shape) != 4 or kp.dtype is not dtype or vp.dtype is not dtype or vp.shape != shape or shape[1] != Hkv:
+        raise ValueError(f"hipinfer_amd.{what}: kp and vp must be {'fp16' if dtype is _F16 else dtype} [pages, Hkv {Hkv}, page, D], "
+                         f"got {kp.dtype} {tuple(shape)} and {vp.dtype} {tuple(vp.shape)}")
     if len(tshape) != 2 or table.dtype is not _I32:
         raise ValueError(f"hipinfer_amd.{what}: the table must be int32 [B, W], got {table.dtype} {tuple(tshape)}")
     pages, _, page, D = shape
@@ -524,10 +531,59 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
                                      _raw_stream(gpu)), what)
 
 
-def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu):
+def _exponents(what, kp, kexp, vexp):
+    """Checks the exponents of an 8-bit cache."""
+    shape = kp.shape[:2]
+    for name, t in (("kexp", kexp), ("vexp", vexp)):
+        if t.dtype is not _I8 or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"hipinfer_amd.{what}: {name} must be packed int8 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def rope_cache_paged8(qkv, Hq, Hkv, cs, kp, vp, kexp, vexp, table, pos, start=None, interleaved=False, q_out=None):
+    """rope_cache_paged for a cache in 8 bits: kp / vp [pages, Hkv, page, D] float8_e4m3fn codes and kexp / vexp [pages, Hkv]
+    int8, an element's value its code times 2 to the power of its page's and head's exponent. qkv, cs, interleaved and q_out are
+    rope_cache_paged's. Rows are attn_paged's: row b of qkv is sequence b's one row at position pos[b], or with start [B + 1]
+    int32 rows start[b] .. start[b + 1] - 1 are sequence b's, at positions pos[b], pos[b] + 1, ... (start does not decrease).
+
+    The exponent of a page and head is the least k of -32 to 8 that holds every value |x| <= 448 * 2^k written to its positions
+    so far (a page's first position, when written, begins anew); each value is rounded once, to the nearest of 4 significant
+    bits, k after its rotation without a rounding to fp16 before. Where k grows, the page's earlier positions are moved
+    to it, which loses only bits below 2^-15 of the page's largest value. Values beyond +-61440 (infinities too) become that, NaN
+    stays NaN.
+
+    Rows append: positions of a page behind the last one written are not kept, and every page that a call writes belongs to one
+    sequence. A row that has no place is left out, its q too, as in rope_cache_paged."""
+    what = "rope_cache_paged8"
+    gpu = qkv.get_device()
+    if not (gpu == kp.get_device() == vp.get_device() == kexp.get_device() == vexp.get_device() == table.get_device() ==
+            pos.get_device() == cs.get_device()) or (start is not None and start.get_device() != gpu) or \
+            (q_out is not None and q_out.get_device() != gpu) or gpu < 0 or gpu != _current_gpu():
+        _elsewhere(what, qkv, cs, kp, vp, kexp, vexp, table, pos, start, q_out)
+    cache, B, D = _paged(what, kp, vp, table, Hkv, _F8)
+    _exponents(what, kp, kexp, vexp)
+    M = qkv.shape[0]
+    ldq = _rows_of(what, "qkv", qkv, M, (Hq + 2 * Hkv) * D)
+    cshape, wide = cs.shape, cs.dtype is _F32
+    if not (wide or cs.dtype is _F16) or len(cshape) != 3 or cshape[2] != 2 or not cs.is_contiguous():
+        raise ValueError(f"hipinfer_amd.{what}: cs must be packed [positions, rot/2, 2], fp16 or fp32")
+    _vector(what, "pos", pos, B)
+    if start is not None:
+        _vector(what, "start", start, B + 1)
+    elif M != B:
+        raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences (one row each without start)")
+    if q_out is None:
+        q_out, ldo = qkv, ldq
+    else:
+        ldo = _rows_of(what, "q_out", q_out, M, Hq * D)
+    check_rc(lib.hi_rope_cache_paged8(qkv.data_ptr(), ldq, q_out.data_ptr(), ldo, M, Hq, Hkv, D, cs.data_ptr(), cshape[0],
+                                      wide, 2 * cshape[1], interleaved, _addr(start), pos.data_ptr(), *cache[:2],
+                                      kexp.data_ptr(), vexp.data_ptr(), *cache[2:], B, _raw_stream(gpu)), what)
+
+
+def _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu, dtype=_F16):
     """Checks what attn_paged and attn_shared have in common; returns the cache's arguments, M, B, D, q's row stride, out
     and its row stride."""
-    cache, B, D = _paged(what, kp, vp, table, Hkv)
+    cache, B, D = _paged(what, kp, vp, table, Hkv, dtype)
     M, width = q.shape[0], Hq * D
     ldq = _rows_of(what, "q", q, M, width)
     _vector(what, "pos", pos, B)
@@ -590,6 +646,30 @@ def attn_paged(q, kp, vp, table, pos, Hq, Hkv, start=None, out=None, lse=None, w
         work = _attn_work(what, lib.hi_attn_paged_work_bytes(M, B, Hq, Hkv, D, int(start is not None)))
     check_rc(lib.hi_attn_paged(q.data_ptr(), ldq, *cache, _addr(start), pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), M,
                                B, Hq, Hkv, D, work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
+    return out
+
+
+def attn_paged8(q, kp, vp, kexp, vexp, table, pos, Hq, Hkv, start=None, out=None, lse=None, work=None):
+    """attn_paged over a cache in 8 bits (rope_cache_paged8's kp, vp, kexp, vexp): keys and values are code * 2^exponent, as fp16.
+    Everything else is attn_paged's, its work buffers (attn_paged_work) too."""
+    what = "attn_paged8"
+    gpu = q.get_device()
+    if not (gpu == kp.get_device() == vp.get_device() == kexp.get_device() == vexp.get_device() == table.get_device() ==
+            pos.get_device()) or gpu < 0 or gpu != _current_gpu():
+        _elsewhere(what, q, kp, vp, kexp, vexp, table, pos)
+    cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu, _F8)
+    _exponents(what, kp, kexp, vexp)
+    if start is not None:
+        _vector(what, "start", start, B + 1)
+        if start.get_device() != gpu:
+            _elsewhere(what, q, start)
+    elif M != B:
+        raise ValueError(f"hipinfer_amd.{what}: {M} rows for a table of {B} sequences (one row each without start)")
+    if work is None:
+        work = _attn_work(what, lib.hi_attn_paged_work_bytes(M, B, Hq, Hkv, D, int(start is not None)))
+    check_rc(lib.hi_attn_paged8(q.data_ptr(), ldq, *cache[:2], kexp.data_ptr(), vexp.data_ptr(), *cache[2:], _addr(start),
+                                pos.data_ptr(), out.data_ptr(), ldo, _addr(lse), M, B, Hq, Hkv, D, work.data_ptr(),
+                                work.numel(), _raw_stream(gpu)), what)
     return out
 
 

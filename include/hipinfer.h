@@ -195,6 +195,22 @@ size_t hi_attn_paged_work_bytes_max(int M, int B, int Hq, int Hkv, int D, int ra
 int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long long page_stride, int pages, int page,
                   const int* table, int ldt, int W, const int* start, const int* pos, void* out, int ldo, float* lse,
                   int M, int B, int Hq, int Hkv, int D, void* work, size_t work_bytes, void* stream);
+/* The two over a cache in 8 bits: kp / vp [pages][Hkv][page][D] e4m3 codes (page_stride in elements, a multiple of 16), kexp /
+ * vexp [pages][Hkv] int8, a value code * 2^exponent, as fp16.
+ * hi_rope_cache_paged8's rows are hi_attn_paged's: start NULL, row b at pos[b] of sequence b (M == B), else runs of rows. The
+ * exponent of a page and head is the least of -32 .. 8 with |x| <= 448 * 2^k for the values written to its positions so far (writing
+ * a page's first position begins anew); values are rounded once, to nearest, k as fp32 after its rotation. Where it grows, the
+ * page's earlier positions are moved to it. Beyond +-61440 values become that, NaN stays NaN. Rows append: positions of a page behind
+ * the last one written are not kept, and a page that is written belongs to one sequence. */
+int hi_rope_cache_paged8(void* qkv, int ldq, void* q_out, int ldqo, int M, int Hq, int Hkv, int D, const void* cs,
+                         int cs_rows, int cs_f32, int rot, int interleaved, const int* start, const int* pos, void* kp,
+                         void* vp, void* kexp, void* vexp, long long page_stride, int pages, int page, const int* table,
+                         int ldt, int W, int B, void* stream);
+/* hi_attn_paged in all else, its work buffer (hi_attn_paged_work_bytes) too. */
+int hi_attn_paged8(const void* q, int ldq, const void* kp, const void* vp, const void* kexp, const void* vexp,
+                   long long page_stride, int pages, int page, const int* table, int ldt, int W, const int* start,
+                   const int* pos, void* out, int ldo, float* lse, int M, int B, int Hq, int Hkv, int D, void* work,
+                   size_t work_bytes, void* stream);
 /* The same for hi_attn_shared. */
 size_t hi_attn_shared_work_bytes(int B, int Hq, int Hkv, int D);
 size_t hi_attn_shared_work_bytes_max(int B, int Hq, int Hkv, int D);
