@@ -38,8 +38,21 @@ template <int D, int RG>
 struct FpSmem {
   static constexpr int kTile = kFpBKV * D / 8;                // 16-byte chunks of one K or V tile
   static constexpr int kMl = 2 * kFpStages * kTile;           // chunk index of m and l
+  static constexpr int kFlag = kMl;
   static constexpr size_t kBytes = kMl * 16 + 2 * RG * 64 * 4;
   static_assert(RG * (D / 32) * 64 * 64 <= kMl * 16, "merge fits the stages");
+};
+
+// The same for tiles that come as codes of 8 bits: each wave's share of the next K and V tile lies as codes behind the stages until it
+// is made into fp16. m and l are in the last V stage's bytes then, behind the accumulators.
+template <int D, int RG>
+struct Fp8Smem {
+  static constexpr int kTile = kFpBKV * D / 8;
+  static constexpr int kMl = (2 * kFpStages - 1) * kTile;
+  static constexpr int kFlag = kMl + kTile / 2;               // (the prologue has codes in the first half)
+  static constexpr int kRaw = 2 * kFpStages * kTile;          // chunk index of the K codes; the V codes follow
+  static constexpr size_t kBytes = (kRaw + kTile) * 16;
+  static_assert(RG * (D / 32) * 64 * 64 <= kMl * 16 && 2 * RG * 64 * 4 <= kTile * 16, "merge fits the stages");
 };
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));

@@ -4,7 +4,9 @@
 //   lane, fr, fk, kh, qf, scale_log2             the lane's place and its Q fragments
 //   nt, n_full                                   key tiles, and how many at the front hold no masked key for this wave
 //   issue_k(i, st), issue_v(i, st)               DMA instruction i of the next K (V) tile into stage st
-//   advance()                                    called once before the DMA of each K tile but the first
+//   kSpread                                      whether issue_k and issue_v do something: they are called between the MFMAs
+//   advance(st)                                  called once before the DMA of each K tile (into stage st) but the first: ahead
+//                                                of the others by first_advance()
 //   before_barrier(), after_barrier()            called around the prologue's barrier, before n_full is read
 //   kGuard, odd_tile                             whether infinities and NaN in V are taken out of masked tiles, and the first
 //                                                tile where any were (INT_MAX)
@@ -121,7 +123,7 @@
     wait_lgkm0();
     wait_vmcnt<0>();     // this wave's shares of K tile t + 1 and V tile t are in LDS
     barrier_no_fence();  // every share is, and every wave is done with K tile t and V tile t - 1
-    advance();
+    advance(st);
     if constexpr (MASK) {
       enter_masked(t);
 #pragma unroll
@@ -139,18 +141,18 @@
     // slots of the first logits block; with 4 waves, each issuing twice as many and without a second
     // wave on its SIMD to fill its stalls, over all of them (64 rows after 2000 positions 26.1 ->
     // 22.6 us, 512 after 2048 36.0 -> 32.7; 8 waves: no gain, 2 % slower at T = 2048 after 4096).
-    constexpr int ND = 2 * IPW, LA = 3;  // DMA instructions, LDS reads ahead of their MFMA
+    constexpr int ND = kSpread ? 2 * IPW : 0, LA = 3;  // DMA instructions, LDS reads ahead of their MFMA
     constexpr int S0 = RG == 2 ? 0 : 2 * DT, NS = RG == 2 ? 2 * DT + 2 * NQ : NQ;
     auto dma_here = [](int m) constexpr {  // DMA instructions that go before slot m
       int n = 0;
-      for (int j = 0; j < ND; j++) n += S0 + j * NS / ND == m;
+      for (int j = 0; j < ND; j++) n += S0 + j * NS / (ND ? ND : 1) == m;
       return n;
     };
     constexpr int kDma = (ND + NS - 1) / NS;  // at most this many before one slot
     auto dma = [&](int m) {
 #pragma unroll
       for (int j = 0; j < ND; j++)
-        if (S0 + j * NS / ND == m) j < IPW ? issue_k(j, st) : issue_v(j - IPW, st ^ 1);
+        if (S0 + j * NS / (ND ? ND : 1) == m) j < IPW ? issue_k(j, st) : issue_v(j - IPW, st ^ 1);
     };
     auto load_k = [&](int kt, int ks) {
       return __builtin_bit_cast(f16x8, ks_[(st ^ 1) * Sm::kTile + (kr + 32 * kt) * CPR + ((2 * ks + fk) ^ ksw)]);
@@ -256,7 +258,7 @@
   // ---- prologue: K tiles 0 and 1 and V tile 0 in flight, the logits of tile 0
 #pragma unroll
   for (int i = 0; i < IPW; i++) issue_k(i, 0);
-  advance();
+  first_advance();
 #pragma unroll
   for (int i = 0; i < IPW; i++) {
     issue_v(i, 0);
@@ -290,7 +292,7 @@
       wait_lgkm0();
       wait_vmcnt<0>();
       barrier_no_fence();
-      advance();
+      advance(t & 1);
 #pragma unroll
       for (int i = 0; i < IPW; i++) {
         issue_k(i, t & 1);

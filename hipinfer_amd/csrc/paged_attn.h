@@ -210,13 +210,13 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
   constexpr int NG = KPW / 8;                  // in groups of 8, one page each
   constexpr int IPG = IPW / NG;                // DMA instructions per group
   static_assert(IPW * 64 * NW == kFpBKV * CPR && IPG * NG == IPW, "tile DMA split");
-  using Sm = FpSmem<D, RG>;
+  using Sm = typename std::conditional<C::kF8, Fp8Smem<D, RG>, FpSmem<D, RG>>::type;
   extern __shared__ u32x4 fp_smem[];
   u32x4* const ks_ = fp_smem;                                // [2][kTile]: K stages
   u32x4* const vs_ = fp_smem + kFpStages * Sm::kTile;        // [2][kTile]: V stages
   f32x16* const mo = reinterpret_cast<f32x16*>(fp_smem);     // [RG][DT][64]: the merge
   float* const ml = reinterpret_cast<float*>(fp_smem + Sm::kMl);  // [2][RG][64]: the second waves' m and l
-  int* const flag = reinterpret_cast<int*>(fp_smem + Sm::kMl);    // [NW], before the loop
+  int* const flag = reinterpret_cast<int*>(fp_smem + Sm::kFlag);  // [NW], before the loop
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wave % RG, kh = wave / RG;     // row group, key half
@@ -302,74 +302,103 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<typename C::Elem*>(base) + (((uint64_t)hi << 32) | lo), (short)0, n,
                                                0x00020000);
     };
+    constexpr bool kSpread = !C::kF8;
     int koff[IPW], voff[IPW];
-    // F8: the codes of the next K and V tile that go to LDS, a group of 8 keys in each, and their scales (vscale2: of the V tile after it)
-    constexpr int RL = C::kF8 ? NG : 1;
-    u32x4 kcode[RL], vcode[RL];
-    float kscale[RL], vscale[RL], vscale2[RL];
-    const int key8 = lane >> 3, piece = lane & 7;  // of a group: this lane's key and its D / 8 dims
-    auto scales = [&] {
-#pragma unroll
-      for (int g = 0; g < RL; g++) {
-        vscale[g] = vscale2[g];
-        kscale[g] = exponent_scale(__builtin_amdgcn_readlane(ke, g));
-        vscale2[g] = exponent_scale(__builtin_amdgcn_readlane(ve, g));
-      }
-    };
-    auto codes = [&](__amdgpu_buffer_rsrc_t rs) {
-      const int at = key8 * D + piece * (D / 8);
-      if constexpr (D == 128) {
-        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
-      } else {
-        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0));
-        return u32x4{v[0], v[1], 0u, 0u};
-      }
-    };
-    // chunk j of a group's codes as fp16 into a tile's rows
-    auto put = [&](u32x4* tile, const u32x4& w, float scale, int g, int j, auto swz) {
-      const int k = wave * KPW + 8 * g + key8;
-      const f16x8 x = j == 0 ? f8x8_to_f16(w[0], w[1], scale) : f8x8_to_f16(w[2], w[3], scale);
-      tile[k * CPR + ((IPG * piece + j) ^ swz(k))] = __builtin_bit_cast(u32x4, x);
-    };
-    auto issue_k = [&](int i, int st) {
-      if constexpr (C::kF8) {
-        const int g = i / IPG;
-        put(ks_ + st * Sm::kTile, kcode[g], kscale[g], g, i % IPG, [](int k) { return k_swz<D>(k); });
-        if (i % IPG == IPG - 1) kcode[g] = codes(group(c.kp, klo[g], khi[g], kn[g]));
-      } else {
-        lds_dma16(group(c.kp, klo[i / IPG], khi[i / IPG], kn[i / IPG]), ks_ + st * Sm::kTile + (wave * IPW + i) * 64, koff[i]);
-      }
-    };
-    auto issue_v = [&](int i, int st) {
-      if constexpr (C::kF8) {
-        const int g = i / IPG;
-        put(vs_ + st * Sm::kTile, vcode[g], vscale[g], g, i % IPG, [](int k) { return v_swz<D>(k); });
-        if (i % IPG == IPG - 1) vcode[g] = codes(group(c.vp, vlo[g], vhi[g], vn[g]));
-      } else {
-        lds_dma16(group(c.vp, vlo[i / IPG], vhi[i / IPG], vn[i / IPG]), vs_ + st * Sm::kTile + (wave * IPW + i) * 64, voff[i]);
-      }
-    };
-    auto advance = [&] {
+    auto next = [&] {
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         vlo[g] = klo[g];
         vhi[g] = khi[g];
         vn[g] = kn[g];
       }
-      if constexpr (C::kF8) scales();
       take();
       fetch();
+    };
+    auto issue_k = [&](int i, int st) {
+      if constexpr (kSpread)
+        lds_dma16(group(c.kp, klo[i / IPG], khi[i / IPG], kn[i / IPG]), ks_ + st * Sm::kTile + (wave * IPW + i) * 64, koff[i]);
+    };
+    auto issue_v = [&](int i, int st) {
+      if constexpr (kSpread)
+        lds_dma16(group(c.vp, vlo[i / IPG], vhi[i / IPG], vn[i / IPG]), vs_ + st * Sm::kTile + (wave * IPW + i) * 64, voff[i]);
+    };
+    // F8: a wave's share of a tile comes as codes (a group of 8 keys is D / 2 lanes of DMA) and is made into fp16 by the wave itself,
+    // one tile before the others read it: no barrier, and no registers held while a tile is computed. The codes' place in LDS is free
+    // again as soon as they are read.
+    constexpr int RPW = KPW * D / 1024;  // 16-byte reads of a lane per wave and operand
+    int vexps = 0;  // the exponents of the V tile that lies there as codes; the K tile's are ke
+    u32x4* const own_k = fp_smem + 2 * kFpStages * Sm::kTile + wave * RPW * 64;
+    u32x4* const own_v = own_k + Sm::kTile / 2;
+    auto codes_to = [&](const typename C::Elem* base, const uint32_t (&lo)[NG], const uint32_t (&hi)[NG], const int (&n)[NG], u32x4* to) {
+      if constexpr (C::kF8) {
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+          if (D == 128 || lane < 32) lds_dma16(group(base, lo[g], hi[g], n[g]), to + g * (D / 2), lane * 16);
+      }
+    };
+    auto widen = [&](const u32x4* from, int exps, u32x4* tile, auto swz) {
+      if constexpr (C::kF8) {
+        u32x4 w[RPW];
+#pragma unroll
+        for (int i = 0; i < RPW; i++) w[i] = from[i * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < RPW; i++) {
+          const int at = i * 64 + lane, key_at = at / (D / 16), piece = at % (D / 16), k = wave * KPW + key_at;
+          float scale;
+          if constexpr (D == 128) {
+            scale = exponent_scale(__builtin_amdgcn_readlane(exps, i));
+          } else {
+            const int e0 = __builtin_amdgcn_readlane(exps, 2 * i), e1 = __builtin_amdgcn_readlane(exps, 2 * i + 1);
+            scale = exponent_scale(lane < 32 ? e0 : e1);
+          }
+          tile[k * CPR + ((2 * piece) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][0], w[i][1], scale));
+          tile[k * CPR + ((2 * piece + 1) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][2], w[i][3], scale));
+        }
+      }
+    };
+    auto kz = [](int k) { return k_swz<D>(k); };
+    auto vz = [](int k) { return v_swz<D>(k); };
+    auto advance = [&](int st) {
+      if constexpr (C::kF8) {
+        widen(own_k, ke, ks_ + st * Sm::kTile, kz);
+        widen(own_v, vexps, vs_ + (st ^ 1) * Sm::kTile, vz);
+        vexps = ve;
+        wait_lgkm0();  // the codes are read
+        asm volatile("" ::: "memory");
+        next();
+        codes_to(c.kp, klo, khi, kn, own_k);
+        codes_to(c.vp, vlo, vhi, vn, own_v);
+      } else {
+        next();
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
+    auto first_advance = [&] {
+      if constexpr (!C::kF8) advance(0);
+    };
     if constexpr (C::kF8) {
+      // K tiles 0 and 1 and V tile 0 at once (K tile 1's codes in the last V stage, which is free until tile 0 is computed), then K tile 2's
+      // and V tile 1's codes on their way
+      u32x4* const more_k = vs_ + Sm::kTile + wave * RPW * 64;
       take();
       fetch();
-#pragma unroll
-      for (int g = 0; g < RL; g++) {
-        kcode[g] = codes(group(c.kp, klo[g], khi[g], kn[g]));
-        vcode[g] = codes(group(c.vp, klo[g], khi[g], kn[g]));
-      }
-      scales();
+      const int ke0 = ke, ve0 = ve;
+      codes_to(c.kp, klo, khi, kn, own_k);
+      codes_to(c.vp, klo, khi, kn, own_v);
+      next();
+      const int ke1 = ke, ve1 = ve;
+      codes_to(c.kp, klo, khi, kn, more_k);
+      wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      widen(own_k, ke0, ks_, kz);
+      widen(own_v, ve0, vs_, vz);
+      widen(more_k, ke1, ks_ + Sm::kTile, kz);
+      wait_lgkm0();
+      asm volatile("" ::: "memory");
+      vexps = ve1;
+      next();
+      codes_to(c.kp, klo, khi, kn, own_k);
+      codes_to(c.vp, vlo, vhi, vn, own_v);
     } else {
       // DMA instruction i of this wave fills slots (wave IPW + i) * 64 + lane of a tile: slot s holds
       // key s / CPR, physical chunk s % CPR, i.e. logical chunk (s % CPR) ^ swz(key)
@@ -379,9 +408,9 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
         koff[i] = ((r & 7) * D + 8 * (p ^ k_swz<D>(r))) * 2;
         voff[i] = ((r & 7) * D + 8 * (p ^ v_swz<D>(r))) * 2;
       }
+      take();
+      fetch();
     }
-    take();
-    fetch();
     // whether some key of the block lies on no page
     int hid[2], hi = (kb >> c.shift) + tid;
     const int h_last = (kv_end - 1) >> c.shift;
@@ -1641,7 +1670,7 @@ int flash_launch(const AttnArgs& a, const C& c, int cus, void* work, hipStream_t
   if (units > 65535 || (int64_t)a.B * plan_tiles(a.M, G, 32 * RG) > INT32_MAX)
     HI_FAIL("%s: %d rows of %d sequences are too many", who, a.M, a.B);
   const auto kern = attn_pages_kernel<D, RG, C>;
-  const size_t lds = FpSmem<D, RG>::kBytes;
+  const size_t lds = C::kF8 ? Fp8Smem<D, RG>::kBytes : FpSmem<D, RG>::kBytes;
   if (const int rc = flash_fits(kern, 128 * RG, lds, who)) return rc;
   hipLaunchKernelGGL(kern, dim3(a.Hkv, (unsigned)units), dim3(128 * RG), lds, s, a, c, f);
   HI_TRY(hipGetLastError());

@@ -133,7 +133,9 @@ __global__ void __launch_bounds__(128 * RG)
   auto enter_masked = [](int) {};
   constexpr bool kGuard = false;
   int odd_tile = 0;
-  auto advance = [] {};
+  constexpr bool kSpread = true;
+  auto advance = [](int) {};
+  auto first_advance = [] {};
   auto before_barrier = [] {};
   auto after_barrier = [] {};
   auto live = [&](int t) {
