@@ -17,8 +17,11 @@ namespace {
 constexpr int kSeg = 512;         // logits of a segment: a wave's 16-byte loads
 constexpr int kSegs = 4;          // segments of a wave
 constexpr int kMaxBeams = 64, kMaxBest = 64;
-constexpr int kPick = 256;        // threads of the second kernel
+constexpr int kPick = 1024;       // threads of the second kernel
+constexpr int kGroups = 64;       // of them, for a bound on the n-th best segment: at least n
+constexpr int kAhead = 4;         // segments that a thread has in registers
 constexpr int kList = 2048;       // candidates that are ranked in LDS
+constexpr float kSlack = 1 + 0x1p-19f;  // more than fp32 distances are off by
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint64_t kNone = ~0ull;
 
@@ -97,11 +100,12 @@ __device__ __forceinline__ double wave_sum64(double v) {
 struct PickSmem {
   double base[kMaxBeams];   // scores[k] - log sum; NaN for a beam without candidates
   float top[kMaxBeams];     // the beam's largest logit
-  uint64_t best[kPick];
+  float far[kMaxBeams];     // how far its best candidate is from the best of all; infinite without candidates
+  float best[kGroups];
   uint64_t list[kList];
   uint64_t out[kMaxBest];   // the n least keys in order
   uint64_t red[kPick / 64];
-  uint64_t limit;
+  float limit;
   int found;
 };
 
@@ -111,35 +115,26 @@ __device__ __forceinline__ uint64_t key_of(double d, uint32_t at) {
   const uint64_t b = (uint64_t)__builtin_bit_cast(int64_t, 1.0 + d) - 0x3ff0000000000000ull;
   return (b >> 17) << 24 | at;
 }
+// No distance whose key is that of d or less exceeds this.
+__device__ __forceinline__ float limit_of(uint64_t key) {
+  const double d = __builtin_bit_cast(double, (int64_t)((((key >> 24) + 1) << 17) + 0x3ff0000000000000ull)) - 1.0;
+  return (float)d * kSlack;
+}
 
-// The n least of the block's keys, in order, into sh.out (kNone behind the last). each(f) calls f with every key of the thread, the
-// same ones every time; keys are unique but for kNone.
-template <typename Each>
-__device__ __forceinline__ void least_keys(PickSmem& sh, int n, Each each) {
+// The n least of the block's keys, in order, into sh.out (kNone behind the last); keys are unique but for kNone. push(f) calls f with
+// a few keys of the thread, the n least of all among them; all(f) with every one. The few are ranked in LDS; where they are too many
+// for it (thousands of equal logits), all are gone through n times.
+template <typename Push, typename All>
+__device__ __forceinline__ void least_keys(PickSmem& sh, int n, Push push, All all) {
   const int tid = threadIdx.x;
-  uint64_t mine = kNone;
-  each([&](uint64_t k) { mine = k < mine ? k : mine; });
-  sh.best[tid] = mine;
   if (tid < n) sh.out[tid] = kNone;
-  if (tid == 0) {
-    sh.limit = kNone - 1;  // with fewer than n threads that have any, all keys that are any
-    sh.found = 0;
-  }
+  if (tid == 0) sh.found = 0;
   __syncthreads();
-  // the n-th least of the threads' least keys bounds the n-th least of all
-  int before = 0;
-#pragma unroll 16
-  for (int t = 0; t < kPick; t++) before += sh.best[t] < mine;
-  if (before == n - 1 && mine != kNone) sh.limit = mine;
-  __syncthreads();
-  const uint64_t limit = sh.limit;
-  if (mine <= limit)
-    each([&](uint64_t k) {
-      if (k <= limit) {
-        const int at = atomicAdd(&sh.found, 1);
-        if (at < kList) sh.list[at] = k;
-      }
-    });
+  push([&](uint64_t k) {
+    if (k == kNone) return;
+    const int at = atomicAdd(&sh.found, 1);
+    if (at < kList) sh.list[at] = k;
+  });
   __syncthreads();
   const int found = sh.found;
   if (found <= kList) {
@@ -152,11 +147,10 @@ __device__ __forceinline__ void least_keys(PickSmem& sh, int n, Each each) {
     __syncthreads();
     return;
   }
-  // so many at or before the bound (thousands of equal logits): one after the other
   uint64_t last = 0;
   for (int j = 0; j < n; j++) {
     uint64_t k = kNone;
-    each([&](uint64_t v) {
+    all([&](uint64_t v) {
       if ((j == 0 || v > last) && v < k) k = v;
     });
 #pragma unroll
@@ -174,7 +168,10 @@ __device__ __forceinline__ void least_keys(PickSmem& sh, int n, Each each) {
   }
 }
 
-// One block per sequence.
+// One block per sequence. What is compared for every segment and logit is the fp32 distance from the best, far[k] + (top[k] - x), off
+// by 2^-22 of it at most; the keys of 64 bits are made for those alone that can be among the n best by it:
+//  * of the segments, those up to the n-th least of 64 groups' least distances (at least n segments are that near);
+//  * of their logits, those up to the n-th segment's best one (the segments' best ones are n that near).
 template <bool WIDE>
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict__ logits, int64_t ldl, const float* __restrict__ scores,
                                                           int V, int R, int K, int n, const char* work, float* best, int* parent,
@@ -182,12 +179,16 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict_
   __shared__ PickSmem sh;
   __shared__ uint32_t seg[kMaxBest];  // the places of the first logits of the picked segments
   const BeamWork w(R, V);
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const f16* const most = (const f16*)work + (int64_t)b * K * w.segs;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = K * w.segs;
+  const f16* const most = (const f16*)work + (int64_t)b * S;
   const float* const pairs = (const float*)(work + w.pairs) + 2 * (int64_t)b * K * w.waves;
+  f16 x0[kAhead];  // the thread's first segments, requested ahead of the sums
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) x0[j] = tid + j * kPick < S ? most[tid + j * kPick] : (f16)0.f;
   // ---- the beams' log sums
   for (int k = wave; k < K; k += kPick / 64) {
     const float* p = pairs + 2 * (int64_t)k * w.waves;
+    const double s = (double)scores[b * K + k];
     float M = -__builtin_huge_valf();
     for (int i = lane; i < w.waves; i += 64) M = fmaxf(M, p[2 * i]);
     M = wave_max(M);
@@ -195,45 +196,83 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict_
     for (int i = lane; i < w.waves; i += 64) sum += (double)p[2 * i + 1] * exp((double)p[2 * i] - (double)M);
     sum = wave_sum64(sum);
     if (lane == 0) {
-      const double s = (double)scores[b * K + k];
       sh.top[k] = M;
       sh.base[k] = s - s == 0.0 && M - M == 0.f && sum - sum == 0.0 ? s - log(sum) : __builtin_nan("");  // none of them infinite
     }
   }
   __syncthreads();
-  auto score = [&](int k, float x) { return ((double)x - (double)sh.top[k]) + sh.base[k]; };
   double top = -__builtin_huge_val();
   for (int k = 0; k < K; k++)
     if (sh.base[k] > top) top = sh.base[k];  // a beam's best candidate is its largest logit
+  if (tid < K) sh.far[tid] = sh.base[tid] <= top ? (float)(top - sh.base[tid]) : __builtin_huge_valf();
+  __syncthreads();
+  auto key = [&](int k, float x, int t) {
+    return key_of(top - (((double)x - (double)sh.top[k]) + sh.base[k]), (uint32_t)(k * V + t));
+  };
+  auto far = [&](int k, float x) { return sh.far[k] + (sh.top[k] - x); };
   // ---- the n best segments
-  least_keys(sh, n, [&](auto f) {
-    for (int i = tid; i < K * w.segs; i += kPick) {
-      const int k = i / w.segs;
-      f(key_of(top - score(k, (float)most[i]), (uint32_t)(k * V + (i - k * w.segs) * kSeg)));
+  auto segments = [&](auto f) {  // f(beam, segment, its largest logit)
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int i = tid + j * kPick;
+      if (i < S) f(i / w.segs, i % w.segs, (float)x0[j]);
     }
-  });
+    for (int i = tid + kAhead * kPick; i < S; i += kPick) f(i / w.segs, i % w.segs, (float)most[i]);
+  };
+  float near = __builtin_huge_valf();
+  segments([&](int k, int, float x) { near = fminf(near, far(k, x)); });
+  constexpr int kLanes = kPick / kGroups;  // of a group
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) near = fminf(near, __shfl_xor(near, o, 64));
+  if ((tid & (kLanes - 1)) == 0) sh.best[tid / kLanes] = near;
+  if (tid == 0) sh.limit = __builtin_huge_valf();
+  __syncthreads();
+  int before = 0, group = tid / kLanes;
+#pragma unroll
+  for (int g = 0; g < kGroups; g++) before += sh.best[g] < near || (sh.best[g] == near && g < group);
+  if (before == n - 1) sh.limit = near * kSlack + 0x1p-34f;  // (infinite with fewer than n groups that have any)
+  __syncthreads();
+  const float limit = sh.limit;
+  least_keys(
+      sh, n,
+      [&](auto f) {
+        segments([&](int k, int s, float x) {
+          if (far(k, x) <= limit) f(key(k, x, s * kSeg));
+        });
+      },
+      [&](auto f) { segments([&](int k, int s, float x) { f(key(k, x, s * kSeg)); }); });
   if (tid < n) seg[tid] = sh.out[tid] == kNone ? ~0u : (uint32_t)sh.out[tid] & 0xffffff;
+  const uint64_t nth = sh.out[n - 1];
+  const float cut = nth == kNone ? __builtin_huge_valf() : limit_of(nth);
   __syncthreads();
   // ---- the n best candidates in them
-  least_keys(sh, n, [&](auto f) {
+  auto chunks = [&](auto f) {  // f(beam, logit, token)
     for (int i = tid; i < n * (kSeg / 8); i += kPick) {
       const uint32_t first = seg[i / (kSeg / 8)];
       if (first == ~0u) continue;
       const int k = first / V, t = first - k * V + i % (kSeg / 8) * 8;
       const f16x8 x = load8<WIDE>(logits + ((int64_t)b * K + k) * ldl, V, t);
 #pragma unroll
-      for (int e = 0; e < 8; e++) f(key_of(top - score(k, (float)x[e]), (uint32_t)(k * V + t + e)));
+      for (int e = 0; e < 8; e++) f(k, (float)x[e], t + e);
     }
-  });
+  };
+  least_keys(
+      sh, n,
+      [&](auto f) {
+        chunks([&](int k, float x, int t) {
+          if (far(k, x) <= cut) f(key(k, x, t));
+        });
+      },
+      [&](auto f) { chunks([&](int k, float x, int t) { f(key(k, x, t)); }); });
   if (tid < n) {
-    const uint64_t key = sh.out[tid];
+    const uint64_t q = sh.out[tid];
     float s = -__builtin_huge_valf();
     int k = -1, t = -1;
-    if (key != kNone) {
-      const int at = (int)(key & 0xffffff);
+    if (q != kNone) {
+      const int at = (int)(q & 0xffffff);
       k = at / V;
       t = at - k * V;
-      s = (float)score(k, (float)logits[((int64_t)b * K + k) * ldl + t]);
+      s = (float)(((double)logits[((int64_t)b * K + k) * ldl + t] - (double)sh.top[k]) + sh.base[k]);
       k += b * K;
     }
     best[b * n + tid] = s;

@@ -38,6 +38,15 @@ struct PagedCache8 {
 
 // 2^e as a float for a stored exponent (-128 and -127, which no float has: 2^-126).
 __device__ __forceinline__ float exponent_scale(int e) { return __builtin_bit_cast(float, (max(e, -126) + 127) << 23); }
+// 2 of 4 codes as fp16 values, the lower or the upper two.
+__device__ __forceinline__ uint32_t f8x2_to_f16(uint32_t w, int upper, float scale) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return upper ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))
+               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+#else
+  return 0;
+#endif
+}
 // 4 codes as fp16 values: the product of code and scale rounded once (exact unless it is subnormal or overflows).
 __device__ __forceinline__ void f8x4_to_f16(uint32_t w, float scale, f16x2& lo, f16x2& hi) {
 #if defined(__HIP_DEVICE_COMPILE__)

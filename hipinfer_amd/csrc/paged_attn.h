@@ -682,6 +682,10 @@ struct PageFrags<D, PagedCache> {
 #pragma unroll
     for (int i = 0; i < 8; i++) out[i] = vr[i];
   }
+  // V row i's dims 2 n and 2 n + 1 (of the lane's DL) as two fp16, and row i made zero
+  __device__ __forceinline__ float v_scale() const { return 1.f; }
+  __device__ __forceinline__ uint32_t v2(int i, int n, float) const { return vr[i][n]; }
+  __device__ __forceinline__ void clear_v(int i) { vr[i] = VT{}; }
 };
 template <int D>
 struct PageFrags<D, PagedCache8> {
@@ -709,6 +713,14 @@ struct PageFrags<D, PagedCache8> {
     const u32x4 w = kr[x][s >> 1];
     return s & 1 ? f8x8_to_f16(w[2], w[3], scale) : f8x8_to_f16(w[0], w[1], scale);
   }
+  __device__ __forceinline__ float v_scale() const { return exponent_scale(ve); }
+  __device__ __forceinline__ uint32_t v2(int i, int n, float scale) const {
+    uint32_t w;
+    if constexpr (D == 128) w = vr[i][n >> 1];
+    else w = vr[i];
+    return f8x2_to_f16(w, n & 1, scale);
+  }
+  __device__ __forceinline__ void clear_v(int i) { vr[i] = VR{}; }
   __device__ __forceinline__ void v(VT (&out)[8]) const {
     const float scale = exponent_scale(ve);
 #pragma unroll
@@ -879,21 +891,25 @@ __device__ __forceinline__ void step_block(const AttnArgs& a, const C& c, const 
       for (int n = 0; n < DL; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) o[n][i] *= alpha;
-      typename Fr::VT vf[8];
-      kv.v(vf);
       if constexpr (MASK) {
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          if (!(was && t0 + vg + k < end)) vf[k] = typename Fr::VT{};
+          if (!(was && t0 + vg + k < end)) kv.clear_v(k);
       }
+      const float vs = kv.v_scale();
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = 0; n < DL; n++) {
-        u32x4 w;
+      for (int n2 = 0; n2 < DL / 2; n2++) {
+        uint32_t v2[8];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          w[k] = __builtin_amdgcn_perm(vf[2 * k + 1][n >> 1], vf[2 * k][n >> 1], n & 1 ? 0x07060302u : 0x05040100u);
-        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), ph, o[n], 0, 0, 0);
+        for (int k = 0; k < 8; k++) v2[k] = kv.v2(k, n2, vs);
+#pragma unroll
+        for (int n = 2 * n2; n < 2 * n2 + 2; n++) {
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[k] = __builtin_amdgcn_perm(v2[2 * k + 1], v2[2 * k], n & 1 ? 0x07060302u : 0x05040100u);
+          o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), ph, o[n], 0, 0, 0);
+        }
       }
       if constexpr (!LAST) {
         __builtin_amdgcn_sched_barrier(0);

@@ -17,7 +17,9 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPerThread = 16;      // pages that a thread of a plan looks at in one step
 constexpr int kMaxRows = 8192;      // rows of a table: the plan keeps 12 bytes a row in LDS
 constexpr int kSetMax = 128;        // cache tensors of one launch: their addresses are kernel arguments (3 KB)
-constexpr int kPart = 16384;        // bytes of a page that a block copies at a time
+constexpr int kPart = 4096;         // bytes of a page that a wave copies at a time: 4 loads of 16 bytes a lane
+constexpr int kSmall = 64;          // pages of at most so many bytes are copied by a lane
+constexpr int kListed = 4096;       // free pages that a plan keeps in LDS
 
 // One cache tensor: pages `stride` bytes apart. A page's `bytes` are `runs` runs of one value per position, or with runs 0
 // belong to the page as a whole.
@@ -28,8 +30,8 @@ struct CacheDesc {
   uint32_t runs_unit;  // runs << 5 | bytes of an access (16, 4 or 1)
 };
 struct CacheSet {
-  CacheDesc d[kSetMax];
-  int n, parts;  // tensors, and parts of kPart bytes that the largest page has
+  CacheDesc d[kSetMax];  // those with pages of over kSmall bytes first
+  int n, large, parts;   // tensors, the large ones, and parts of kPart bytes that the largest page has
 };
 
 // A copy of page src to page dst, of the first `rows` positions (a whole page: `page` of them).
@@ -127,6 +129,11 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   int* const count = lds;            // [S] children
   int* const first = lds + a.S;      // [S] the first of them
   int* const fresh = first + a.S;    // [N] fresh pages
+  int* const source = fresh + a.N;   // [N] page to be copied, or -1
+  int* const near = source + a.N;    // [kListed] the first free pages
+  const bool wide = ((uintptr_t)a.refs & 15) == 0;
+  int r[kPerThread];  // (requested ahead of all that comes before their use)
+  load_counts(a.refs, a.pages, tid * kPerThread, wide, r);
   for (int r = tid; r < a.S; r += kPlanThreads) {
     count[r] = 0;
     first[r] = INT_MAX;
@@ -154,14 +161,19 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     const int p = i < a.N ? a.parent_of(i) : -1;
     const int n = p >= 0 ? a.len(p) : 0, full = n >> a.shift, need = p >= 0 ? a.need(n) : 0;
     const bool heir = p >= 0 && first[p] == i;
+    const int rows = n & (a.page - 1);
     int rank = 0;
+    if (sub == 0 && i < a.N) source[i] = -1;
     for (int j0 = full; __any(j0 < need); j0 += per) {
       const int j = j0 + sub;
       bool take = j < need;
       int keep = -1;
-      if (take && heir) {
+      if (take && (heir || (j == full && rows > 0))) {
         const int e = a.table[(int64_t)p * a.ldt + j];
-        if (a.has(e) && a.refs[e] == 1) keep = e;
+        if (a.has(e)) {
+          if (heir && a.refs[e] == 1) keep = e;
+          else if (j == full && rows > 0) source[i] = e;  // (the row's lane 0, as above)
+        }
       }
       const uint64_t all = __ballot(take && keep < 0);
       if (take) a.table_out[(int64_t)i * a.ldo + j] = keep >= 0 ? keep : -2 - (rank + __popcll(all & below));
@@ -182,10 +194,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   }
   // the first T free pages
   int* const list = (int*)(a.work + w.list);
-  const bool wide = ((uintptr_t)a.refs & 15) == 0;
   int found = 0;
-  int r[kPerThread];
-  if (T > 0) load_counts(a.refs, a.pages, tid * kPerThread, wide, r);
   for (int p0 = 0; p0 < a.pages && found < T; p0 += kPlanThreads * kPerThread) {
     const int mine = p0 + tid * kPerThread;
     int free = 0;
@@ -200,7 +209,10 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     while (which) {
       const int k = __ffs(which) - 1;
       which &= which - 1;
-      if (at < T) list[at] = mine + k;
+      if (at < T) {
+        list[at] = mine + k;
+        if (at < kListed) near[at] = mine + k;
+      }
       at++;
     }
     found += total;
@@ -213,18 +225,12 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   for (int i0 = 0; i0 < a.N; i0 += kPlanThreads) {
     const int i = i0 + tid;
     Move m{-1, -1, 0};
-    if (i < a.N) {
-      const int p = a.parent_of(i);
-      if (p >= 0) {
-        const int n = a.len(p), full = n >> a.shift, at = ((int*)(a.work + w.base))[i];
-        m.rows = n & (a.page - 1);
-        if (m.rows > 0 && full < a.need(n) && at < found) {
-          const int e = a.table[(int64_t)p * a.ldt + full];
-          if (a.has(e) && !(first[p] == i && a.refs[e] == 1)) {
-            m.src = e;
-            m.dst = __hip_atomic_load(list + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          }
-        }
+    if (i < a.N && source[i] >= 0) {  // the row's first fresh page
+      const int at = ((int*)(a.work + w.base))[i];
+      if (at < found) {
+        m.src = source[i];
+        m.dst = at < kListed ? near[at] : __hip_atomic_load(list + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        m.rows = a.len(a.parent_of(i)) & (a.page - 1);
       }
     }
     int total;
@@ -238,11 +244,11 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   }
 }
 
-// Units [lo, hi) of those that a move copies of one tensor: of each run of `run` units the first `take`.
+// By a wave: units [lo, hi) of those that a move copies of one tensor, of each run of `run` units the first `take`.
 template <typename T>
 __device__ __forceinline__ void copy_units(char* dst, const char* src, uint32_t lo, uint32_t hi, uint32_t run, uint32_t take) {
   constexpr int U = 4;
-  const uint32_t r0 = lo / take, in0 = lo - r0 * take;
+  const uint32_t lane = threadIdx.x & 63, r0 = lo / take, in0 = lo - r0 * take;
   const T* const s = (const T*)src + (size_t)r0 * run;
   T* const d = (T*)dst + (size_t)r0 * run;
   const float inv = 1.0f / (float)take;
@@ -251,22 +257,22 @@ __device__ __forceinline__ void copy_units(char* dst, const char* src, uint32_t 
     uint32_t q = in0 + kPart < 1u << 22 ? (uint32_t)((float)at * inv) : at / take;  // off by one at most
     if (q * take > at) q--;
     if (at - q * take >= take) q++;
-    return (size_t)q * run + (at - q * take);
+    return q * run + (at - q * take);
   };
   const uint32_t n = hi - lo;
-  for (uint32_t i = threadIdx.x; i < n; i += U * 256) {
+  for (uint32_t i = lane; i < n; i += U * 64) {
     T v[U];
-    size_t at[U];
+    uint32_t at[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (i + u * 256 < n) v[u] = s[at[u] = place(i + u * 256)];
+      if (i + u * 64 < n) v[u] = s[at[u] = place(i + u * 64)];
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (i + u * 256 < n) d[at[u]] = v[u];
+      if (i + u * 64 < n) d[at[u]] = v[u];
   }
 }
 
-// Part `part` of tensor d's share of a move.
+// By a wave: part `part` of tensor d's share of a move.
 __device__ __forceinline__ void copy_part(const CacheDesc& d, const Move& m, int page, int part) {
   const uint32_t unit = d.runs_unit & 31, runs = d.runs_unit >> 5;
   const bool whole = runs == 0 || m.rows == page;
@@ -282,24 +288,61 @@ __device__ __forceinline__ void copy_part(const CacheDesc& d, const Move& m, int
   else copy_units<uint8_t>(dst, src, lo, hi, run, take);
 }
 
-// All tensors' parts of n moves, block by block.
-__device__ __forceinline__ void copy_moves(const CacheSet& c, const Move* moves, int n, int page, int block, int blocks) {
-  const int each = c.n * c.parts;
+// By a lane: tensor d's share of a move, of kSmall bytes at most.
+__device__ __forceinline__ void copy_small(const CacheDesc& d, const Move& m, int page) {
+  const uint32_t runs = d.runs_unit >> 5, run = runs ? d.bytes / runs : d.bytes, take = runs ? run / page * m.rows : run;
+  const char* const src = d.p + (int64_t)m.src * d.stride;
+  char* const dst = d.p + (int64_t)m.dst * d.stride;
+  if (take == run && (d.runs_unit & 31) >= 4) {
+    for (uint32_t i = 0; i < d.bytes; i += 4) *(uint32_t*)(dst + i) = *(const uint32_t*)(src + i);
+    return;
+  }
+  for (uint32_t r = 0; r < d.bytes; r += run)
+    for (uint32_t i = 0; i < take; i++) dst[r + i] = src[r + i];
+}
+
+// All tensors' shares of n moves, by `waves` waves of which this is number `wave`. The large ones' parts are a wave's: 4 KB each in
+// flight on every wave of the GPU (2475 moves of 28 layers' pages of 2 x 4 KB 353 us by blocks of 16 KB).
+__device__ __forceinline__ void copy_moves(const CacheSet& c, const Move* moves, int n, int page, int wave, int waves) {
+  const int each = c.large * c.parts;
   const int64_t items = (int64_t)n * each;
-  for (int64_t i = block; i < items; i += blocks) {
-    const int m = items <= INT_MAX ? (int)i / each : (int)(i / each), rest = (int)(i - (int64_t)m * each), t = rest / c.parts;
-    copy_part(c.d[t], moves[m], page, rest - t * c.parts);
+  auto split = [&](int64_t i, int& m) {
+    m = items <= INT_MAX ? (int)i / each : (int)(i / each);
+    return (int)(i - (int64_t)m * each);
+  };
+  if (wave < items) {
+    int m, rest = split(wave, m);
+    Move move = moves[m];
+    for (int64_t i = wave;;) {
+      const Move now = move;
+      const int t = rest / c.parts, part = rest - t * c.parts;
+      i += waves;
+      const bool more = i < items;
+      if (more) {
+        rest = split(i, m);
+        move = moves[m];
+      }
+      copy_part(c.d[t], now, page, part);
+      if (!more) break;
+    }
+  }
+  const int small = c.n - c.large;
+  for (int64_t i = (int64_t)wave * 64 + (threadIdx.x & 63); i < (int64_t)n * small; i += (int64_t)waves * 64) {
+    const int m = (int)(i / small);
+    copy_small(c.d[c.large + (int)(i - (int64_t)m * small)], moves[m], page);
   }
 }
 
+__device__ __forceinline__ int wave_of(int block) { return 4 * block + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // Blocks 0 .. N - 1 write the new rows, the next S account for what the old ones held, the others copy.
-__global__ void __launch_bounds__(256) fork_apply_kernel(ForkArgs a, CacheSet c, bool rows) {
+__global__ void __launch_bounds__(256, 8) fork_apply_kernel(ForkArgs a, CacheSet c, bool rows) {
   const WorkLayout w(a.S, a.N, a.pages);
   const PlanHead* head = (const PlanHead*)a.work;
   const int tid = threadIdx.x, lead = rows ? a.N + a.S : 0;
   int x = blockIdx.x;
   if (x >= lead) {
-    copy_moves(c, (const Move*)(a.work + w.moves), head->moves, a.page, x - lead, gridDim.x - lead);
+    copy_moves(c, (const Move*)(a.work + w.moves), head->moves, a.page, wave_of(x - lead), 4 * (gridDim.x - lead));
     return;
   }
   if (x < a.N) {
@@ -364,24 +407,35 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs 
   }
   int U;
   block_scan(used, sh, U);
+  const bool once = a.pages <= kStep;  // the counts are still there
   int out = 0, in = 0;  // pages to be moved, and places for them
   for (int p0 = 0; p0 < a.pages; p0 += kStep) {
     const int mine = p0 + tid * kPerThread;
     uint32_t moving = 0, hole = 0;
     if (mine < a.pages) {
-      load_counts(a.refs, a.pages, mine, wide, r);
+      if (!once) load_counts(a.refs, a.pages, mine, wide, r);
 #pragma unroll
       for (int k = 0; k < kPerThread; k++) {
         const int p = mine + k;
         if (p >= a.pages) continue;
         const bool u = r[k] > 0;
         if (u && p >= U) moving |= 1u << k;
-        else a.moved[p] = u ? p : -1;
         if (!u && p < U) hole |= 1u << k;
+        r[k] = u ? p : -1;  // (of a page that moves: written again below)
+      }
+      if (((uintptr_t)a.moved & 15) == 0 && mine + kPerThread <= a.pages) {
+#pragma unroll
+        for (int k = 0; k < kPerThread; k += 4)
+          *reinterpret_cast<u32x4*>(a.moved + mine + k) = u32x4{(uint32_t)r[k], (uint32_t)r[k + 1], (uint32_t)r[k + 2], (uint32_t)r[k + 3]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < kPerThread; k++)
+          if (mine + k < a.pages) a.moved[mine + k] = r[k];
       }
     }
-    int n_out, n_in;
-    int at_out = out + block_scan(__popc(moving), sh, n_out), at_in = in + block_scan(__popc(hole), sh, n_in);
+    int both;  // (at most 2^14 of either in a step)
+    const int at = block_scan(__popc(moving) << 16 | __popc(hole), sh, both), n_out = both >> 16, n_in = both & 0xffff;
+    int at_out = out + (at >> 16), at_in = in + (at & 0xffff);
     for (; moving; moving &= moving - 1)
       __hip_atomic_store(&moves[at_out++].src, mine + __ffs(moving) - 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (; hole; hole &= hole - 1)
@@ -402,11 +456,11 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs 
 }
 
 // `lead` blocks rename the table's entries and move the counts, the others copy.
-__global__ void __launch_bounds__(256) compact_apply_kernel(CompactArgs a, CacheSet c, int lead) {
+__global__ void __launch_bounds__(256, 8) compact_apply_kernel(CompactArgs a, CacheSet c, int lead) {
   const WorkLayout w(a.S, 0, a.pages);
   const PlanHead* head = (const PlanHead*)a.work;
   if ((int)blockIdx.x >= lead) {
-    copy_moves(c, (const Move*)(a.work + w.moves), head->moves, a.page, blockIdx.x - lead, gridDim.x - lead);
+    copy_moves(c, (const Move*)(a.work + w.moves), head->moves, a.page, wave_of(blockIdx.x - lead), 4 * (gridDim.x - lead));
     return;
   }
   const int64_t entries = (int64_t)a.S * a.W;
@@ -427,18 +481,22 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(CompactArgs a, Cache
 int cache_set(const char* who, void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
               int pages, int t0, CacheSet& c) {
   c.n = min(n - t0, kSetMax);
+  c.large = 0;
   c.parts = 1;
-  for (int k = 0; k < c.n; k++) {
-    const long long b = bytes[t0 + k], st = strides[t0 + k];
-    const int r = runs[t0 + k];
-    const uintptr_t p = (uintptr_t)caches[t0 + k];
-    if (!p || b < 1 || b > INT32_MAX || (pages > 1 && st < b) || r < 0 || r >= 1 << 26 || (r && b % ((long long)r * page)))
-      HI_FAIL("%s: cache %d: %lld bytes a page, %lld apart, %d runs of %d positions", who, t0 + k, b, st, r, page);
-    const long long each = r ? b / ((long long)r * page) : b;  // of a position in one run
-    const uint64_t all = p | (uint64_t)(pages > 1 ? st : 0) | (uint64_t)each;
-    c.d[k] = CacheDesc{(char*)p, (int64_t)st, (uint32_t)b, (uint32_t)r << 5 | (all % 16 == 0 ? 16u : all % 4 == 0 ? 4u : 1u)};
-    c.parts = max(c.parts, (int)((b + kPart - 1) / kPart));
-  }
+  for (int pass = 0, at = 0; pass < 2; pass++)
+    for (int k = t0; k < t0 + c.n; k++) {
+      const long long b = bytes[k], st = strides[k];
+      const int r = runs[k];
+      const uintptr_t p = (uintptr_t)caches[k];
+      if (!p || b < 1 || b > INT32_MAX || (pages > 1 && st < b) || r < 0 || r >= 1 << 26 || (r && b % ((long long)r * page)))
+        HI_FAIL("%s: cache %d: %lld bytes a page, %lld apart, %d runs of %d positions", who, k, b, st, r, page);
+      if ((b <= kSmall) != (pass == 1)) continue;
+      const long long each = r ? b / ((long long)r * page) : b;  // of a position in one run
+      const uint64_t all = p | (uint64_t)(pages > 1 ? st : 0) | (uint64_t)each;
+      c.d[at++] = CacheDesc{(char*)p, (int64_t)st, (uint32_t)b, (uint32_t)r << 5 | (all % 16 == 0 ? 16u : all % 4 == 0 ? 4u : 1u)};
+      if (pass == 0) c.parts = max(c.parts, (int)((b + kPart - 1) / kPart));
+      if (pass == 0) c.large = at;
+    }
   return 0;
 }
 
@@ -467,9 +525,9 @@ int pool_check(const char* who, void* const* caches, const long long* strides, c
   return 0;
 }
 
-// Blocks that copy: what the largest number of moves needs, at most 8 a CU.
+// Blocks (of 4 waves) that copy: what the largest number of moves needs, at most 8 a CU.
 int copy_blocks(int64_t moves, const CacheSet& c, int cus) {
-  return (int)max((int64_t)1, min(moves * c.n * c.parts, (int64_t)8 * cus));
+  return (int)max((int64_t)1, min((moves * c.n * c.parts + 3) / 4, (int64_t)8 * cus));
 }
 
 }  // namespace
@@ -501,7 +559,7 @@ HI_EXPORT int hi_cache_fork(void* const* caches, const long long* strides, const
   const ForkArgs a{table, lens, parent, refs, table_out, lens_out, refs_out, missing, (char*)work, ldt, ldo, W, S, N, pages, grow,
                    page, shift};
   const int copiers = refs == refs_out ? 0 : min(d->cus, (pages + kPlanThreads - 1) / kPlanThreads);
-  const size_t lds = (size_t)(2 * S + N) * 4;
+  const size_t lds = (size_t)(2 * S + 2 * N + kListed) * 4;
   if (lds > 48 * 1024 && hi_blocks_per_cu(reinterpret_cast<const void*>(fork_plan_kernel), kPlanThreads, lds) < 1) return -2;
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), lds, s, a);
   HI_TRY(hipGetLastError());
