@@ -74,6 +74,16 @@ __device__ __forceinline__ Run run_of(const Rope8Args& a, int cap, int b) {
   return r;
 }
 
+// n entries of a cs row, 16 bytes at a time.
+template <typename CS, int n>
+__device__ __forceinline__ void load_cs(const CS* tab, CS (&t)[n]) {
+#pragma unroll
+  for (int k = 0; k < (int)(n * sizeof(CS) / 16); k++) {
+    const u32x4 w = reinterpret_cast<const u32x4*>(tab)[k];
+    __builtin_memcpy((char*)t + 16 * k, &w, 16);
+  }
+}
+
 // A K or V head's 8 elements from d on of a row, rotated for K: products of fp16 numbers are exact in fp32.
 template <typename CS, bool WIDE>
 __device__ __forceinline__ void head8(const Rope8Args& a, const f16* head, const CS* tab, int rot, int d, float (&y)[8]) {
@@ -85,11 +95,7 @@ __device__ __forceinline__ void head8(const Rope8Args& a, const f16* head, const
       for (int e = 0; e < 8; e++) y[e] = (float)x[e];
     } else if (a.inter) {
       CS t[8];
-#pragma unroll
-      for (int k = 0; k < (int)(8 * sizeof(CS) / 16); k++) {
-        const u32x4 w = reinterpret_cast<const u32x4*>(tab + d)[k];
-        __builtin_memcpy((char*)t + 16 * k, &w, 16);
-      }
+      load_cs<CS, 8>(tab + d, t);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const float u = (float)x[e], v = (float)x[e + 1], c = (float)t[e], s = (float)t[e + 1];
@@ -101,11 +107,7 @@ __device__ __forceinline__ void head8(const Rope8Args& a, const f16* head, const
       const int j = low ? d : d - half;
       const f16x8 z = *reinterpret_cast<const f16x8*>(head + (low ? d + half : j));
       CS t[16];
-#pragma unroll
-      for (int k = 0; k < (int)(16 * sizeof(CS) / 16); k++) {
-        const u32x4 w = reinterpret_cast<const u32x4*>(tab + 2 * j)[k];
-        __builtin_memcpy((char*)t + 16 * k, &w, 16);
-      }
+      load_cs<CS, 16>(tab + 2 * j, t);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const float own = (float)x[e], other = (float)z[e], c = (float)t[2 * e], s = (float)t[2 * e + 1];
@@ -131,7 +133,23 @@ __device__ __forceinline__ void head8(const Rope8Args& a, const f16* head, const
 // The q heads of row m, in pair steps that read all of what they write (in place too).
 template <typename CS, bool WIDE>
 __device__ __forceinline__ void rotate_q(const Rope8Args& a, const PagedCache8& c, int m) {
-  const int lane = threadIdx.x & 63, cap = min(c.capacity(), a.cs_rows);
+  const int lane = threadIdx.x & 63, cap = min(c.capacity(), a.cs_rows), half = a.rot / 2, D = a.D;
+  const f16* const row = a.qkv + (int64_t)m * a.ldq;
+  f16* const out = a.qo + (int64_t)m * a.ldqo;
+  // steps of 8 pairs (or 4 interleaved ones: the same 8 elements), then of 8 elements that stay; the first two are requested before
+  // the row's place is known
+  const int turns = a.rot / (a.inter ? 8 : 16), per = turns + (D - a.rot) / 8, steps = WIDE ? a.Hq * per : 0;
+  struct Step {
+    f16x8 x, z;
+  } ahead[2] = {};
+  auto load = [&](int i, Step& s) {
+    const int h = i / per, j = i - h * per, d = j < turns ? 8 * j : a.rot + 8 * (j - turns);
+    s.x = *reinterpret_cast<const f16x8*>(row + h * D + d);
+    if (!a.inter && j < turns) s.z = *reinterpret_cast<const f16x8*>(row + h * D + d + half);
+  };
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+    if ((int)threadIdx.x + 256 * k < steps) load(threadIdx.x + 256 * k, ahead[k]);
   int b = -1, p = -1;
   if (a.start) {
     for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -151,32 +169,42 @@ __device__ __forceinline__ void rotate_q(const Rope8Args& a, const PagedCache8& 
     if ((unsigned)p >= (unsigned)cap) p = -1;
   }
   if (p < 0 || !c.has(c.entry(b, p >> c.shift))) return;
-  const f16* row = a.qkv + (int64_t)m * a.ldq;
-  f16* out = a.qo + (int64_t)m * a.ldqo;
   const CS* tab = (const CS*)a.cs + (int64_t)p * a.rot;
-  const int half = a.rot / 2, D = a.D;
   if constexpr (WIDE) {
-    const int turns = a.rot / (a.inter ? 8 : 16), per = turns + (D - a.rot) / 8;
-    for (int i = threadIdx.x; i < a.Hq * per; i += 256) {
-      const int h = i / per, j = i - h * per;
-      const f16* src = row + h * D;
-      f16* dst = out + h * D;
-      if (j >= turns) {
-        const int d = a.rot + 8 * (j - turns);
-        if (src != dst) *reinterpret_cast<f16x8*>(dst + d) = *reinterpret_cast<const f16x8*>(src + d);
-        continue;
-      }
-      float y[8], z[8];
-      head8<CS, true>(a, src, tab, a.rot, 8 * j, y);
-      if (!a.inter) head8<CS, true>(a, src, tab, a.rot, 8 * j + half, z);
-      f16x8 v, w;
+    auto finish = [&](int i, Step& s) {
+      const int h = i / per, j = i - h * per, d = j < turns ? 8 * j : a.rot + 8 * (j - turns);
+      f16* const dst = out + h * D + d;
+      if (j < turns) {
+        if (a.inter) {
+          CS t[8];
+          load_cs<CS, 8>(tab + d, t);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        v[e] = (f16)y[e];
-        w[e] = (f16)z[e];
+          for (int e = 0; e < 8; e += 2) {
+            const float u = (float)s.x[e], v = (float)s.x[e + 1], cc = (float)t[e], sn = (float)t[e + 1];
+            s.x[e] = (f16)__builtin_fmaf(u, cc, -(v * sn));
+            s.x[e + 1] = (f16)__builtin_fmaf(v, cc, u * sn);
+          }
+        } else {
+          CS t[16];
+          load_cs<CS, 16>(tab + 2 * d, t);
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float u = (float)s.x[e], v = (float)s.z[e], cc = (float)t[2 * e], sn = (float)t[2 * e + 1];
+            s.x[e] = (f16)__builtin_fmaf(u, cc, -(v * sn));
+            s.z[e] = (f16)__builtin_fmaf(v, cc, u * sn);
+          }
+          *reinterpret_cast<f16x8*>(dst + half) = s.z;
+        }
       }
-      *reinterpret_cast<f16x8*>(dst + 8 * j) = v;
-      if (!a.inter) *reinterpret_cast<f16x8*>(dst + 8 * j + half) = w;
+      *reinterpret_cast<f16x8*>(dst) = s.x;
+    };
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+      if ((int)threadIdx.x + 256 * k < steps) finish(threadIdx.x + 256 * k, ahead[k]);
+    for (int i = threadIdx.x + 512; i < steps; i += 256) {
+      Step s;
+      load(i, s);
+      finish(i, s);
     }
   } else {
     for (int i = threadIdx.x; i < a.Hq * (D - half); i += 256) {  // a pair or an element each

@@ -226,7 +226,7 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
   int end;     // keys that some row of the tile sees
   int kb, ke;  // the split's
   // of the next key tile to be located: this lane's group of 8 keys, and its page
-  int key = wave * KPW + 8 * (lane & (NG - 1)), id;
+  int key = wave * KPW + 8 * (lane & (NG - 1)), id, id1 = -1;  // (id1: of the tile after it, for the 8-bit cache's prologue)
   if constexpr (PREFIX) {
     u = FlashUnit{0, 0, a.M, 0, tile, f.splits, unit, 0};
     u.slot = u.tile * f.splits;
@@ -242,6 +242,7 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
     plan_range(end, u.splits, u.split, kb, ke);
     key += kb;
     id = key < ke ? c.entry(u.b, key >> c.shift) : -1;
+    if constexpr (C::kF8) id1 = key + kFpBKV < ke ? c.entry(u.b, (key + kFpBKV) >> c.shift) : -1;
   }
   const int kv_end = min(ke, end);
   const int nt = kv_end > kb ? (kv_end - kb + kFpBKV - 1) / kFpBKV : 0;
@@ -381,7 +382,7 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       // and V tile 1's codes on their way
       u32x4* const more_k = vs_ + Sm::kTile + wave * RPW * 64;
       take();
-      fetch();
+      id = id1;
       const int ke0 = ke, ve0 = ve;
       codes_to(c.kp, klo, khi, kn, own_k);
       codes_to(c.vp, klo, khi, kn, own_v);

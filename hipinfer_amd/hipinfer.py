@@ -531,12 +531,13 @@ def rope_cache_paged(qkv, Hq, Hkv, cs, kp, vp, table, pos, seq=None, interleaved
                                      _raw_stream(gpu)), what)
 
 
-def _exponents(what, kp, kexp, vexp):
+def _exponents(what, pages, Hkv, kexp, vexp):
     """Checks the exponents of an 8-bit cache."""
-    shape = kp.shape[:2]
-    for name, t in (("kexp", kexp), ("vexp", vexp)):
-        if t.dtype is not _I8 or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"hipinfer_amd.{what}: {name} must be packed int8 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    shape = (pages, Hkv)
+    if kexp.dtype is not _I8 or vexp.dtype is not _I8 or kexp.shape != shape or vexp.shape != shape or \
+            not kexp.is_contiguous() or not vexp.is_contiguous():
+        raise ValueError(f"hipinfer_amd.{what}: kexp and vexp must be packed int8 {shape}, got {kexp.dtype} {tuple(kexp.shape)} and "
+                         f"{vexp.dtype} {tuple(vexp.shape)}")
 
 
 def rope_cache_paged8(qkv, Hq, Hkv, cs, kp, vp, kexp, vexp, table, pos, start=None, interleaved=False, q_out=None):
@@ -560,7 +561,7 @@ def rope_cache_paged8(qkv, Hq, Hkv, cs, kp, vp, kexp, vexp, table, pos, start=No
             (q_out is not None and q_out.get_device() != gpu) or gpu < 0 or gpu != _current_gpu():
         _elsewhere(what, qkv, cs, kp, vp, kexp, vexp, table, pos, start, q_out)
     cache, B, D = _paged(what, kp, vp, table, Hkv, _F8)
-    _exponents(what, kp, kexp, vexp)
+    _exponents(what, cache[3], Hkv, kexp, vexp)
     M = qkv.shape[0]
     ldq = _rows_of(what, "qkv", qkv, M, (Hq + 2 * Hkv) * D)
     cshape, wide = cs.shape, cs.dtype is _F32
@@ -658,7 +659,7 @@ def attn_paged8(q, kp, vp, kexp, vexp, table, pos, Hq, Hkv, start=None, out=None
             pos.get_device()) or gpu < 0 or gpu != _current_gpu():
         _elsewhere(what, q, kp, vp, kexp, vexp, table, pos)
     cache, M, B, D, ldq, out, ldo = _attn_args(what, q, kp, vp, table, pos, Hq, Hkv, out, lse, work, gpu, _F8)
-    _exponents(what, kp, kexp, vexp)
+    _exponents(what, cache[3], Hkv, kexp, vexp)
     if start is not None:
         _vector(what, "start", start, B + 1)
         if start.get_device() != gpu:
@@ -744,29 +745,29 @@ def cache_work(seqs, rows, pages):
     return torch.empty(size, dtype=torch.uint8, device="cuda")
 
 
-def _pool_args(what, caches, table, refs, table_out, refs_out, rows, work, others):
-    """Checks what cache_fork and cache_compact have in common; returns the row strides of table and table_out."""
-    gpu = table.get_device()
-    if gpu < 0 or gpu != _current_gpu() or any(t is not None and t.get_device() != gpu
-                                               for t in (refs, table_out, refs_out, work, *others)):
-        _elsewhere(what, table, refs, table_out, refs_out, work, *others)
-    if not isinstance(caches, CacheSet) or (caches.tensors and (caches.gpu != gpu or caches.pages != refs.shape[0])):
-        raise ValueError(f"hipinfer_amd.{what}: caches must be a cache_set on the current GPU, of as many pages as refs")
-    if refs.dim() != 1:
-        raise ValueError(f"hipinfer_amd.{what}: refs must be int32 [pages], got {tuple(refs.shape)}")
-    for name, t in (("refs", refs), ("refs_out", refs_out)):
-        _vector(what, name, t, refs.shape[0])
-    steps = []
-    for name, t, n in (("table", table, table.shape[0]), ("table_out", table_out, rows)):
-        if t.dtype is not _I32 or t.dim() != 2 or t.shape != (n, table.shape[1]):
-            raise ValueError(f"hipinfer_amd.{what}: {name} must be int32 [{n}, {table.shape[-1]}], got {t.dtype} {tuple(t.shape)}")
-        ld, one = t.stride()
-        if n and one != 1 and t.shape[1] > 1 or n > 1 and not t.shape[1] <= ld <= _INT_MAX:
-            raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous and apart, at most 2^31 - 1 entries")
-        steps.append(ld if n > 1 else t.shape[1])
-    if work is not None and (work.dtype is not _U8 or not work.is_contiguous()):
-        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8")
-    return steps
+def _entries(what, name, t, n, W):
+    """An int32 table [n, W] of contiguous rows; returns its row stride (a single row's is its width)."""
+    shape, steps = t.shape, t.stride()
+    if t.dtype is not _I32 or shape != (n, W):
+        raise ValueError(f"hipinfer_amd.{what}: {name} must be int32 [{n}, {W}], got {t.dtype} {tuple(shape)}")
+    if n and steps[1] != 1 and W > 1 or n > 1 and not W <= steps[0] <= _INT_MAX:
+        raise ValueError(f"hipinfer_amd.{what}: rows of {name} must be contiguous and apart, at most 2^31 - 1 entries")
+    return steps[0] if n > 1 else W
+
+
+def _pool_args(what, caches, gpu, table, refs, refs_out, work):
+    """Checks what cache_fork and cache_compact have in common; returns the shape of the table and the pages."""
+    if not isinstance(caches, CacheSet) or table.dim() != 2 or refs.dim() != 1:
+        raise ValueError(f"hipinfer_amd.{what}: a cache_set, a table [S, W] and refs [pages] are needed")
+    pages = refs.numel()
+    if caches.tensors and (caches.gpu != gpu or caches.pages != pages):
+        raise ValueError(f"hipinfer_amd.{what}: the caches must be on the current GPU and have as many pages as refs, {pages}")
+    _vector(what, "refs", refs, pages)
+    if refs_out is not refs:
+        _vector(what, "refs_out", refs_out, pages)
+    if work is not None and (work.dtype is not _U8 or not work.is_contiguous() or work.get_device() != gpu):
+        raise ValueError(f"hipinfer_amd.{what}: work must be packed uint8 on the current GPU")
+    return table.shape, pages
 
 
 def cache_fork(caches, table, lens, parent, refs, grow=0, table_out=None, lens_out=None, refs_out=None, missing=None,
@@ -786,12 +787,18 @@ def cache_fork(caches, table, lens, parent, refs, grow=0, table_out=None, lens_o
     written instead. missing [1] int32, if given, receives how many pages were not to be had: their entries are -1. Everything
     is read on the device: the call can be captured. At most 8192 rows."""
     what = "cache_fork"
-    N = parent.shape[0]
-    table_out = torch.empty(N, table.shape[-1], dtype=torch.int32, device=table.device) if table_out is None else table_out
-    lens_out = torch.empty(N, dtype=torch.int32, device=table.device) if lens_out is None else lens_out
+    gpu = table.get_device()
+    if not (gpu == refs.get_device() == lens.get_device() == parent.get_device()) or gpu < 0 or gpu != _current_gpu():
+        _elsewhere(what, table, refs, lens, parent)
     refs_out = refs if refs_out is None else refs_out
-    ldt, ldo = _pool_args(what, caches, table, refs, table_out, refs_out, N, work, (lens, parent, lens_out, missing))
-    S, W = table.shape
+    (S, W), pages = _pool_args(what, caches, gpu, table, refs, refs_out, work)
+    N = parent.numel()
+    table_out = torch.empty(N, W, dtype=torch.int32, device=table.device) if table_out is None else table_out
+    lens_out = torch.empty(N, dtype=torch.int32, device=table.device) if lens_out is None else lens_out
+    if not (gpu == table_out.get_device() == lens_out.get_device() == refs_out.get_device()) or \
+            (missing is not None and missing.get_device() != gpu):
+        _elsewhere(what, table, table_out, lens_out, refs_out, missing)
+    ldt, ldo = _entries(what, "table", table, S, W), _entries(what, "table_out", table_out, N, W)
     _vector(what, "lens", lens, S)
     _vector(what, "parent", parent, N)
     _vector(what, "lens_out", lens_out, N)
@@ -800,10 +807,10 @@ def cache_fork(caches, table, lens, parent, refs, grow=0, table_out=None, lens_o
     if not 0 <= grow <= 1 << 30:
         raise ValueError(f"hipinfer_amd.{what}: room for {grow} positions")
     if work is None:
-        work = cache_work(S, N, refs.shape[0])
+        work = cache_work(S, N, pages)
     check_rc(lib.hi_cache_fork(*caches._args, table.data_ptr(), ldt, W, S, lens.data_ptr(), parent.data_ptr(), N,
-                               refs.data_ptr(), refs.shape[0], grow, table_out.data_ptr(), ldo, lens_out.data_ptr(),
-                               refs_out.data_ptr(), _addr(missing), work.data_ptr(), work.numel(), _stream()), what)
+                               refs.data_ptr(), pages, grow, table_out.data_ptr(), ldo, lens_out.data_ptr(),
+                               refs_out.data_ptr(), _addr(missing), work.data_ptr(), work.numel(), _raw_stream(gpu)), what)
     return table_out, lens_out
 
 
@@ -816,19 +823,24 @@ def cache_compact(caches, table, refs, table_out=None, refs_out=None, moved=None
     Returns moved [pages] int32, where each page went (-1 for a free one), for tables of the caller's own, and used [1] int32,
     U. Read on the device: the call can be captured."""
     what = "cache_compact"
+    gpu = table.get_device()
     table_out = table if table_out is None else table_out
     refs_out = refs if refs_out is None else refs_out
     moved = torch.empty_like(refs) if moved is None else moved
     used = torch.empty(1, dtype=torch.int32, device=refs.device) if used is None else used
-    S = table.shape[0]
-    ldt, ldo = _pool_args(what, caches, table, refs, table_out, refs_out, S, work, (moved, used))
-    _vector(what, "moved", moved, refs.shape[0])
+    if not (gpu == refs.get_device() == table_out.get_device() == refs_out.get_device() == moved.get_device() ==
+            used.get_device()) or gpu < 0 or gpu != _current_gpu():
+        _elsewhere(what, table, refs, table_out, refs_out, moved, used)
+    (S, W), pages = _pool_args(what, caches, gpu, table, refs, refs_out, work)
+    ldt = _entries(what, "table", table, S, W)
+    ldo = ldt if table_out is table else _entries(what, "table_out", table_out, S, W)
+    _vector(what, "moved", moved, pages)
     _vector(what, "used", used, 1)
     if work is None:
-        work = cache_work(S, 0, refs.shape[0])
-    check_rc(lib.hi_cache_compact(*caches._args, table.data_ptr(), ldt, table.shape[1], S, refs.data_ptr(), refs.shape[0],
-                                  table_out.data_ptr(), ldo, refs_out.data_ptr(), moved.data_ptr(), used.data_ptr(),
-                                  work.data_ptr(), work.numel(), _stream()), what)
+        work = cache_work(S, 0, pages)
+    check_rc(lib.hi_cache_compact(*caches._args, table.data_ptr(), ldt, W, S, refs.data_ptr(), pages, table_out.data_ptr(), ldo,
+                                  refs_out.data_ptr(), moved.data_ptr(), used.data_ptr(), work.data_ptr(), work.numel(),
+                                  _raw_stream(gpu)), what)
     return moved, used
 
 
