@@ -337,35 +337,36 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
           if (D == 128 || lane < 32) lds_dma16(group(base, lo[g], hi[g], n[g]), to + g * (D / 2), lane * 16);
       }
     };
-    auto widen = [&](const u32x4* from, int exps, u32x4* tile, auto swz) {
-      if constexpr (C::kF8) {
-        u32x4 w[RPW];
+    auto read_codes = [&](const u32x4* from, u32x4 (&w)[RPW]) {
 #pragma unroll
-        for (int i = 0; i < RPW; i++) w[i] = from[i * 64 + lane];
+      for (int i = 0; i < RPW; i++) w[i] = from[i * 64 + lane];
+    };
+    auto widen = [&](const u32x4 (&w)[RPW], int exps, u32x4* tile, auto swz) {
 #pragma unroll
-        for (int i = 0; i < RPW; i++) {
-          const int at = i * 64 + lane, key_at = at / (D / 16), piece = at % (D / 16), k = wave * KPW + key_at;
-          float scale;
-          if constexpr (D == 128) {
-            scale = exponent_scale(__builtin_amdgcn_readlane(exps, i));
-          } else {
-            const int e0 = __builtin_amdgcn_readlane(exps, 2 * i), e1 = __builtin_amdgcn_readlane(exps, 2 * i + 1);
-            scale = exponent_scale(lane < 32 ? e0 : e1);
-          }
-          tile[k * CPR + ((2 * piece) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][0], w[i][1], scale));
-          tile[k * CPR + ((2 * piece + 1) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][2], w[i][3], scale));
+      for (int i = 0; i < RPW; i++) {
+        const int at = i * 64 + lane, key_at = at / (D / 16), piece = at % (D / 16), k = wave * KPW + key_at;
+        float scale;
+        if constexpr (D == 128) {
+          scale = exponent_scale(__builtin_amdgcn_readlane(exps, i));
+        } else {
+          const int e0 = __builtin_amdgcn_readlane(exps, 2 * i), e1 = __builtin_amdgcn_readlane(exps, 2 * i + 1);
+          scale = exponent_scale(lane < 32 ? e0 : e1);
         }
+        tile[k * CPR + ((2 * piece) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][0], w[i][1], scale));
+        tile[k * CPR + ((2 * piece + 1) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][2], w[i][3], scale));
       }
     };
     auto kz = [](int k) { return k_swz<D>(k); };
     auto vz = [](int k) { return v_swz<D>(k); };
     auto advance = [&](int st) {
       if constexpr (C::kF8) {
-        widen(own_k, ke, ks_ + st * Sm::kTile, kz);
-        widen(own_v, vexps, vs_ + (st ^ 1) * Sm::kTile, vz);
+        u32x4 wk[RPW], wv[RPW];
+        read_codes(own_k, wk);
+        read_codes(own_v, wv);
+        widen(wk, ke, ks_ + st * Sm::kTile, kz);
+        widen(wv, vexps, vs_ + (st ^ 1) * Sm::kTile, vz);
         vexps = ve;
-        wait_lgkm0();  // the codes are read
-        asm volatile("" ::: "memory");
+        asm volatile("" ::: "memory");  // (the codes are read: their values have been used)
         next();
         codes_to(c.kp, klo, khi, kn, own_k);
         codes_to(c.vp, vlo, vhi, vn, own_v);
@@ -391,10 +392,13 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       codes_to(c.kp, klo, khi, kn, more_k);
       wait_vmcnt<0>();
       asm volatile("" ::: "memory");
-      widen(own_k, ke0, ks_, kz);
-      widen(own_v, ve0, vs_, vz);
-      widen(more_k, ke1, ks_ + Sm::kTile, kz);
-      wait_lgkm0();
+      u32x4 wk[RPW], wv[RPW], wm[RPW];
+      read_codes(own_k, wk);
+      read_codes(own_v, wv);
+      read_codes(more_k, wm);
+      widen(wk, ke0, ks_, kz);
+      widen(wv, ve0, vs_, vz);
+      widen(wm, ke1, ks_ + Sm::kTile, kz);
       asm volatile("" ::: "memory");
       vexps = ve1;
       next();
