@@ -11,6 +11,7 @@
 // bits, as keys of 64 bits: 40 bits of the distance d from the best (of 1 + d, 2^-35 of it), then the place, so that a key is unique
 // and the lowest (beam, token) wins a tie.
 #include "hi_common.h"
+#include "row_overlap.h"
 
 namespace {
 
@@ -299,6 +300,9 @@ HI_EXPORT int hi_beam_select(const void* logits, long long ldl, const float* sco
   if (!logits || !scores || !best || !parent || !token || ((uintptr_t)logits & 1) || ldl < V ||
       ((uintptr_t)scores | (uintptr_t)best | (uintptr_t)parent | (uintptr_t)token) & 3)
     HI_FAIL("%s: a null or misaligned pointer, or ldl < V", who);
+  // a sequence's block has read its scores before it writes as many in their place; other places are other blocks'
+  if (!in_place_or_apart(scores, 4 * (int64_t)beams, 4 * (int64_t)beams, best, 4 * (int64_t)n, 4 * (int64_t)n, B))
+    HI_FAIL("%s: best must be scores (with n == beams) or apart from it", who);
   const BeamWork w(B * beams, V);
   if (!work || ((uintptr_t)work & 15) || work_bytes < w.bytes)
     HI_FAIL("%s: work of %zu bytes (at least %zu, 16-byte aligned)", who, work_bytes, w.bytes);

@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPerThread = 16;      // pages that a thread of a plan looks at in one step
+constexpr int kMaxPages = 1 << 30;  // of a pool
 constexpr int kMaxRows = 8192;      // rows of a table: the plan keeps 12 bytes a row in LDS
 constexpr int kSetMax = 128;        // cache tensors of one launch: their addresses are kernel arguments (3 KB)
 constexpr int kPart = 4096;         // bytes of a page that a wave copies at a time: 4 loads of 16 bytes a lane
@@ -505,7 +506,7 @@ int pool_check(const char* who, void* const* caches, const long long* strides, c
                const int* table, int ldt, int W, int S, const int* refs, int pages, const int* table_out, int ldo, const int* refs_out,
                const void* work, size_t work_bytes, int N, int& shift) {
   if (page < 1 || page > 1 << 20 || (page & (page - 1))) HI_FAIL("%s: page of %d positions (a power of two)", who, page);
-  if (S < 0 || S > kMaxRows || N < 0 || N > kMaxRows || W < 1 || pages < 1 || n < 0 || ldt < W || ldo < W)
+  if (S < 0 || S > kMaxRows || N < 0 || N > kMaxRows || W < 1 || pages < 1 || pages > kMaxPages || n < 0 || ldt < W || ldo < W)
     HI_FAIL("%s: table [%d, %d] with row strides %d and %d, %d new rows (at most %d), %d pages, %d caches", who, S, W, ldt, ldo, N,
             kMaxRows, pages, n);
   if ((int64_t)W * page > (1 << 30)) HI_FAIL("%s: %d pages of %d positions (at most 2^30 positions a sequence)", who, W, page);
@@ -533,7 +534,7 @@ int copy_blocks(int64_t moves, const CacheSet& c, int cus) {
 }  // namespace
 
 HI_EXPORT size_t hi_cache_work_bytes(int S, int N, int pages) {
-  if (S < 0 || S > kMaxRows || N < 0 || N > kMaxRows || pages < 1) return 0;
+  if (S < 0 || S > kMaxRows || N < 0 || N > kMaxRows || pages < 1 || pages > kMaxPages) return 0;
   return WorkLayout(S, N, pages).bytes;
 }
 
@@ -583,6 +584,10 @@ HI_EXPORT int hi_cache_compact(void* const* caches, const long long* strides, co
                  work_bytes, 0, shift)) return -1;
   if (!moved || (S && !table_out) || ((uintptr_t)moved | (uintptr_t)used) & 3)
     HI_FAIL("%s: moved and used must be 4-byte aligned, moved and the new table not null", who);
+  const int64_t span = 4 * (int64_t)pages;
+  if (rows_meet((uintptr_t)moved, span, span, (uintptr_t)refs, span, span, 1) ||
+      rows_meet((uintptr_t)moved, span, span, (uintptr_t)refs_out, span, span, 1))
+    HI_FAIL("%s: moved must be apart from the counts", who);
   if (S && !in_place_or_apart(table, 4 * (int64_t)ldt, 4 * (int64_t)W, table_out, 4 * (int64_t)ldo, 4 * (int64_t)W, S))
     HI_FAIL("%s: the new table must be the old one (with its row stride) or apart from it", who);
   const HiDevice* d = hi_device();

@@ -225,7 +225,7 @@ int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long 
  * scores[row] + log-probability, in order: best [B][n] fp32, parent [B][n] (the row of logits), token [B][n]. The lowest
  * (beam, token) wins a tie (scores closer than 2^-35 (1 + their distance from the best)); places without a candidate hold
  * -inf, -1, -1: a logit of -inf, a row whose score is not finite or that holds a NaN or +inf, and what lies 2^31 or more below
- * the best are none. beams and n 1 to 64, beams * V <= 2^24, B * beams <= 65535. work: hi_beam_select_work_bytes(...) (0 for
+ * the best are none. best may be scores itself with n == beams, else is apart from it. beams and n 1 to 64, beams * V <= 2^24, B * beams <= 65535. work: hi_beam_select_work_bytes(...) (0 for
  * bad sizes), 16-byte aligned, no state; launches that share it must not run concurrently. */
 size_t hi_beam_select_work_bytes(int B, int beams, int V, int n);
 int hi_beam_select(const void* logits, long long ldl, const float* scores, int B, int beams, int V, int n, float* best,
@@ -247,7 +247,7 @@ int hi_cache_fork(void* const* caches, const long long* strides, const long long
                   int pages, int grow, int* table_out, int ldo, int* lens_out, int* refs_out, int* missing, void* work,
                   size_t work_bytes, void* stream);
 /* Moves the pages in use (refs > 0), U of them, to the front: those at or behind U take the free places before U, both in
- * order. moved [pages]: where each went (-1: free); table_out (table itself, or apart) the renamed entries, refs_out (likewise)
+ * order. moved [pages] (apart from refs and refs_out): where each went (-1: free); table_out (table itself, or apart) the renamed entries, refs_out (likewise)
  * the moved counts, used (if not NULL) U. */
 int hi_cache_compact(void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
                      const int* table, int ldt, int W, int S, const int* refs, int pages, int* table_out, int ldo,

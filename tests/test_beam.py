@@ -159,6 +159,18 @@ def test_out_work_and_repeat(hi):
     assert all(torch.equal(a, b) for a, b in zip(first, out))
 
 
+def test_scores_in_place(hi):
+    """With n == beams the new scores may take the old ones' place."""
+    r = rng(6)
+    B, K, V = 5, 4, 3000
+    x, s = (r.standard_normal((B * K, V)) * 2).astype(np.float16), -r.random(B * K).astype(np.float32)
+    scores = dev(s)
+    out = scores.view(B, K), *(torch.empty(B, K, dtype=torch.int32, device="cuda") for _ in range(2))
+    check("in place", hi.beam_select(dev(x), scores, K, out=out), select(x, s, K, K), K)
+    with pytest.raises(ValueError):
+        hi.beam_select(dev(x), scores[:B * K], K, 3, out=(scores[:B * 3].view(B, 3), *(t[:, :3].contiguous() for t in out[1:])))
+
+
 def test_no_sequences(hi):
     got = hi.beam_select(torch.empty(0, 50, dtype=torch.float16, device="cuda"), torch.empty(0, device="cuda"), 4, 3)
     assert got[1].shape == (0, 3)
