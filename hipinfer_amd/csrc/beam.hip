@@ -174,13 +174,13 @@ __device__ __forceinline__ void least_keys(PickSmem& sh, int n, Push push, All a
 //  * of the segments, those up to the n-th least of 64 groups' least distances (at least n segments are that near);
 //  * of their logits, those up to the n-th segment's best one (the segments' best ones are n that near).
 // What bounds it: a chain of some ten waits (sums and segments from memory, exp and log in 64 bits, two rankings, the picked logits from
-// memory): 8.5 us for 4 beams, 10.2 for 32 times 8 (with 64-bit keys for every segment and logit, in blocks of 256: 16.8 and 27.8).
+// memory): 7.3 us for 4 beams, 9.2 for 32 times 8 (with 64-bit keys for every segment and logit, in blocks of 256: 16.8 and 27.8).
 template <bool WIDE>
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict__ logits, int64_t ldl, const float* __restrict__ scores,
                                                           int V, int R, int K, int n, const char* work, float* best, int* parent,
                                                           int* token) {
   __shared__ PickSmem sh;
-  __shared__ uint32_t seg[kMaxBest];  // the places of the first logits of the picked segments
+  __shared__ int seg_beam[kMaxBest], seg_token[kMaxBest];  // the picked segments' first logits; -1
   const BeamWork w(R, V);
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = K * w.segs;
   const f16* const most = (const f16*)work + (int64_t)b * S;
@@ -214,46 +214,74 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict_
   };
   auto far = [&](int k, float x) { return sh.far[k] + (sh.top[k] - x); };
   // ---- the n best segments
-  auto segments = [&](auto f) {  // f(beam, segment, its largest logit)
-#pragma unroll
-    for (int j = 0; j < kAhead; j++) {
-      const int i = tid + j * kPick;
-      if (i < S) f(i / w.segs, i % w.segs, (float)x0[j]);
-    }
-    for (int i = tid + kAhead * kPick; i < S; i += kPick) f(i / w.segs, i % w.segs, (float)most[i]);
+  const float inv = 1.0f / (float)w.segs;
+  auto beam_of = [&](int i) {  // i / segs, below 64: the product is off by less than one
+    int k = (int)((float)i * inv);
+    if (k * w.segs > i) k--;
+    return i - k * w.segs >= w.segs ? k + 1 : k;
   };
-  float near = __builtin_huge_valf();
-  segments([&](int k, int, float x) { near = fminf(near, far(k, x)); });
+  auto segments = [&](auto f) {  // f(beam, segment, its largest logit)
+    auto one = [&](int i, float x) {
+      const int k = beam_of(i);
+      f(k, i - k * w.segs, x);
+    };
+#pragma unroll
+    for (int j = 0; j < kAhead; j++)
+      if (tid + j * kPick < S) one(tid + j * kPick, (float)x0[j]);
+    for (int i = tid + kAhead * kPick; i < S; i += kPick) one(i, (float)most[i]);
+  };
+  float near = __builtin_huge_valf(), d0[kAhead];  // (d0: the first segments' distances)
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) {
+    const int i = tid + j * kPick;
+    d0[j] = i < S ? far(beam_of(i), (float)x0[j]) : __builtin_huge_valf();
+    near = fminf(near, d0[j]);
+  }
+  for (int i = tid + kAhead * kPick; i < S; i += kPick) near = fminf(near, far(beam_of(i), (float)most[i]));
   constexpr int kLanes = kPick / kGroups;  // of a group
 #pragma unroll
   for (int o = 1; o < kLanes; o <<= 1) near = fminf(near, __shfl_xor(near, o, 64));
   if ((tid & (kLanes - 1)) == 0) sh.best[tid / kLanes] = near;
   if (tid == 0) sh.limit = __builtin_huge_valf();
   __syncthreads();
-  int before = 0, group = tid / kLanes;
+  if (tid < kGroups) {
+    const float mine = sh.best[tid];
+    int before = 0;
 #pragma unroll
-  for (int g = 0; g < kGroups; g++) before += sh.best[g] < near || (sh.best[g] == near && g < group);
-  if (before == n - 1) sh.limit = near * kSlack + 0x1p-34f;  // (infinite with fewer than n groups that have any)
+    for (int g = 0; g < kGroups; g++) before += sh.best[g] < mine || (sh.best[g] == mine && g < tid);
+    if (before == n - 1) sh.limit = mine * kSlack + 0x1p-34f;  // (infinite with fewer than n groups that have any)
+  }
   __syncthreads();
   const float limit = sh.limit;
   least_keys(
       sh, n,
       [&](auto f) {
-        segments([&](int k, int s, float x) {
-          if (far(k, x) <= limit) f(key(k, x, s * kSeg));
-        });
+        auto one = [&](int i, float x) {
+          const int k = beam_of(i);
+          f(key(k, x, (i - k * w.segs) * kSeg));
+        };
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+          if (d0[j] <= limit && tid + j * kPick < S) one(tid + j * kPick, (float)x0[j]);
+        for (int i = tid + kAhead * kPick; i < S; i += kPick) {
+          const float x = (float)most[i];
+          if (far(beam_of(i), x) <= limit) one(i, x);
+        }
       },
       [&](auto f) { segments([&](int k, int s, float x) { f(key(k, x, s * kSeg)); }); });
-  if (tid < n) seg[tid] = sh.out[tid] == kNone ? ~0u : (uint32_t)sh.out[tid] & 0xffffff;
+  if (tid < n) {
+    const int at = sh.out[tid] == kNone ? -1 : (int)(sh.out[tid] & 0xffffff), k = at < 0 ? -1 : at / V;
+    seg_beam[tid] = k;
+    seg_token[tid] = at - k * V;
+  }
   const uint64_t nth = sh.out[n - 1];
   const float cut = nth == kNone ? __builtin_huge_valf() : limit_of(nth);
   __syncthreads();
   // ---- the n best candidates in them
   auto chunks = [&](auto f) {  // f(beam, logit, token)
     for (int i = tid; i < n * (kSeg / 8); i += kPick) {
-      const uint32_t first = seg[i / (kSeg / 8)];
-      if (first == ~0u) continue;
-      const int k = first / V, t = first - k * V + i % (kSeg / 8) * 8;
+      const int k = seg_beam[i / (kSeg / 8)], t = seg_token[i / (kSeg / 8)] + i % (kSeg / 8) * 8;
+      if (k < 0) continue;
       const f16x8 x = load8<WIDE>(logits + ((int64_t)b * K + k) * ldl, V, t);
 #pragma unroll
       for (int e = 0; e < 8; e++) f(k, (float)x[e], t + e);
