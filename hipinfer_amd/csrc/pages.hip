@@ -62,23 +62,24 @@ struct WorkLayout {
   }
 };
 
-// Exclusive sum over the block of v, and the total; sh: one int per wave.
-__device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
+// Exclusive sum over the block of v, and the total; sh: one number per wave.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, int64_t* sh, T& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
+  T x = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
+    const T y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
   __syncthreads();  // the sums of the last call have been read
   if (lane == 63) sh[wave] = x;
   __syncthreads();
-  int before = 0;
+  T before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kPlanThreads / 64; w++) {
-    const int s = sh[w];
+    const T s = (T)sh[w];
     if (w < wave) before += s;
     total += s;
   }
@@ -122,7 +123,7 @@ struct ForkArgs {
 // 256.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   extern __shared__ int lds[];
-  __shared__ int sh[kPlanThreads / 64];
+  __shared__ int64_t sh[kPlanThreads / 64];
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     for (int i = (blockIdx.x - 1) * kPlanThreads + tid; i < a.pages; i += (gridDim.x - 1) * kPlanThreads) a.refs_out[i] = a.refs[i];
@@ -186,13 +187,14 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     if (sub == 0 && i < a.N) fresh[i] = rank;
   }
   __syncthreads();
-  // ranks among all rows' fresh pages
-  int T = 0;
+  // ranks among all rows' fresh pages: as far as there are pages (a rank in a row is below 2^30 too)
+  int64_t T = 0;
   for (int i0 = 0; i0 < a.N; i0 += kPlanThreads) {
-    const int i = i0 + tid, v = i < a.N ? fresh[i] : 0;
-    int total;
-    const int at = T + block_scan(v, sh, total);
-    if (i < a.N) ((int*)(a.work + w.base))[i] = at;
+    const int i = i0 + tid;
+    const int64_t v = i < a.N ? fresh[i] : 0;
+    int64_t total;
+    const int64_t at = T + block_scan(v, sh, total);
+    if (i < a.N) ((int*)(a.work + w.base))[i] = (int)min(at, (int64_t)kMaxPages);
     T += total;
   }
   // the first T free pages
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
     }
     found += total;
   }
-  found = min(found, T);
+  found = (int)min((int64_t)found, T);
   __syncthreads();  // the list is written (a block's own stores, read past the L1 below)
   // part-filled pages to be copied
   Move* const moves = (Move*)(a.work + w.moves);
@@ -237,13 +239,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
       }
     }
     int total;
-    const int at = M + block_scan(m.src >= 0, sh, total);
+    const int at = M + block_scan((int)(m.src >= 0), sh, total);
     if (m.src >= 0) moves[at] = m;
     M += total;
   }
   if (tid == 0) {
     *(PlanHead*)a.work = PlanHead{found, M, 0, 0};
-    if (a.missing) *a.missing = T - found;
+    if (a.missing) *a.missing = (int)min(T - found, (int64_t)INT_MAX);
   }
 }
 
@@ -397,7 +399,7 @@ struct CompactArgs {
 // The used pages at or behind the number U of used pages go, in order, to the free ones before it, in order. 500 pages 4.9 us,
 // 6000 9.6.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs a) {
-  __shared__ int sh[kPlanThreads / 64];
+  __shared__ int64_t sh[kPlanThreads / 64];
   const int tid = threadIdx.x;
   const WorkLayout w(a.S, 0, a.pages);
   Move* const moves = (Move*)(a.work + w.moves);
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(CompactArgs 
       }
     }
     int both;  // (at most 2^14 of either in a step)
-    const int at = block_scan(__popc(moving) << 16 | __popc(hole), sh, both), n_out = both >> 16, n_in = both & 0xffff;
+    const int at = block_scan((int)(__popc(moving) << 16 | __popc(hole)), sh, both), n_out = both >> 16, n_in = both & 0xffff;
     int at_out = out + (at >> 16), at_in = in + (at & 0xffff);
     for (; moving; moving &= moving - 1)
       __hip_atomic_store(&moves[at_out++].src, mine + __ffs(moving) - 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
