@@ -11,6 +11,7 @@ constexpr int kFpRG = 4;              // 32-row groups per block (2 waves each);
 constexpr int kFpKPW = 64;            // keys per wave per tile (32-key MFMA blocks of the wave's half)
 constexpr int kFpBKV = 2 * kFpKPW;    // keys per tile
 constexpr int kFpStages = 2;          // LDS stages of K/V tiles
+constexpr int kFeedDma = 0, kFeedWiden = 1;  // how tiles come into the stages (flash_tile.h)
 constexpr float kFpMaxLag = 8.f;      // log2 of how far a row's reference max may trail its max
 
 // XOR term of key r's 16-byte chunks in the K tile: the 16 keys (D = 128) or 8 key pairs (D = 64)

@@ -4,9 +4,11 @@
 //   lane, fr, fk, kh, qf, scale_log2             the lane's place and its Q fragments
 //   nt, n_full                                   key tiles, and how many at the front hold no masked key for this wave
 //   issue_k(i, st), issue_v(i, st)               DMA instruction i of the next K (V) tile into stage st
-//   kSpread                                      whether issue_k and issue_v do something: they are called between the MFMAs
 //   advance(st)                                  called once before the DMA of each K tile (into stage st) but the first: ahead
 //                                                of the others by first_advance()
+//   kFeed                                        kFeedDma, or kFeedWiden: the prologue has filled the stages already; issue_k(i, st) and
+//                                                issue_v(i, st) are vector work and a write to LDS, codes_v() comes before the latter,
+//                                                and refill() follows the last of a tile
 //   before_barrier(), after_barrier()            called around the prologue's barrier, before n_full is read
 //   kGuard, odd_tile                             whether infinities and NaN in V are taken out of masked tiles, and the first
 //                                                tile where any were (INT_MAX)
@@ -141,7 +143,9 @@
     // slots of the first logits block; with 4 waves, each issuing twice as many and without a second
     // wave on its SIMD to fill its stalls, over all of them (64 rows after 2000 positions 26.1 ->
     // 22.6 us, 512 after 2048 36.0 -> 32.7; 8 waves: no gain, 2 % slower at T = 2048 after 4096).
-    constexpr int ND = kSpread ? 2 * IPW : 0, LA = 3;  // DMA instructions, LDS reads ahead of their MFMA
+    // (With kFeedWiden they go between the MFMAs of the last block's P.V, in the order written.)
+    constexpr bool WIDEN = kFeed == kFeedWiden;
+    constexpr int ND = WIDEN ? 0 : 2 * IPW, LA = 3;  // DMA instructions, LDS reads ahead of their MFMA
     constexpr int S0 = RG == 2 ? 0 : 2 * DT, NS = RG == 2 ? 2 * DT + 2 * NQ : NQ;
     auto dma_here = [](int m) constexpr {  // DMA instructions that go before slot m
       int n = 0;
@@ -169,6 +173,15 @@
         if (m >= 2 * DT - LA) kf[m - (2 * DT - LA)] = load_k(0, m - (2 * DT - LA));
       }
       o[m % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl[m / DT][m % DT], pl[m / DT], o[m % DT], 0, 0, 0);
+      if constexpr (NEXT && WIDEN) {
+        constexpr int PER = IPW / DT;  // chunks a slot: K's in the first half of the slots, V's in the second
+        static_assert(PER * DT == IPW, "chunks per slot");
+        if (m == DT / 2 - 1) codes_v();
+#pragma unroll
+        for (int j = m * PER; j < (m + 1) * PER; j++) j < IPW ? issue_k(j, st) : issue_v(j - IPW, st ^ 1);
+        if (m == 2 * DT - 1) refill();
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if constexpr (NEXT) {
 #pragma unroll
@@ -185,7 +198,7 @@
       for (int e = 0; e < 16; e++) mx = fmaxf(mx, sc[kt][e]);
     constexpr int kMaskOps = MASK ? 8 : 0;  // more vector work per MFMA
 #pragma unroll
-    for (int m = 0; m < 2 * DT; m++) {
+    for (int m = 0; m < (NEXT && WIDEN ? 0 : 2 * DT); m++) {
       if (NEXT && dma_here(m)) __builtin_amdgcn_sched_group_barrier(0x020, kDma, 0);  // DMA
       if (NEXT && m >= 2 * DT - LA) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // MFMA (the last block's P.V)
@@ -256,13 +269,15 @@
   };
 
   // ---- prologue: K tiles 0 and 1 and V tile 0 in flight, the logits of tile 0
+  if constexpr (kFeed == kFeedDma) {
 #pragma unroll
-  for (int i = 0; i < IPW; i++) issue_k(i, 0);
-  first_advance();
+    for (int i = 0; i < IPW; i++) issue_k(i, 0);
+    first_advance();
 #pragma unroll
-  for (int i = 0; i < IPW; i++) {
-    issue_v(i, 0);
-    issue_k(i, 1);
+    for (int i = 0; i < IPW; i++) {
+      issue_v(i, 0);
+      issue_k(i, 1);
+    }
   }
   before_barrier();
   wait_vmcnt<2 * IPW>();
@@ -293,11 +308,13 @@
       wait_vmcnt<0>();
       barrier_no_fence();
       advance(t & 1);
+      if constexpr (kFeed == kFeedWiden) codes_v();
 #pragma unroll
       for (int i = 0; i < IPW; i++) {
         issue_k(i, t & 1);
         issue_v(i, (t & 1) ^ 1);
       }
+      if constexpr (kFeed == kFeedWiden) refill();
     }
   }
   if (live(t)) {

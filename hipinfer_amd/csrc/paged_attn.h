@@ -303,7 +303,7 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<typename C::Elem*>(base) + (((uint64_t)hi << 32) | lo), (short)0, n,
                                                0x00020000);
     };
-    constexpr bool kSpread = !C::kF8;
+    constexpr int kFeed = C::kF8 ? kFeedWiden : kFeedDma;
     int koff[IPW], voff[IPW];
     auto next = [&] {
 #pragma unroll
@@ -315,21 +315,14 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       take();
       fetch();
     };
-    auto issue_k = [&](int i, int st) {
-      if constexpr (kSpread)
-        lds_dma16(group(c.kp, klo[i / IPG], khi[i / IPG], kn[i / IPG]), ks_ + st * Sm::kTile + (wave * IPW + i) * 64, koff[i]);
-    };
-    auto issue_v = [&](int i, int st) {
-      if constexpr (kSpread)
-        lds_dma16(group(c.vp, vlo[i / IPG], vhi[i / IPG], vn[i / IPG]), vs_ + st * Sm::kTile + (wave * IPW + i) * 64, voff[i]);
-    };
     // F8: a wave's share of a tile comes as codes (a group of 8 keys is D / 2 lanes of DMA) and is made into fp16 by the wave itself,
-    // one tile before the others read it: no barrier, and no registers held while a tile is computed. The codes' place in LDS is free
-    // again as soon as they are read.
-    constexpr int RPW = KPW * D / 1024;  // 16-byte reads of a lane per wave and operand
+    // one tile before the others read it: no barrier more, and no registers held from tile to tile. The codes' place in LDS is free
+    // again as soon as they are read, and the next tile's are sent for.
+    constexpr int RPW = KPW * D / 1024;  // 16-byte reads of a lane per wave and operand, 2 chunks each
     int vexps = 0;  // the exponents of the V tile that lies there as codes; the K tile's are ke
     u32x4* const own_k = fp_smem + 2 * kFpStages * Sm::kTile + wave * RPW * 64;
     u32x4* const own_v = own_k + Sm::kTile / 2;
+    u32x4 wk[RPW], wv[RPW];  // a tile's codes
     auto codes_to = [&](const typename C::Elem* base, const uint32_t (&lo)[NG], const uint32_t (&hi)[NG], const int (&n)[NG], u32x4* to) {
       if constexpr (C::kF8) {
 #pragma unroll
@@ -341,43 +334,46 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
 #pragma unroll
       for (int i = 0; i < RPW; i++) w[i] = from[i * 64 + lane];
     };
-    auto widen = [&](const u32x4 (&w)[RPW], int exps, u32x4* tile, auto swz) {
-#pragma unroll
-      for (int i = 0; i < RPW; i++) {
-        const int at = i * 64 + lane, key_at = at / (D / 16), piece = at % (D / 16), k = wave * KPW + key_at;
-        float scale;
-        if constexpr (D == 128) {
-          scale = exponent_scale(__builtin_amdgcn_readlane(exps, i));
-        } else {
-          const int e0 = __builtin_amdgcn_readlane(exps, 2 * i), e1 = __builtin_amdgcn_readlane(exps, 2 * i + 1);
-          scale = exponent_scale(lane < 32 ? e0 : e1);
-        }
-        tile[k * CPR + ((2 * piece) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][0], w[i][1], scale));
-        tile[k * CPR + ((2 * piece + 1) ^ swz(k))] = __builtin_bit_cast(u32x4, f8x8_to_f16(w[i][2], w[i][3], scale));
+    auto widen = [&](int j, const u32x4 (&w)[RPW], int exps, u32x4* tile, auto swz) {  // chunk j of a lane's
+      const int i = j / 2, at = i * 64 + lane, key_at = at / (D / 16), piece = at % (D / 16), k = wave * KPW + key_at;
+      float scale;
+      if constexpr (D == 128) {
+        scale = exponent_scale(__builtin_amdgcn_readlane(exps, i));
+      } else {
+        const int e0 = __builtin_amdgcn_readlane(exps, 2 * i), e1 = __builtin_amdgcn_readlane(exps, 2 * i + 1);
+        scale = exponent_scale(lane < 32 ? e0 : e1);
       }
+      const f16x8 x = j & 1 ? f8x8_to_f16(w[i][2], w[i][3], scale) : f8x8_to_f16(w[i][0], w[i][1], scale);
+      tile[k * CPR + ((2 * piece + (j & 1)) ^ swz(k))] = __builtin_bit_cast(u32x4, x);
     };
     auto kz = [](int k) { return k_swz<D>(k); };
     auto vz = [](int k) { return v_swz<D>(k); };
-    auto advance = [&](int st) {
+    auto issue_k = [&](int i, int st) {
+      if constexpr (C::kF8) widen(i, wk, ke, ks_ + st * Sm::kTile, kz);
+      else lds_dma16(group(c.kp, klo[i / IPG], khi[i / IPG], kn[i / IPG]), ks_ + st * Sm::kTile + (wave * IPW + i) * 64, koff[i]);
+    };
+    auto issue_v = [&](int i, int st) {
+      if constexpr (C::kF8) widen(i, wv, vexps, vs_ + st * Sm::kTile, vz);
+      else lds_dma16(group(c.vp, vlo[i / IPG], vhi[i / IPG], vn[i / IPG]), vs_ + st * Sm::kTile + (wave * IPW + i) * 64, voff[i]);
+    };
+    auto codes_v = [&] {
+      if constexpr (C::kF8) read_codes(own_v, wv);
+    };
+    auto refill = [&] {  // (the codes are read: their values have been used)
       if constexpr (C::kF8) {
-        u32x4 wk[RPW], wv[RPW];
-        read_codes(own_k, wk);
-        read_codes(own_v, wv);
-        widen(wk, ke, ks_ + st * Sm::kTile, kz);
-        widen(wv, vexps, vs_ + (st ^ 1) * Sm::kTile, vz);
         vexps = ve;
-        asm volatile("" ::: "memory");  // (the codes are read: their values have been used)
+        asm volatile("" ::: "memory");
         next();
         codes_to(c.kp, klo, khi, kn, own_k);
         codes_to(c.vp, vlo, vhi, vn, own_v);
-      } else {
-        next();
       }
+    };
+    auto advance = [&](int) {
+      if constexpr (C::kF8) read_codes(own_k, wk);
+      else next();
       __builtin_amdgcn_sched_barrier(0);
     };
-    auto first_advance = [&] {
-      if constexpr (!C::kF8) advance(0);
-    };
+    auto first_advance = [&] { advance(0); };
     if constexpr (C::kF8) {
       // K tiles 0 and 1 and V tile 0 at once (K tile 1's codes in the last V stage, which is free until tile 0 is computed), then K tile 2's
       // and V tile 1's codes on their way
@@ -392,18 +388,18 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       codes_to(c.kp, klo, khi, kn, more_k);
       wait_vmcnt<0>();
       asm volatile("" ::: "memory");
-      u32x4 wk[RPW], wv[RPW], wm[RPW];
+      u32x4 wm[RPW];
       read_codes(own_k, wk);
       read_codes(own_v, wv);
       read_codes(more_k, wm);
-      widen(wk, ke0, ks_, kz);
-      widen(wv, ve0, vs_, vz);
-      widen(wm, ke1, ks_ + Sm::kTile, kz);
-      asm volatile("" ::: "memory");
-      vexps = ve1;
-      next();
-      codes_to(c.kp, klo, khi, kn, own_k);
-      codes_to(c.vp, vlo, vhi, vn, own_v);
+#pragma unroll
+      for (int i = 0; i < IPW; i++) {
+        widen(i, wk, ke0, ks_, kz);
+        widen(i, wv, ve0, vs_, vz);
+        widen(i, wm, ke1, ks_ + Sm::kTile, kz);
+      }
+      ve = ve1;
+      refill();
     } else {
       // DMA instruction i of this wave fills slots (wave IPW + i) * 64 + lane of a tile: slot s holds
       // key s / CPR, physical chunk s % CPR, i.e. logical chunk (s % CPR) ^ swz(key)

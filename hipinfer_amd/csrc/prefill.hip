@@ -133,9 +133,11 @@ __global__ void __launch_bounds__(128 * RG)
   auto enter_masked = [](int) {};
   constexpr bool kGuard = false;
   int odd_tile = 0;
-  constexpr bool kSpread = true;
+  constexpr int kFeed = kFeedDma;
   auto advance = [](int) {};
   auto first_advance = [] {};
+  auto codes_v = [] {};
+  auto refill = [] {};
   auto before_barrier = [] {};
   auto after_barrier = [] {};
   auto live = [&](int t) {
