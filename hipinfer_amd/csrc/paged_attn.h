@@ -334,8 +334,15 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
 #pragma unroll
       for (int i = 0; i < RPW; i++) w[i] = from[i * 64 + lane];
     };
-    auto widen = [&](int j, const u32x4 (&w)[RPW], int exps, u32x4* tile, auto swz) {  // chunk j of a lane's
-      const int i = j / 2, at = i * 64 + lane, key_at = at / (D / 16), piece = at % (D / 16), k = wave * KPW + key_at;
+    // Where a lane's first chunk goes in a K and a V tile, in bytes. The others' places follow from it by constants: the second
+    // chunk of a read in bit 4, and at D = 128 K's second group of keys in the swizzle's bit 3. The asm below keeps the compiler
+    // from holding each place in a register of its own for the whole loop, where it then spilled 16 (100 rows behind 4000
+    // positions, Hq 32, Hkv 8: 29.5 us with those, 28.0 without).
+    const int key0 = wave * KPW + lane / (D / 16), piece0 = lane % (D / 16);
+    const int k_put = 16 * (key0 * CPR + ((2 * piece0) ^ k_swz<D>(key0))), v_put = 16 * (key0 * CPR + ((2 * piece0) ^ v_swz<D>(key0)));
+    static_assert(!C::kF8 || D == 64 || KPW % 16 == 0, "a wave's keys begin a period of the swizzle");
+    auto widen = [&](int j, const u32x4 (&w)[RPW], int exps, u32x4* tile, int put, bool k) {  // chunk j of a lane's
+      const int i = j / 2;
       float scale;
       if constexpr (D == 128) {
         scale = exponent_scale(__builtin_amdgcn_readlane(exps, i));
@@ -343,17 +350,17 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
         const int e0 = __builtin_amdgcn_readlane(exps, 2 * i), e1 = __builtin_amdgcn_readlane(exps, 2 * i + 1);
         scale = exponent_scale(lane < 32 ? e0 : e1);
       }
+      asm("" : "+v"(put));
+      const int at = (put ^ (16 * (j & 1)) ^ (k && D == 128 ? 128 * (i & 1) : 0)) + i * (1024 / D) * CPR * 16;
       const f16x8 x = j & 1 ? f8x8_to_f16(w[i][2], w[i][3], scale) : f8x8_to_f16(w[i][0], w[i][1], scale);
-      tile[k * CPR + ((2 * piece + (j & 1)) ^ swz(k))] = __builtin_bit_cast(u32x4, x);
+      *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(tile) + at) = __builtin_bit_cast(u32x4, x);
     };
-    auto kz = [](int k) { return k_swz<D>(k); };
-    auto vz = [](int k) { return v_swz<D>(k); };
     auto issue_k = [&](int i, int st) {
-      if constexpr (C::kF8) widen(i, wk, ke, ks_ + st * Sm::kTile, kz);
+      if constexpr (C::kF8) widen(i, wk, ke, ks_ + st * Sm::kTile, k_put, true);
       else lds_dma16(group(c.kp, klo[i / IPG], khi[i / IPG], kn[i / IPG]), ks_ + st * Sm::kTile + (wave * IPW + i) * 64, koff[i]);
     };
     auto issue_v = [&](int i, int st) {
-      if constexpr (C::kF8) widen(i, wv, vexps, vs_ + st * Sm::kTile, vz);
+      if constexpr (C::kF8) widen(i, wv, vexps, vs_ + st * Sm::kTile, v_put, false);
       else lds_dma16(group(c.vp, vlo[i / IPG], vhi[i / IPG], vn[i / IPG]), vs_ + st * Sm::kTile + (wave * IPW + i) * 64, voff[i]);
     };
     auto codes_v = [&] {
@@ -394,9 +401,9 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
       read_codes(more_k, wm);
 #pragma unroll
       for (int i = 0; i < IPW; i++) {
-        widen(i, wk, ke0, ks_, kz);
-        widen(i, wv, ve0, vs_, vz);
-        widen(i, wm, ke1, ks_ + Sm::kTile, kz);
+        widen(i, wk, ke0, ks_, k_put, true);
+        widen(i, wv, ve0, vs_, v_put, false);
+        widen(i, wm, ke1, ks_ + Sm::kTile, k_put, true);
       }
       ve = ve1;
       refill();
