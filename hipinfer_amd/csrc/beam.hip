@@ -99,9 +99,11 @@ __device__ __forceinline__ double wave_sum64(double v) {
 }
 
 struct PickSmem {
-  double base[kMaxBeams];   // scores[k] - log sum; NaN for a beam without candidates
-  float top[kMaxBeams];     // the beam's largest logit
-  float far[kMaxBeams];     // how far its best candidate is from the best of all; infinite without candidates
+  double logsum[kMaxBeams];  // log sum exp(x - top); NaN for a beam without candidates
+  double off[kMaxBeams];     // how far the beam's best candidate is from the best of all; infinite without candidates
+  float score[kMaxBeams];    // scores[k]
+  float top[kMaxBeams];      // the beam's largest logit
+  float far[kMaxBeams];      // off as fp32
   float best[kGroups];
   uint64_t list[kList];
   uint64_t out[kMaxBest];   // the n least keys in order
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict_
   // ---- the beams' log sums
   for (int k = wave; k < K; k += kPick / 64) {
     const float* p = pairs + 2 * (int64_t)k * w.waves;
-    const double s = (double)scores[b * K + k];
+    const float s = scores[b * K + k];
     float M = -__builtin_huge_valf();
     for (int i = lane; i < w.waves; i += 64) M = fmaxf(M, p[2 * i]);
     M = wave_max(M);
@@ -199,19 +201,29 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict_
     for (int i = lane; i < w.waves; i += 64) sum += (double)p[2 * i + 1] * exp((double)p[2 * i] - (double)M);
     sum = wave_sum64(sum);
     if (lane == 0) {
+      sh.score[k] = s;
       sh.top[k] = M;
-      sh.base[k] = s - s == 0.0 && M - M == 0.f && sum - sum == 0.0 ? s - log(sum) : __builtin_nan("");  // none of them infinite
+      sh.logsum[k] = s - s == 0.f && M - M == 0.f && sum - sum == 0.0 ? log(sum) : __builtin_nan("");  // none of them infinite
     }
   }
   __syncthreads();
-  double top = -__builtin_huge_val();
-  for (int k = 0; k < K; k++)
-    if (sh.base[k] > top) top = sh.base[k];  // a beam's best candidate is its largest logit
-  if (tid < K) sh.far[tid] = sh.base[tid] <= top ? (float)(top - sh.base[tid]) : __builtin_huge_valf();
+  // ---- how far the beams' best candidates (their largest logits) are from the best of all. Log sums and logits are added to
+  // differences of scores, never to a score: beside one of 1e17 or the lowest float they would be rounded away, and candidates that
+  // differ would be equal by their keys but not by `far`.
+  static_assert(kMaxBeams <= 64, "a lane per beam");
+  if (wave == 0) {
+    const bool any = lane < K && sh.logsum[lane] == sh.logsum[lane];
+    const float s = any ? sh.score[lane] : -__builtin_huge_valf(), most = wave_max(s);
+    const double e = any ? ((double)s - (double)most) - sh.logsum[lane] : -__builtin_huge_val();
+    double top = e;
+    for (int o = 1; o < K; o <<= 1) top = fmax(top, __shfl_xor(top, o, 64));  // (of the 2^i >= K lanes that hold the beams)
+    if (lane < K) {
+      sh.off[lane] = any ? top - e : __builtin_huge_val();
+      sh.far[lane] = (float)sh.off[lane];
+    }
+  }
   __syncthreads();
-  auto key = [&](int k, float x, int t) {
-    return key_of(top - (((double)x - (double)sh.top[k]) + sh.base[k]), (uint32_t)(k * V + t));
-  };
+  auto key = [&](int k, float x, int t) { return key_of(sh.off[k] + ((double)sh.top[k] - (double)x), (uint32_t)(k * V + t)); };
   auto far = [&](int k, float x) { return sh.far[k] + (sh.top[k] - x); };
   // ---- the n best segments
   const float inv = 1.0f / (float)w.segs;
@@ -303,7 +315,7 @@ __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict_
       const int at = (int)(q & 0xffffff);
       k = at / V;
       t = at - k * V;
-      s = (float)(((double)logits[((int64_t)b * K + k) * ldl + t] - (double)sh.top[k]) + sh.base[k]);
+      s = (float)(((double)logits[((int64_t)b * K + k) * ldl + t] - (double)sh.top[k]) + ((double)sh.score[k] - sh.logsum[k]));
       k += b * K;
     }
     best[b * n + tid] = s;
