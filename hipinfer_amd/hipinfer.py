@@ -783,8 +783,8 @@ def cache_fork(caches, table, lens, parent, refs, grow=0, table_out=None, lens_o
     all tensors of `caches` (cache_set). What no new row holds loses its count, and is free for the next call. Entries
     that name no page are taken over as they are found missing (-1 for a whole page).
 
-    Returns (table_out [N, W], lens_out [N]), memory apart from table and lens; refs is updated in place, or refs_out
-    written instead. missing [1] int32, if given, receives how many pages were not to be had: their entries are -1. Everything
+    Returns (table_out [N, W], lens_out [N]), memory apart from table, lens, parent and refs; refs is updated in place, or refs_out
+    written instead, apart from the others too. missing [1] int32, if given, receives how many pages were not to be had: their entries are -1. Everything
     is read on the device: the call can be captured. At most 8192 rows."""
     what = "cache_fork"
     gpu = table.get_device()

@@ -240,8 +240,8 @@ size_t hi_cache_work_bytes(int S, int N, int pages);
  * `missing` if not NULL, when there are none) and the positions held of a part-filled page are copied. refs_out (refs itself,
  * or apart) has the new counts; pages that they free are handed out by later calls.
  * The n cache tensors (host arrays): caches[t] with pages strides[t] bytes apart, bytes[t] per page, which are runs[t] runs of
- * `page` positions (heads), or with runs[t] 0 are copied whole. table_out and lens_out are apart from table and lens. S, N
- * <= 8192. */
+ * `page` positions (heads), or with runs[t] 0 are copied whole. table_out, lens_out, missing and work share no memory with each
+ * other or with anything else of the call (rows of tables may alternate in one buffer). S, N <= 8192. */
 int hi_cache_fork(void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
                   const int* table, int ldt, int W, int S, const int* lens, const int* parent, int N, const int* refs,
                   int pages, int grow, int* table_out, int ldo, int* lens_out, int* refs_out, int* missing, void* work,
