@@ -599,12 +599,16 @@ HI_EXPORT int hi_cache_compact(void* const* caches, const long long* strides, co
                  work_bytes, 0, shift)) return -1;
   if (!moved || (S && !table_out) || ((uintptr_t)moved | (uintptr_t)used) & 3)
     HI_FAIL("%s: moved and used must be 4-byte aligned, moved and the new table not null", who);
-  const int64_t span = 4 * (int64_t)pages;
-  if (rows_meet((uintptr_t)moved, span, span, (uintptr_t)refs, span, span, 1) ||
-      rows_meet((uintptr_t)moved, span, span, (uintptr_t)refs_out, span, span, 1))
-    HI_FAIL("%s: moved must be apart from the counts", who);
   if (S && !in_place_or_apart(table, 4 * (int64_t)ldt, 4 * (int64_t)W, table_out, 4 * (int64_t)ldo, 4 * (int64_t)W, S))
     HI_FAIL("%s: the new table must be the old one (with its row stride) or apart from it", who);
+  // moved is read by the blocks that write the new table and counts beside each other
+  const int64_t span = 4 * (int64_t)pages;
+  const CallRows rows[] = {{"table", table, 4 * (int64_t)ldt, 4 * (int64_t)W, S, false}, flat("refs", refs, span, false),
+                           {"table_out", table_out, 4 * (int64_t)ldo, 4 * (int64_t)W, S, true, 0}, flat("refs_out", refs_out, span, true, 1),
+                           flat("moved", moved, span, true), flat("used", used, 4, true),
+                           flat("work", work, (int64_t)WorkLayout(S, 0, pages).bytes, true)};
+  const char *a0, *a1;
+  if (call_rows_meet(rows, a0, a1)) HI_FAIL("%s: %s and %s must be apart", who, a0, a1);
   const HiDevice* d = hi_device();
   if (!d) return -2;
   const hipStream_t s = (hipStream_t)stream;

@@ -821,7 +821,7 @@ def cache_compact(caches, table, refs, table_out=None, refs_out=None, moved=None
     table_out and refs_out.
 
     Returns moved [pages] int32, where each page went (-1 for a free one), for tables of the caller's own, and used [1] int32,
-    U. Read on the device: the call can be captured."""
+    U, both apart from the other tensors. Read on the device: the call can be captured."""
     what = "cache_compact"
     gpu = table.get_device()
     table_out = table if table_out is None else table_out

@@ -247,8 +247,9 @@ int hi_cache_fork(void* const* caches, const long long* strides, const long long
                   int pages, int grow, int* table_out, int ldo, int* lens_out, int* refs_out, int* missing, void* work,
                   size_t work_bytes, void* stream);
 /* Moves the pages in use (refs > 0), U of them, to the front: those at or behind U take the free places before U, both in
- * order. moved [pages] (apart from refs and refs_out): where each went (-1: free); table_out (table itself, or apart) the renamed entries, refs_out (likewise)
- * the moved counts, used (if not NULL) U. */
+ * order. moved [pages]: where each went (-1: free); table_out (table itself, or apart) the renamed entries, refs_out (refs itself, or
+ * apart) the moved counts, used (if not NULL) U. Otherwise what is written, work too, shares no memory with anything else of the
+ * call. */
 int hi_cache_compact(void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
                      const int* table, int ldt, int W, int S, const int* refs, int pages, int* table_out, int ldo,
                      int* refs_out, int* moved, int* used, void* work, size_t work_bytes, void* stream);

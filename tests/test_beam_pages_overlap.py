@@ -85,3 +85,37 @@ def test_fork(out, other, capfd):
 ], ids=str)
 def test_fork_accepts(change):
     assert call("hi_cache_fork", FORK | change) == -2
+
+
+COMPACT = dict(arrays(), n=2, page=16, table=MB, ldt=6, W=4, S=3, refs=4 * MB, pages=30, table_out=5 * MB, ldo=6, refs_out=7 * MB,
+               moved=2 * MB, used=8 * MB, work=9 * MB, work_bytes=1 << 16, stream=None)
+COMPACT_READ = ("table", "refs")
+COMPACT_WRITTEN = ("table_out", "refs_out", "moved", "used", "work")
+IN_PLACE = {("table", "table_out"), ("refs", "refs_out")}
+
+
+@pytest.mark.parametrize("out", COMPACT_WRITTEN)
+@pytest.mark.parametrize("other", COMPACT_READ + COMPACT_WRITTEN)
+def test_compact(out, other, capfd):
+    if out == other or (other, out) in IN_PLACE:
+        return
+    refused("hi_cache_compact", COMPACT | {out: COMPACT[other]}, (other, out), capfd)
+    if other != "used" and out != "work":
+        refused("hi_cache_compact", COMPACT | {out: COMPACT[other] + 8}, (other, out), capfd)
+
+
+def test_compact_in_place(capfd):
+    """moved on the table and the counts that are renamed in place."""
+    base = COMPACT | dict(table_out=MB, refs_out=4 * MB)
+    for at, name in ((MB, "table"), (MB + 24 + 8, "table"), (4 * MB, "refs"), (4 * MB + 116, "refs")):
+        refused("hi_cache_compact", base | dict(moved=at), (name, "moved"), capfd)
+        refused("hi_cache_compact", base | dict(used=at), (name, "used"), capfd)
+
+
+@accepted
+@pytest.mark.parametrize("change", [
+    {}, dict(table_out=MB, refs_out=4 * MB), dict(used=None), dict(moved=MB + 12 * 6), dict(used=MB + 16),  # used in a gap of the table
+    dict(table_out=MB + 16, ldt=8, ldo=8), dict(S=0, table=None, table_out=None),
+], ids=str)
+def test_compact_accepts(change):
+    assert call("hi_cache_compact", COMPACT | change) == -2
