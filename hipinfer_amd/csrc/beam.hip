@@ -348,6 +348,13 @@ HI_EXPORT int hi_beam_select(const void* logits, long long ldl, const float* sco
   const BeamWork w(B * beams, V);
   if (!work || ((uintptr_t)work & 15) || work_bytes < w.bytes)
     HI_FAIL("%s: work of %zu bytes (at least %zu, 16-byte aligned)", who, work_bytes, w.bytes);
+  const int64_t places = 4 * (int64_t)B * n;
+  const CallRows rows[] = {{"logits", logits, 2 * (int64_t)ldl, 2 * (int64_t)V, B * beams, false},
+                           call_flat("scores", scores, 4 * (int64_t)B * beams, false), call_flat("best", best, places, true, 1),
+                           call_flat("parent", parent, places, true), call_flat("token", token, places, true),
+                           call_flat("work", work, (int64_t)w.bytes, true)};
+  const char *a0, *a1;
+  if (call_rows_meet(rows, a0, a1)) HI_FAIL("%s: %s and %s must be apart", who, a0, a1);
   if (!hi_device()) return -2;
   const hipStream_t s = (hipStream_t)stream;
   const f16* x = (const f16*)logits;

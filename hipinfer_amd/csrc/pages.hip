@@ -507,11 +507,6 @@ int cache_set(const char* who, void* const* caches, const long long* strides, co
   return 0;
 }
 
-// One of a call's tensors without rows.
-CallRows flat(const char* name, const void* p, int64_t bytes, bool out, int in_place = -1) {
-  return CallRows{name, p, bytes, bytes, 1, out, in_place};
-}
-
 // Checks what both calls have in common; the position shift of a page.
 int pool_check(const char* who, void* const* caches, const long long* strides, const long long* bytes, const int* runs, int n, int page,
                const int* table, int ldt, int W, int S, const int* refs, int pages, const int* table_out, int ldo, const int* refs_out,
@@ -562,11 +557,11 @@ HI_EXPORT int hi_cache_fork(void* const* caches, const long long* strides, const
   if (((uintptr_t)lens | (uintptr_t)parent | (uintptr_t)lens_out | (uintptr_t)missing) & 3)
     HI_FAIL("%s: lens, parent and missing must be 4-byte aligned", who);
   // parent is read in the launch that writes table_out and lens_out, and the rows' blocks run beside each other
-  const CallRows rows[] = {{"table", table, 4 * (int64_t)ldt, 4 * (int64_t)W, S, false}, flat("lens", lens, 4 * (int64_t)S, false),
-                           flat("parent", parent, 4 * (int64_t)N, false), flat("refs", refs, 4 * (int64_t)pages, false),
+  const CallRows rows[] = {{"table", table, 4 * (int64_t)ldt, 4 * (int64_t)W, S, false}, call_flat("lens", lens, 4 * (int64_t)S, false),
+                           call_flat("parent", parent, 4 * (int64_t)N, false), call_flat("refs", refs, 4 * (int64_t)pages, false),
                            {"table_out", table_out, 4 * (int64_t)ldo, 4 * (int64_t)W, N, true},
-                           flat("lens_out", lens_out, 4 * (int64_t)N, true), flat("refs_out", refs_out, 4 * (int64_t)pages, true, 3),
-                           flat("missing", missing, 4, true), flat("work", work, (int64_t)WorkLayout(S, N, pages).bytes, true)};
+                           call_flat("lens_out", lens_out, 4 * (int64_t)N, true), call_flat("refs_out", refs_out, 4 * (int64_t)pages, true, 3),
+                           call_flat("missing", missing, 4, true), call_flat("work", work, (int64_t)WorkLayout(S, N, pages).bytes, true)};
   const char *a0, *a1;
   if (call_rows_meet(rows, a0, a1)) HI_FAIL("%s: %s and %s must be apart", who, a0, a1);
   const HiDevice* d = hi_device();
@@ -603,10 +598,10 @@ HI_EXPORT int hi_cache_compact(void* const* caches, const long long* strides, co
     HI_FAIL("%s: the new table must be the old one (with its row stride) or apart from it", who);
   // moved is read by the blocks that write the new table and counts beside each other
   const int64_t span = 4 * (int64_t)pages;
-  const CallRows rows[] = {{"table", table, 4 * (int64_t)ldt, 4 * (int64_t)W, S, false}, flat("refs", refs, span, false),
-                           {"table_out", table_out, 4 * (int64_t)ldo, 4 * (int64_t)W, S, true, 0}, flat("refs_out", refs_out, span, true, 1),
-                           flat("moved", moved, span, true), flat("used", used, 4, true),
-                           flat("work", work, (int64_t)WorkLayout(S, 0, pages).bytes, true)};
+  const CallRows rows[] = {{"table", table, 4 * (int64_t)ldt, 4 * (int64_t)W, S, false}, call_flat("refs", refs, span, false),
+                           {"table_out", table_out, 4 * (int64_t)ldo, 4 * (int64_t)W, S, true, 0}, call_flat("refs_out", refs_out, span, true, 1),
+                           call_flat("moved", moved, span, true), call_flat("used", used, 4, true),
+                           call_flat("work", work, (int64_t)WorkLayout(S, 0, pages).bytes, true)};
   const char *a0, *a1;
   if (call_rows_meet(rows, a0, a1)) HI_FAIL("%s: %s and %s must be apart", who, a0, a1);
   const HiDevice* d = hi_device();

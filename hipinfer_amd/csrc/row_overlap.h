@@ -35,6 +35,10 @@ struct CallRows {
   bool out;
   int in_place = -1;
 };
+// One without rows.
+inline CallRows call_flat(const char* name, const void* p, int64_t bytes, bool out, int in_place = -1) {
+  return CallRows{name, p, bytes, bytes, 1, out, in_place};
+}
 // Whether two of n tensors meet though the call writes one of them; a and b: which.
 template <int n>
 inline bool call_rows_meet(const CallRows (&t)[n], const char*& a, const char*& b) {

@@ -858,8 +858,8 @@ def beam_select(logits, scores, beams, n=None, out=None, work=None):
     the n (default beams; at most 64) with the best scores, in order: scores[row] fp32 + the token's log-probability.
     The lowest (beam, token) wins a tie; scores closer than 2^-35 (1 + their distance from the best) are one.
 
-    Returns (best [B, n] fp32, parent [B, n] int32, token [B, n] int32), parent the row of logits (cache_fork's parent); with n
-    == beams, best given in `out` may be the scores' memory. A
+    Returns (best [B, n] fp32, parent [B, n] int32, token [B, n] int32), parent the row of logits (cache_fork's parent). Given in
+    `out`, they are apart from each other and from the rest; best may be the scores' memory with n == beams. A
     candidate has no finite score where its logit is -inf, its row's score is not finite (a beam that has ended), or a logit
     of its row is NaN or +inf; nor do those 2^31 or more below the best count. Places without a candidate hold -inf, -1 and -1.
     At most 64 beams, beams * V at most 2^24."""

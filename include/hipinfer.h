@@ -225,8 +225,9 @@ int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long 
  * scores[row] + log-probability, in order: best [B][n] fp32, parent [B][n] (the row of logits), token [B][n]. The lowest
  * (beam, token) wins a tie (scores closer than 2^-35 (1 + their distance from the best)); places without a candidate hold
  * -inf, -1, -1: a logit of -inf, a row whose score is not finite or that holds a NaN or +inf, and what lies 2^31 or more below
- * the best are none. best may be scores itself with n == beams, else is apart from it. beams and n 1 to 64, beams * V <= 2^24, B * beams <= 65535. work: hi_beam_select_work_bytes(...) (0 for
- * bad sizes), 16-byte aligned, no state; launches that share it must not run concurrently. */
+ * the best are none. best may be scores itself with n == beams; otherwise what is written, work too, shares no memory with
+ * anything else of the call. beams and n 1 to 64, beams * V <= 2^24, B * beams <= 65535. work: hi_beam_select_work_bytes(...) (0
+ * for bad sizes), 16-byte aligned, no state; launches that share it must not run concurrently. */
 size_t hi_beam_select_work_bytes(int B, int beams, int V, int n);
 int hi_beam_select(const void* logits, long long ldl, const float* scores, int B, int beams, int V, int n, float* best,
                    int* parent, int* token, void* work, size_t work_bytes, void* stream);

@@ -1,4 +1,4 @@
-"""Which of their tensors the calls of the page pool may find in one memory, on the CPU: the rule for rows of different numbers
+"""Which of their tensors the calls of beam search and of the page pool may find in one memory, on the CPU: the rule for rows of different numbers
 (hipinfer_amd/csrc/row_overlap.h), compiled for the host, against every byte of small cases, and what the C entry points refuse and
 accept. Pointers here are numbers that are never followed; accepted calls end where they find no GPU (-2)."""
 import ctypes
@@ -119,3 +119,35 @@ def test_compact_in_place(capfd):
 ], ids=str)
 def test_compact_accepts(change):
     assert call("hi_cache_compact", COMPACT | change) == -2
+
+
+BEAM = dict(logits=MB, ldl=110, scores=2 * MB, B=2, beams=4, V=100, n=8, best=3 * MB, parent=4 * MB, token=5 * MB, work=6 * MB,
+            work_bytes=1 << 16, stream=None)
+BEAM_READ = ("logits", "scores")
+BEAM_WRITTEN = ("best", "parent", "token", "work")
+
+
+@pytest.mark.parametrize("out", BEAM_WRITTEN)
+@pytest.mark.parametrize("other", BEAM_READ + BEAM_WRITTEN)
+def test_beam_select(out, other, capfd):
+    """One sequence's block writes its places while others still read their logits and scores."""
+    if out == other or (other, out) == ("scores", "best"):
+        return
+    refused("hi_beam_select", BEAM | {out: BEAM[other]}, (other, out), capfd)
+    if out != "work":
+        refused("hi_beam_select", BEAM | {out: BEAM[other] + 28}, (other, out), capfd)
+
+
+@pytest.mark.parametrize("out", ["parent", "token"])
+def test_beam_select_in_place(out, capfd):
+    """With best in the scores' place, the other outputs are as little allowed there."""
+    refused("hi_beam_select", BEAM | {"n": 4, "best": 2 * MB, out: 2 * MB}, ("scores", out), capfd)
+
+
+@accepted
+@pytest.mark.parametrize("change", [
+    {}, dict(n=4, best=2 * MB), dict(best=2 * MB + 32), dict(parent=2 * MB + 32), dict(token=MB + 8 * 220),  # behind scores and logits
+    dict(B=1, beams=1, n=5, token=MB + 200),  # one row ends with its logits, whatever its stride
+], ids=str)
+def test_beam_select_accepts(change):
+    assert call("hi_beam_select", BEAM | change) == -2
