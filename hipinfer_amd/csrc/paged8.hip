@@ -3,9 +3,12 @@
 //
 // An element's value is its e4m3 code times 2^k with one k per page and kv head, of K and of V apart. e4m3 has 4 significant bits at
 // any magnitude, so an exponent as good as any other scale costs a byte a page, and a power of two makes both directions exact but
-// for the one rounding to 4 bits: a page whose k grows with later positions re-rounds nothing (codes move down by whole binary
-// orders; only what falls below 2^-6 of the new scale, 2^-15 of the page's largest value, loses bits), and the attention
-// kernels' fp16 operands are the stored values themselves.
+// for the one rounding to 4 bits. Where a page's k grows with later positions, codes move down by whole binary orders: exactly, but
+// those that come below 2^-6 * 2^k (2^-13 of the page's largest value at most) become subnormal codes and are rounded again, to steps
+// of 2^-9 * 2^k, at every growth, so that such small values depend on which rows came in one call. A stored value is off by less
+// than 2^-4 of it + 2^-9 * 2^k in all: half steps of exponents that grow add up to less than twice the last one's.
+//
+// The attention kernels' fp16 operands are the stored values; those below 2^-21 are rounded to fp16's least steps, 2^-24.
 #include "paged_attn.h"
 
 namespace {

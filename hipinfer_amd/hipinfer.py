@@ -549,8 +549,9 @@ def rope_cache_paged8(qkv, Hq, Hkv, cs, kp, vp, kexp, vexp, table, pos, start=No
     The exponent of a page and head is the least k of -32 to 8 that holds every value |x| <= 448 * 2^k written to its positions
     so far (a page's first position, when written, begins anew); each value is rounded once, to the nearest of 4 significant
     bits, k after its rotation without a rounding to fp16 before. Where k grows, the page's earlier positions are moved
-    to it, which loses only bits below 2^-15 of the page's largest value. Values beyond +-61440 (infinities too) become that, NaN
-    stays NaN.
+    to it: exactly, but those below 2^-6 * 2^k (2^-13 of the page's largest value at most) are rounded again, to steps of 2^-9 * 2^k,
+    and so depend on which rows came in one call. A stored value is off by less than 2^-4 |x| + 2^-9 * 2^k. Values beyond +-61440
+    (infinities too) become that, NaN stays NaN.
 
     Rows append: positions of a page behind the last one written are not kept, and every page that a call writes belongs to one
     sequence. A row that has no place is left out, its q too, as in rope_cache_paged."""

@@ -199,8 +199,9 @@ int hi_attn_paged(const void* q, int ldq, const void* kp, const void* vp, long l
  * vexp [pages][Hkv] int8, a value code * 2^exponent, as fp16.
  * hi_rope_cache_paged8's rows are hi_attn_paged's: start NULL, row b at pos[b] of sequence b (M == B), else runs of rows. The
  * exponent of a page and head is the least of -32 .. 8 with |x| <= 448 * 2^k for the values written to its positions so far (writing
- * a page's first position begins anew); values are rounded once, to nearest, k as fp32 after its rotation. Where it grows, the
- * page's earlier positions are moved to it. Beyond +-61440 values become that, NaN stays NaN. Rows append: positions of a page behind
+ * a page's first position begins anew); values are rounded to nearest, k as fp32 after its rotation. Where it grows, the
+ * page's earlier positions are moved to it: exactly, but those below 2^-6 * 2^k are rounded again. A stored value is off by less
+ * than 2^-4 |x| + 2^-9 * 2^k, k the page's last. Beyond +-61440 values become that, NaN stays NaN. Rows append: positions of a page behind
  * the last one written are not kept, and a page that is written belongs to one sequence. */
 int hi_rope_cache_paged8(void* qkv, int ldq, void* q_out, int ldqo, int M, int Hq, int Hkv, int D, const void* cs,
                          int cs_rows, int cs_f32, int rot, int interleaved, const int* start, const int* pos, void* kp,
