@@ -7,9 +7,11 @@
 // candidate outside them has n segments, so n candidates, before it. So a second kernel, a block per sequence, joins the sums,
 // picks n segments, and reads those again: 512 n logits instead of beams * vocabulary.
 //
-// Exponentials and a lane's sum of 32 are fp32 (relative to the lane's own maximum), joined in 64 bits; scores are compared in 64
-// bits, as keys of 64 bits: 40 bits of the distance d from the best (of 1 + d, 2^-35 of it), then the place, so that a key is unique
-// and the lowest (beam, token) wins a tie.
+// Exponentials are fp32, and so are their sums within a wave's 2048 logits (a lane's 32 relative to the lane's own maximum, then over
+// the lanes); a row's waves are joined in 64 bits. That leaves a row's log sum off by 2^-17 at most, a small part of what the fp16
+// logits are rounded by, and candidates of different rows that are nearer to each other may come in either order. Computed scores
+// are compared by keys of 64 bits: 40 bits of the distance d from the best (of 1 + d, 2^-35 of it), then the place, so that a key is
+// unique and the lowest (beam, token) wins a tie.
 #include "hi_common.h"
 #include "row_overlap.h"
 

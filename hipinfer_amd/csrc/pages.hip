@@ -5,7 +5,7 @@
 // Both are a plan by one block and a launch that carries it out on the whole GPU. What a plan has to find is small (which pages are
 // free, in order) but global: 4 bytes a page, read by 1024 threads, 16 pages each at a time. Everything is found on the device, so
 // both can be captured; results do not depend on the order of blocks: pages are handed out in ascending order to rows in ascending
-// order, and the only atomics add integers.
+// order, and the only atomics are sums and minima of integers.
 #include <climits>
 
 #include "hi_common.h"
@@ -20,7 +20,9 @@ constexpr int kMaxRows = 8192;      // rows of a table: the plan keeps 12 bytes 
 constexpr int kSetMax = 128;        // cache tensors of one launch: their addresses are kernel arguments (3 KB)
 constexpr int kPart = 4096;         // bytes of a page that a wave copies at a time: 4 loads of 16 bytes a lane
 constexpr int kSmall = 64;          // pages of at most so many bytes are copied by a lane
-constexpr int kListed = 4096;       // free pages that a plan keeps in LDS
+constexpr int kListed = 4096;       // free pages that a fork's plan keeps there
+constexpr size_t fork_lds(int S, int N) { return (2 * (size_t)S + 2 * (size_t)N + kListed) * 4; }
+static_assert(fork_lds(kMaxRows, kMaxRows) + kPlanThreads / 64 * 8 <= 160 * 1024, "a fork's plan and its sums fit a CU's LDS");
 
 // One cache tensor: pages `stride` bytes apart. A page's `bytes` are `runs` runs of one value per position, or with runs 0
 // belong to the page as a whole.
@@ -570,7 +572,7 @@ HI_EXPORT int hi_cache_fork(void* const* caches, const long long* strides, const
   const ForkArgs a{table, lens, parent, refs, table_out, lens_out, refs_out, missing, (char*)work, ldt, ldo, W, S, N, pages, grow,
                    page, shift};
   const int copiers = refs == refs_out ? 0 : min(d->cus, (pages + kPlanThreads - 1) / kPlanThreads);
-  const size_t lds = (size_t)(2 * S + 2 * N + kListed) * 4;
+  const size_t lds = fork_lds(S, N);
   if (lds > 48 * 1024 && hi_blocks_per_cu(reinterpret_cast<const void*>(fork_plan_kernel), kPlanThreads, lds) < 1) return -2;
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), lds, s, a);
   HI_TRY(hipGetLastError());

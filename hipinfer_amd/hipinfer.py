@@ -857,7 +857,9 @@ def beam_select_work(seqs, beams, V, n):
 def beam_select(logits, scores, beams, n=None, out=None, work=None):
     """Beam search's selection: of every sequence's candidates, its `beams` rows of logits [B * beams, V] fp16 by their V tokens,
     the n (default beams; at most 64) with the best scores, in order: scores[row] fp32 + the token's log-probability.
-    The lowest (beam, token) wins a tie; scores closer than 2^-35 (1 + their distance from the best) are one.
+    A row's log sum is computed to 2^-17: candidates of different rows that are nearer than that may come in either order. Of
+    computed scores the lowest (beam, token) wins a tie, their distances from the best taken in steps of 2^-35 (1 + distance).
+    Scores may be of any size: what is compared are their differences.
 
     Returns (best [B, n] fp32, parent [B, n] int32, token [B, n] int32), parent the row of logits (cache_fork's parent). Given in
     `out`, they are apart from each other and from the rest; best may be the scores' memory with n == beams. A

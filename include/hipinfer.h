@@ -223,8 +223,10 @@ int hi_attn_shared(const void* q, int ldq, const void* kp, const void* vp, long 
 
 /* ---- beam search over a pool of pages. No counterpart in the reference.
  * Selection: of each of B sequences' candidates, `beams` rows of logits [B * beams, ldl] fp16 by V tokens, the n with the best
- * scores[row] + log-probability, in order: best [B][n] fp32, parent [B][n] (the row of logits), token [B][n]. The lowest
- * (beam, token) wins a tie (scores closer than 2^-35 (1 + their distance from the best)); places without a candidate hold
+ * scores[row] + log-probability, in order: best [B][n] fp32, parent [B][n] (the row of logits), token [B][n]. A row's log sum is
+ * computed to 2^-17 (candidates of different rows nearer than that may come in either order), and best is rounded to fp32; what is
+ * compared are differences of scores, whose size takes nothing from the order. The lowest (beam, token) wins a tie of computed
+ * scores (their distances from the best in steps of 2^-35 (1 + distance)); places without a candidate hold
  * -inf, -1, -1: a logit of -inf, a row whose score is not finite or that holds a NaN or +inf, and what lies 2^31 or more below
  * the best are none. best may be scores itself with n == beams; otherwise what is written, work too, shares no memory with
  * anything else of the call. beams and n 1 to 64, beams * V <= 2^24, B * beams <= 65535. work: hi_beam_select_work_bytes(...) (0
