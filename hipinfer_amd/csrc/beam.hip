@@ -178,7 +178,7 @@ __device__ __forceinline__ void least_keys(PickSmem& sh, int n, Push push, All a
 //  * of the segments, those up to the n-th least of 64 groups' least distances (at least n segments are that near);
 //  * of their logits, those up to the n-th segment's best one (the segments' best ones are n that near).
 // What bounds it: a chain of some ten waits (sums and segments from memory, exp and log in 64 bits, two rankings, the picked logits from
-// memory): 7.3 us for 4 beams, 9.2 for 32 times 8 (with 64-bit keys for every segment and logit, in blocks of 256: 16.8 and 27.8).
+// memory): 7.5 us for 4 beams, 8.8 for 32 times 8 (with 64-bit keys for every segment and logit, in blocks of 256: 16.8 and 27.8).
 template <bool WIDE>
 __global__ void __launch_bounds__(kPick) beam_pick_kernel(const f16* __restrict__ logits, int64_t ldl, const float* __restrict__ scores,
                                                           int V, int R, int K, int n, const char* work, float* best, int* parent,

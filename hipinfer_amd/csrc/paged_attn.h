@@ -318,7 +318,8 @@ __device__ __forceinline__ void pages_block(const AttnArgs& a, const C& c, const
     // F8: a wave's share of a tile comes as codes (a group of 8 keys is D / 2 lanes of DMA) and is made into fp16 by the wave itself,
     // one tile before the others read it: no barrier more, and no registers held from tile to tile. The codes' place in LDS is free
     // again as soon as they are read, and the next tile's are sent for. One chunk goes behind each MFMA of the last block's P.V
-    // (2048 rows behind 4096 positions, Hq 32, Hkv 8, D 128: 190.8 us, all of them after those MFMAs 196.7; the fp16 cache 184).
+    // (2048 rows behind 4096 positions, Hq 32, Hkv 8, D 128: 190 to 195 us by card, with all of them after those MFMAs 3 % more on
+    // one card; the fp16 cache 184).
     constexpr int RPW = KPW * D / 1024;  // 16-byte reads of a lane per wave and operand, 2 chunks each
     int vexps = 0;  // the exponents of the V tile that lies there as codes; the K tile's are ke
     u32x4* const own_k = fp_smem + 2 * kFpStages * Sm::kTile + wave * RPW * 64;

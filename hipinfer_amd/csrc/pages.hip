@@ -16,7 +16,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPerThread = 16;      // pages that a thread of a plan looks at in one step
 constexpr int kMaxPages = 1 << 30;  // of a pool
-constexpr int kMaxRows = 8192;      // rows of a table: the plan keeps 12 bytes a row in LDS
+constexpr int kMaxRows = 8192;      // rows of a table: a fork's plan keeps 8 bytes of each old row and of each new one in LDS
 constexpr int kSetMax = 128;        // cache tensors of one launch: their addresses are kernel arguments (3 KB)
 constexpr int kPart = 4096;         // bytes of a page that a wave copies at a time: 4 loads of 16 bytes a lane
 constexpr int kSmall = 64;          // pages of at most so many bytes are copied by a lane
@@ -121,8 +121,8 @@ struct ForkArgs {
 // Block 0 plans; the others, where the counts are not updated in place, copy them.
 // A row's pages: entries below `full` (whole pages) are its parent's, shared. Of those from there on up to `need`, a parent's first
 // child keeps the pages that nobody else holds; every other is a fresh page, noted as -2 - its rank among the row's.
-// What bounds it: four loads one after the other (parent, length, entry, count) and the search for free pages: 6.3 us for 4 rows, 7.8 for
-// 256.
+// What bounds it: four loads one after the other (parent, length, entry, count) and the search for free pages: 6.3 to 6.8 us for 4 rows,
+// 7.8 to 8.7 for 256, by card.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(ForkArgs a) {
   extern __shared__ int lds[];
   __shared__ int64_t sh[kPlanThreads / 64];

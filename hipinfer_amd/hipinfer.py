@@ -547,7 +547,7 @@ def rope_cache_paged8(qkv, Hq, Hkv, cs, kp, vp, kexp, vexp, table, pos, start=No
     int32 rows start[b] .. start[b + 1] - 1 are sequence b's, at positions pos[b], pos[b] + 1, ... (start does not decrease).
 
     The exponent of a page and head is the least k of -32 to 8 that holds every value |x| <= 448 * 2^k written to its positions
-    so far (a page's first position, when written, begins anew); each value is rounded once, to the nearest of 4 significant
+    so far (a page's first position, when written, begins anew); each value is rounded to the nearest of 4 significant
     bits, k after its rotation without a rounding to fp16 before. Where k grows, the page's earlier positions are moved
     to it: exactly, but those below 2^-6 * 2^k (2^-13 of the page's largest value at most) are rounded again, to steps of 2^-9 * 2^k,
     and so depend on which rows came in one call. A stored value is off by less than 2^-4 |x| + 2^-9 * 2^k. Values beyond +-61440
@@ -774,8 +774,8 @@ def _pool_args(what, caches, gpu, table, refs, refs_out, work):
 def cache_fork(caches, table, lens, parent, refs, grow=0, table_out=None, lens_out=None, refs_out=None, missing=None,
                work=None):
     """Makes N new rows of a page table [S, W], row i the continuation of row parent[i]: the same lens[parent[i]] positions, and
-    pages for `grow` more. Beams after beam_select, several answers to one prompt, sequences that begin (a parent of length 0)
-    or end (a parent that is no row, as -1: an empty row).
+    pages for `grow` more, as far as W entries reach. Beams after beam_select, several answers to one prompt, sequences that begin
+    (a parent of length 0) or end (a parent that is no row, as -1: an empty row).
 
     refs [pages] int32 counts who holds a page: a table row that names it counts 1, 0 is free; pages that the caller keeps for
     itself (a cached prompt) count 1 more. Whole pages are shared with the parent. Of the entries behind them the parent's first

@@ -238,11 +238,11 @@ int hi_beam_select(const void* logits, long long ldl, const float* scores, int B
  * state; launches that share it must not run concurrently. */
 size_t hi_cache_work_bytes(int S, int N, int pages);
 /* N new table rows, row i the continuation of row parent[i] of table [S, ldt] (W entries, pages of `page` positions): lens_out[i] =
- * lens[parent[i]] positions and pages for `grow` more; a parent outside [0, S) gives an empty row. refs [pages] counts a
- * page's holders (table entries, and the caller's own), 0 is free. Whole pages are shared; of the entries behind them the first child
- * keeps those pages whose count is 1, others get free pages (lowest first, in the order of rows and entries; -1, counted in
- * `missing` if not NULL, when there are none) and the positions held of a part-filled page are copied. refs_out (refs itself,
- * or apart) has the new counts; pages that they free are handed out by later calls.
+ * lens[parent[i]] positions and pages for `grow` more, as far as W entries reach; a parent outside [0, S) gives an empty row. refs
+ * [pages] counts a page's holders (table entries, and the caller's own), 0 is free. Whole pages are shared; of the entries behind
+ * them the first child keeps those pages whose count is 1, others get free pages (lowest first, in the order of rows and entries;
+ * -1, counted in `missing` if not NULL, when there are none) and the positions held of a part-filled page are copied. refs_out
+ * (refs itself, or apart) has the new counts; pages that they free are handed out by later calls.
  * The n cache tensors (host arrays): caches[t] with pages strides[t] bytes apart, bytes[t] per page, which are runs[t] runs of
  * `page` positions (heads), or with runs[t] 0 are copied whole. table_out, lens_out, missing and work share no memory with each
  * other or with anything else of the call (rows of tables may alternate in one buffer). S, N <= 8192. */
