@@ -26,7 +26,7 @@ inline bool in_place_or_apart(const void* x, int64_t lx, int64_t wx, const void*
 }
 
 // A tensor of a call: m rows of w bytes, ld apart (none where p is null or m or w 0); whether the call writes it, and if it may take
-// the place of one that the call reads, the number of that (their meeting is in_place_or_apart's to judge).
+// the place of one that the call reads, the number of that (whether those two may meet is in_place_or_apart's).
 struct CallRows {
   const char* name;
   const void* p;
